@@ -531,6 +531,107 @@ int spx_layer_backward_sizes(const spx_layer_dims* dims, size_t* workspace_bytes
 int spx_layer_backward(const spx_layer_dims* dims, const spx_packed_weights* weights, const uint16_t* hidden,
                        const spx_layer_grads* grads, void* workspace, void* stream);
 
+/* ---- the token half of a block
+ * Operators between two channel mixers.  The reference's token mixers
+ * (attention/, KDA and MLA) and its block's residual stream
+ * (modeling.py:246-302) are where a user needs them; none is a restatement of
+ * one of its modules.  All take device pointers and `stream`, allocate
+ * nothing and do not synchronise.
+ *
+ * spx_add_rmsnorm_rows: h = hidden + residual, stored in the residual's type
+ *   (residual_f32: FP32, else BF16), and RMSNorm of h as stored, rounded once:
+ *   y = h * w / sqrt(mean(h^2) + eps).  Either `normed` (BF16 [rows, d]) or
+ *   mx_values / mx_scales (E4M3 [rows, d] and E8M0 [rows, d / 32], the layout
+ *   of spx_mxfp8_quantize_rows, quantised from the FP32 result; d % 32 == 0).
+ *   residual NULL: h = hidden, `sum` unused.  Row strides in elements; `sum`
+ *   may be the residual itself when its rows are contiguous.  d % 8 == 0,
+ *   d <= 16384; 16-byte aligned rows.
+ * spx_add_rmsnorm_backward: gradients from d_normed and d_sum (in the
+ *   residual's type; NULL = zero), given h: d_hidden (BF16), d_residual (FP32;
+ *   NULL for a BF16 residual, whose gradient d_hidden is) and d_weight (BF16
+ *   [d]; NULL = not computed).  workspace: spx_add_rmsnorm_backward_workspace
+ *   bytes, not initialised.  Deterministic. */
+int spx_add_rmsnorm_rows(const uint16_t* hidden, int64_t ld_hidden, const void* residual, int64_t ld_residual,
+                         int32_t residual_f32, const uint16_t* norm_weight, float eps, int64_t rows, int32_t d,
+                         void* sum, uint16_t* normed, uint8_t* mx_values, uint8_t* mx_scales, void* stream);
+size_t spx_add_rmsnorm_backward_workspace(int64_t rows, int32_t d);
+int spx_add_rmsnorm_backward(const void* sum, int64_t ld_sum, int32_t residual_f32, const uint16_t* norm_weight,
+                             float eps, const uint16_t* d_normed, int64_t ld_d_normed, const void* d_sum,
+                             int64_t ld_d_sum, int64_t rows, int32_t d, uint16_t* d_hidden, float* d_residual,
+                             uint16_t* d_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Heads of BF16 vectors: element [b, t, h, i] at ptr[b * batch_stride +
+ * t * token_stride + h * head_stride + i] (a view of a fused projection, say). */
+typedef struct spx_heads {
+  const uint16_t* ptr;
+  int64_t batch_stride, token_stride, head_stride;
+} spx_heads;
+
+/* Rotary positions: pair p of every query and key head of token t turns by
+ * positions[t % position_period] * frequencies[p] radians and is scaled by
+ * `factor`; pairs are (p, p + pairs) of the head, or (2p, 2p + 1) when
+ * interleaved; elements from 2 * pairs on are copied.  inverse = 1 turns back
+ * (the gradient).  frequencies: FP64 [pairs]; positions int32, or int64
+ * (positions_64).  q or k may be empty (heads 0).  Outputs are contiguous
+ * [tokens, heads, head_dim].  head_dim <= 4096, 2 * pairs <= head_dim; 16-byte
+ * aligned heads with head_dim % 8 == 0 and whole 16-byte halves take vector
+ * loads, all others run element by element. */
+int spx_rotary(const spx_heads* q, int32_t q_heads, const spx_heads* k, int32_t k_heads, int64_t tokens,
+               int32_t head_dim, int32_t pairs, const void* positions, int32_t positions_64, int64_t position_period,
+               const double* frequencies, float factor, int32_t interleaved, int32_t inverse, uint16_t* q_out,
+               uint16_t* k_out, void* stream);
+
+/* Linear attention with a decay per query head.  Per sequence and head, with
+ * the state S [key_dim, value_dim] (FP32, from initial_state or zero):
+ *   S_t = exp(decay_t) S_{t-1} + k_t v_t^T,   out_t = scale * S_t^T q_t.
+ * Decays are natural logarithms, FP32 or BF16 (decay_f32), meant to be <= 0;
+ * a factor below 2^-126 is zero.  Query head h uses key/value head
+ * h / (heads / kv_heads).  packed = 0: `batch` sequences of seq_len tokens;
+ * packed = 1: one batch row of seq_len tokens in all, cut into `batch`
+ * sequences by cu_seqlens (int32 [batch + 1] on the device, from 0 to
+ * seq_len, not decreasing; an entry that is not is recorded in *status and
+ * its sequence skipped).  States are FP32 [batch, heads, key_dim, value_dim].
+ * key_dim and value_dim: multiples of 8 up to 128; heads 16-byte aligned.
+ * status: device int, zero before the first call (NULL = not recorded);
+ * workspace 16-byte aligned, not initialised, sized by the functions below. */
+typedef struct spx_linattn_dims {
+  int64_t batch, seq_len;
+  int32_t heads, kv_heads, key_dim, value_dim;
+  int32_t packed, decay_f32;
+  float scale; /* not 0 */
+} spx_linattn_dims;
+typedef struct spx_decays {
+  const void* ptr; /* [b, t, h] */
+  int64_t batch_stride, token_stride, head_stride;
+} spx_decays;
+
+size_t spx_linear_attention_workspace(const spx_linattn_dims* dims);
+/* out: BF16 [batch, seq_len, heads, value_dim] contiguous; final_state may be NULL. */
+int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const spx_heads* k, const spx_heads* v,
+                         const spx_decays* decays, const int32_t* cu_seqlens, const float* initial_state,
+                         uint16_t* out, float* final_state, void* workspace, size_t workspace_bytes, int* status,
+                         void* stream);
+/* Gradients from d_out and d_final_state (NULL = zero) of everything the
+ * forward read: d_q, d_k, d_v (BF16, contiguous, the shapes of q, k, v; shared
+ * heads sum over their query heads in FP32), d_decay (the decays' type,
+ * contiguous [batch, seq_len, heads]) and d_initial_state (NULL = not
+ * computed).  Nothing but the forward's inputs is needed.  Deterministic. */
+size_t spx_linear_attention_backward_workspace(const spx_linattn_dims* dims);
+int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads* q, const spx_heads* k,
+                                  const spx_heads* v, const spx_decays* decays, const int32_t* cu_seqlens,
+                                  const float* initial_state, const spx_heads* d_out, const float* d_final_state,
+                                  uint16_t* d_q, uint16_t* d_k, uint16_t* d_v, void* d_decay, float* d_initial_state,
+                                  void* workspace, size_t workspace_bytes, int* status, void* stream);
+/* One token of `batch` requests against a cache of states [slots, heads,
+ * key_dim, value_dim], updated in place: request i's state is slot_index[i]
+ * (int64; NULL = i).  An index outside [0, slots) is an empty row: zeros out,
+ * no state touched.  Indexes of one call must differ.  The heads' token_stride
+ * is not used; out is contiguous [batch, heads, value_dim]. */
+int spx_linear_attention_step(const spx_heads* q, const spx_heads* k, const spx_heads* v, const spx_decays* decays,
+                              int32_t decay_f32, int64_t batch, int32_t heads, int32_t kv_heads, int32_t key_dim,
+                              int32_t value_dim, float scale, float* state, int64_t slots, const int64_t* slot_index,
+                              uint16_t* out, void* stream);
+
 /* spx_dispatch without a workspace: same outputs, no device allocation by
  * anyone.  No counterpart in the reference; it exists for callers that cannot
  * allocate device memory (an FFI client holding only the buffers it was

@@ -22,6 +22,15 @@ from spalmer_b200.experts import (
     rms_norm,
     route,
 )
+from spalmer_b200.token_ops import (
+    add_rms_norm,
+    add_rms_norm_mxfp8,
+    linear_attention,
+    linear_attention_status,
+    linear_attention_step,
+    rotary_embed,
+    rotary_frequencies,
+)
 
 __all__ = [
     "B200ChannelBlock",
@@ -36,7 +45,14 @@ __all__ = [
     "RMSNorm",
     "SurpriseRouter",
     "SwiGLU",
+    "add_rms_norm",
+    "add_rms_norm_mxfp8",
     "dispatch",
+    "linear_attention",
+    "linear_attention_status",
+    "linear_attention_step",
     "rms_norm",
+    "rotary_embed",
+    "rotary_frequencies",
     "route",
 ]

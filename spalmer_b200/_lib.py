@@ -76,6 +76,15 @@ EXPORTED = (
     "spx_router_sizes",
     "spx_router_forward",
     "spx_dispatch_static_status",
+    "spx_add_rmsnorm_rows",
+    "spx_add_rmsnorm_backward_workspace",
+    "spx_add_rmsnorm_backward",
+    "spx_rotary",
+    "spx_linear_attention_workspace",
+    "spx_linear_attention",
+    "spx_linear_attention_backward_workspace",
+    "spx_linear_attention_backward",
+    "spx_linear_attention_step",
 )
 
 ABI_VERSION = 12
@@ -196,6 +205,33 @@ class LayerGrads(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [
+        ("ptr", _vp),
+        ("batch_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class Decays(ctypes.Structure):
+    _fields_ = Heads._fields_
+
+
+class LinAttnDims(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("seq_len", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("key_dim", ctypes.c_int32),
+        ("value_dim", ctypes.c_int32),
+        ("packed", ctypes.c_int32),
+        ("decay_f32", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 STAGE_EVENTS = 8
 STAGE_NAMES = ("router_gemm", "route_topk", "dispatch", "expert_gemm1_swiglu", "expert_gemm2_scatter",
                "shared_gemm1_swiglu", "shared_gemm2_combine")
@@ -311,6 +347,39 @@ def load() -> ctypes.CDLL:
         "spx_nvfp4_mm_nt": (
             ctypes.c_int,
             [_vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp],
+        ),
+        "spx_add_rmsnorm_rows": (
+            ctypes.c_int,
+            [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int32, _vp, ctypes.c_float, ctypes.c_int64,
+             ctypes.c_int32, _vp, _vp, _vp, _vp, _vp],
+        ),
+        "spx_add_rmsnorm_backward_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+        "spx_add_rmsnorm_backward": (
+            ctypes.c_int,
+            [_vp, ctypes.c_int64, ctypes.c_int32, _vp, ctypes.c_float, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+             ctypes.c_int64, ctypes.c_int32, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+        ),
+        "spx_rotary": (
+            ctypes.c_int,
+            [P(Heads), ctypes.c_int32, P(Heads), ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _vp,
+             ctypes.c_int32, ctypes.c_int64, _vp, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp],
+        ),
+        "spx_linear_attention_workspace": (ctypes.c_size_t, [P(LinAttnDims)]),
+        "spx_linear_attention": (
+            ctypes.c_int,
+            [P(LinAttnDims), P(Heads), P(Heads), P(Heads), P(Decays), _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp,
+             _vp],
+        ),
+        "spx_linear_attention_backward_workspace": (ctypes.c_size_t, [P(LinAttnDims)]),
+        "spx_linear_attention_backward": (
+            ctypes.c_int,
+            [P(LinAttnDims), P(Heads), P(Heads), P(Heads), P(Decays), _vp, _vp, P(Heads), _vp, _vp, _vp, _vp, _vp,
+             _vp, _vp, ctypes.c_size_t, _vp, _vp],
+        ),
+        "spx_linear_attention_step": (
+            ctypes.c_int,
+            [P(Heads), P(Heads), P(Heads), P(Decays), ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+             ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _vp, ctypes.c_int64, _vp, _vp, _vp],
         ),
         "spx_mxfp8_mm_nt": (
             ctypes.c_int,

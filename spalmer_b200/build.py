@@ -17,7 +17,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 TARGET = HERE / "libspx.so"
-SOURCES = ("abi.cu", "gemm.cu", "route.cu", "dispatch.cu", "pack.cu", "dispatch_static.cu", "launch.cu", "mxfp8.cu", "calibration.cu", "backward.cu", "block.cu", "paged.cu", "nvfp4.cu", "peer.cu", "gemv.cu", "quant_error.cu", "wgrad.cu")
+SOURCES = ("abi.cu", "gemm.cu", "route.cu", "dispatch.cu", "pack.cu", "dispatch_static.cu", "launch.cu", "mxfp8.cu", "calibration.cu", "backward.cu", "block.cu", "paged.cu", "nvfp4.cu", "peer.cu", "gemv.cu", "quant_error.cu", "wgrad.cu", "add_norm.cu", "rotary.cu", "linear_step.cu", "linear_recurrent.cu", "linear_chunk.cu", "token_abi.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1243,6 +1243,29 @@ int encode_3d(CUtensorMap* map, const void* base, int64_t groups, int64_t rows, 
   return r == CUDA_SUCCESS ? SPX_OK : SPX_ERR_DRIVER;
 }
 
+// BF16 heads [batch][tokens][heads][d] with element strides: boxes of 64
+// elements of one head over box_tokens tokens, 128B swizzle, zero outside.
+int encode_heads(CUtensorMap* map, const void* base, int64_t d, int64_t heads, int64_t tokens, int64_t batch,
+                 int64_t head_stride, int64_t token_stride, int64_t batch_stride, int box_tokens) {
+  if (int rc = get_encoder(); rc != SPX_OK) return rc;
+  const int64_t extent[3] = {heads, tokens, batch}, stride[3] = {head_stride, token_stride, batch_stride};
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens),
+                        static_cast<cuuint64_t>(batch)};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (extent[i] > 1 && stride[i] <= 0) return SPX_ERR_UNSUPPORTED;  // a broadcast dimension
+    // the stride of a dimension of one element is not used, but it has to be a valid one
+    strides[i] = static_cast<cuuint64_t>(extent[i] > 1 ? stride[i] * 2 : 128);
+  }
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return SPX_ERR_ALIGNMENT;
+  cuuint32_t box[4] = {64u, 1u, static_cast<cuuint32_t>(box_tokens), 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SPX_OK : SPX_ERR_DRIVER;
+}
+
 size_t gemm_smem_bytes(int bn, int stages, bool mx, int epi, bool nv) {
   const size_t per_stage =
       kTileRows * 128 + static_cast<size_t>(bn) * 128 + (mx ? (nv ? kNvStageSfBytes : kMxStageSfBytes) : 0);

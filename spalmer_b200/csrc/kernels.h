@@ -241,6 +241,8 @@ int encode_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, in
               int elem_bytes = 2);
 int encode_3d(CUtensorMap* map, const void* base, int64_t groups, int64_t rows, int64_t cols, int box_rows,
               int elem_bytes = 2);
+int encode_heads(CUtensorMap* map, const void* base, int64_t d, int64_t heads, int64_t tokens, int64_t batch,
+                 int64_t head_stride, int64_t token_stride, int64_t batch_stride, int box_tokens);
 size_t gemm_smem_bytes(int bn, int stages, bool mx, int epi, bool nv = false);
 int gemm_pick_stages(int bn, int k_blocks, bool mx, int epi, bool nv = false);
 // `mx` selects the block-scaled MXFP8 kernel (bn <= 128, k_blocks of 128 elements).
@@ -472,5 +474,116 @@ int launch_bwd_swiglu(const uint16_t* gu, int ld_gu, int c, const uint16_t* dhp,
                       const uint16_t* sorted_w, const int* order, int64_t P, int I, int kI, uint16_t* h_sorted,
                       uint16_t* dgu, float* dw_pair, cudaStream_t stream);
 int launch_bwd_router(const BwdRouterArgs& a, cudaStream_t stream);
+
+// Residual addition + RMSNorm of BF16 rows (add_norm.cu).
+struct AddNormArgs {
+  const uint16_t* x;      // [rows, d], row stride ld_x
+  const void* res;        // [rows, d] BF16 / FP32, row stride ld_res | null
+  const uint16_t* w;      // [d]
+  void* sum;              // [rows, d] in res's type (null without res)
+  uint16_t* y;            // [rows, d] BF16, or
+  uint8_t* mx_values;     // [rows, d] E4M3 and
+  uint8_t* mx_scales;     // [rows, d / 32] E8M0
+  int64_t rows, ld_x, ld_res;
+  int d;
+  int res_f32;
+  float eps;
+};
+struct AddNormBackwardArgs {
+  const void* h;          // [rows, d] the forward's sum (BF16 / FP32), row stride ld_h
+  const uint16_t* w;      // [d]
+  const uint16_t* dy;     // [rows, d], row stride ld_dy
+  const void* dsum;       // [rows, d] in h's type, row stride ld_dsum | null
+  uint16_t* dx;           // [rows, d] BF16
+  float* dres;            // [rows, d] FP32 | null (BF16 residual: dx is its gradient too)
+  float* dw_part;         // [add_norm_backward_parts, d] | null
+  int64_t rows, ld_h, ld_dy, ld_dsum;
+  int d;
+  int res_f32;
+  float eps;
+};
+constexpr int kNormMaxD = 16384;
+int add_norm_backward_parts(int64_t rows, int d);
+int launch_add_norm(const AddNormArgs& a, cudaStream_t stream);
+int launch_add_norm_backward(const AddNormBackwardArgs& a, uint16_t* dw, cudaStream_t stream);
+
+// Rotary positions (rotary.cu).
+struct RotaryArgs {
+  const uint16_t *q, *k;      // [tokens][heads][d], element strides below | null
+  uint16_t *q_out, *k_out;    // contiguous
+  const void* pos;            // [pos_period] int32 / int64: token t is at pos[t % pos_period]
+  const double* freq;         // [pairs] radians per position
+  int64_t tokens, pos_period;
+  int64_t q_st, q_sh, k_st, k_sh;
+  int heads_q, heads_k, d, pairs;
+  int pos64, interleaved, inverse;
+  float factor;
+  int tokens_per_cta;         // set by launch_rotary
+};
+constexpr int kRotMaxD = 4096;
+int launch_rotary(RotaryArgs a, cudaStream_t stream);
+
+// Linear attention with a decay per head (linear_step.cu, linear_recurrent.cu).
+// One job computes, over each sequence and query head,
+//   out_i = scale * sum_j exp(decay between j and i) (a_i . b_j) c_j
+// over the j up to i (or, reverse, from i on), carrying a state [da][dc] =
+// the decayed sum of b_j c_j^T.  The forward pass is one job (a, b, c) =
+// (q, k, v); the gradients are three: dq = (do, v, k), dk = (v, do, q)
+// reverse, dv = (k, q, do) reverse.
+struct LaOperand {
+  const uint16_t* p;
+  int64_t sb, st, sh;  // element strides of batch, token, head
+  int group;           // query heads that share one head of this tensor
+};
+struct LaJob {
+  LaOperand a, b, c;
+  LaOperand e;         // e.p: dots[h][token] = sum over the columns of e . out (the decay's gradient) | null
+  float* dots;         // [slices of 64 columns][H][total]
+  void* out;           // [total][H][dc] BF16 / FP32
+  const float* init;   // [nseq][H][da * dc], strides s_row, s_col | null = zero
+  float* fin;          // the last state, same layout | null
+  int64_t s_row, s_col;
+  float init_scale, fin_scale;
+  int da, dc, out_f32, reverse;
+};
+struct LaArgs {
+  LaJob job[3];
+  const void* g;           // log decays, FP32 / BF16
+  int64_t g_sb, g_st, g_sh;
+  const int32_t* cu;       // [nseq + 1] packed sequences | null
+  int64_t T, total;        // tokens of a sequence (unpacked), tokens in all
+  int njobs, nseq, H, g_f32;
+  float scale;
+  int* status;
+};
+constexpr int kLaMaxD = 128;
+struct LaStepArgs {
+  LaOperand q, k, v;       // strides: sb = batch, sh = head
+  const void* g;           // [batch][H] FP32 / BF16, strides g_sb, g_sh
+  float* state;            // [slots][H][dk][dv]
+  const int64_t* slot;     // [batch], -1 = an empty row | null = row i of state
+  uint16_t* out;           // [batch][H][dv]
+  int64_t g_sb, g_sh, batch, slots;
+  int H, dk, dv, g_f32;
+  float scale;
+};
+int launch_la_step(const LaStepArgs& a, cudaStream_t stream);
+int launch_la_recurrent(const LaArgs& a, cudaStream_t stream);
+size_t la_chunk_workspace(const LaArgs& a);
+// precise: more parts of the rounded operands (the gradients); dots then hold one plane per 64 columns
+int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream);
+// dg[t, h] = <last state, its gradient> + sum over t' >= t of (q . dq - k . dk), from the jobs' dots
+struct LaDecayGradArgs {
+  const float *q_dots, *k_dots;  // [slices][H][total]
+  int q_slices, k_slices;
+  const float *last, *d_last;    // [nseq][H][state_elems] | null
+  void* dg;                      // contiguous [total][H], FP32 / BF16
+  const int32_t* cu;
+  int64_t T, total, state_elems;
+  int nseq, H, g_f32;
+};
+int launch_la_decay_grad(const LaDecayGradArgs& a, cudaStream_t stream);
+// out[t][kv][d] = bf16(sum over the group's query heads of in[t][h][d])
+int launch_la_group_sum(const float* in, uint16_t* out, int64_t total, int H, int group, int d, cudaStream_t stream);
 
 }  // namespace spx

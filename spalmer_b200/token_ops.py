@@ -1,0 +1,510 @@
+"""Operators of the token half of a block, between two channel mixers.
+
+* ``add_rms_norm`` / ``add_rms_norm_mxfp8``: the residual's addition and RMSNorm
+  in one pass, with BF16 rows (trains) or MXFP8 rows (serving) out.
+* ``rotary_embed`` with ``rotary_frequencies``: rotary positions of queries and
+  keys (trains).
+* ``linear_attention``: linear attention with a decay per head over batched or
+  packed sequences, with carried states (trains); ``linear_attention_step``:
+  one token a request against a cache of states.
+
+They run on libspx (``spx_add_rmsnorm_rows``, ``spx_rotary``,
+``spx_linear_attention``, ...; ``include/spx.h``) on the current stream of the
+tensors' device, without host synchronisation.  The reference's block
+(modeling.py:246-302) is where they belong; they restate none of its modules.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor
+
+from spalmer_b200 import _lib
+
+_MAX_HEAD_DIM = 128
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _require(tensor: Tensor, name: str, dtype: torch.dtype | tuple, device: torch.device | None = None) -> None:
+    allowed = dtype if isinstance(dtype, tuple) else (dtype,)
+    if not isinstance(tensor, Tensor) or not tensor.is_cuda or tensor.dtype not in allowed:
+        kinds = " or ".join(str(d).replace("torch.", "") for d in allowed)
+        raise ValueError(f"{name} must be a {kinds} CUDA tensor")
+    if device is not None and tensor.device != device:
+        raise ValueError(f"{name} is on {tensor.device}, not on {device}")
+
+
+# ---------------------------------------------------------------- residual + RMSNorm
+def _rows(t: Tensor, d: int, item: int) -> Tensor:
+    """``t`` as [rows, d] whose rows start on 16 bytes (a copy only if it must be)."""
+
+    r = t.reshape(-1, d)
+    if r.shape[0] and (r.stride(1) != 1 or (r.stride(0) * item) % 16 or r.data_ptr() % 16):
+        r = r.contiguous()
+        if r.data_ptr() % 16:
+            r = r.clone()
+    return r
+
+
+def _check_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float) -> int:
+    _require(hidden, "hidden", torch.bfloat16)
+    if hidden.ndim < 1 or hidden.shape[-1] < 1:
+        raise ValueError("hidden must be [..., d]")
+    d = hidden.shape[-1]
+    if residual is not None:
+        _require(residual, "residual", (torch.bfloat16, torch.float32), hidden.device)
+        if residual.shape != hidden.shape:
+            raise ValueError(f"residual must have hidden's shape {tuple(hidden.shape)}")
+    _require(weight, "weight", torch.bfloat16, hidden.device)
+    if weight.shape != (d,):
+        raise ValueError(f"weight must be [{d}]")
+    if not eps > 0:
+        raise ValueError("eps must be positive")
+    return d
+
+
+def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float,
+                  mxfp8: bool) -> tuple[Tensor, Tensor | None, Tensor]:
+    """(normed, None, sum) or (values, scales, sum); sum is hidden itself without a residual."""
+
+    d = hidden.shape[-1]
+    x = _rows(hidden, d, 2)
+    n, dev = x.shape[0], x.device
+    f32 = residual is not None and residual.dtype == torch.float32
+    r = None if residual is None else _rows(residual, d, 4 if f32 else 2)
+    w = weight.contiguous()
+    total = hidden if r is None else torch.empty(hidden.shape, dtype=residual.dtype, device=dev)
+    scales = None
+    if mxfp8:
+        out = torch.empty(hidden.shape, dtype=torch.uint8, device=dev)
+        scales = torch.empty(*hidden.shape[:-1], d // 32, dtype=torch.uint8, device=dev)
+    else:
+        out = torch.empty(hidden.shape, dtype=torch.bfloat16, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.spx_add_rmsnorm_rows(
+            x.data_ptr(), x.stride(0), _lib.ptr(r), 0 if r is None else r.stride(0), int(f32), w.data_ptr(), float(eps),
+            n, d, None if r is None else total.data_ptr(), None if mxfp8 else out.data_ptr(),
+            out.data_ptr() if mxfp8 else None, _lib.ptr(scales), _stream(dev)), "spx_add_rmsnorm_rows")
+    return out, scales, total
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, residual, weight, eps):
+        out, _, total = _norm_forward(hidden, residual, weight, eps, False)
+        ctx.set_materialize_grads(False)
+        ctx.eps = eps
+        ctx.has_residual = residual is not None
+        ctx.save_for_backward(total, weight)
+        if residual is None:
+            return out, None
+        return out, total
+
+    @staticmethod
+    def backward(ctx, d_out, d_total):
+        total, weight = ctx.saved_tensors
+        d = total.shape[-1]
+        dev = total.device
+        if d_out is None:
+            d_out = torch.zeros(total.shape, dtype=torch.bfloat16, device=dev)
+        f32 = total.dtype == torch.float32
+        item = 4 if f32 else 2
+        h, dy = _rows(total, d, item), _rows(d_out.to(torch.bfloat16), d, 2)
+        ds = None if d_total is None else _rows(d_total.to(total.dtype), d, item)
+        n = h.shape[0]
+        d_hidden = torch.empty(total.shape, dtype=torch.bfloat16, device=dev)
+        d_residual = torch.empty(total.shape, dtype=torch.float32, device=dev) if f32 else None
+        d_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
+        lib = _lib.load()
+        nbytes = lib.spx_add_rmsnorm_backward_workspace(n, d) if d_weight is not None else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with torch.cuda.device(dev):
+            _lib.check(lib.spx_add_rmsnorm_backward(
+                h.data_ptr(), h.stride(0), int(f32), weight.contiguous().data_ptr(), ctx.eps, dy.data_ptr(),
+                dy.stride(0), _lib.ptr(ds), 0 if ds is None else ds.stride(0), n, d, d_hidden.data_ptr(),
+                _lib.ptr(d_residual), _lib.ptr(d_weight), _lib.ptr(ws), nbytes, _stream(dev)),
+                "spx_add_rmsnorm_backward")
+        d_res = None
+        if ctx.has_residual:
+            d_res = d_residual if f32 else d_hidden
+        return d_hidden, d_res, d_weight, None
+
+
+def add_rms_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """``(normed, summed)``: ``summed = hidden + residual`` in the residual's type and
+    RMSNorm of it, ``normed = bf16(summed * weight / sqrt(mean(summed^2) + eps))``.
+
+    ``hidden`` [..., d] BF16, ``residual`` the same shape in BF16 or FP32 (a
+    residual stream kept in FP32), ``weight`` [d] BF16; d a multiple of 8 up to
+    16,384.  Without a residual ``summed`` is ``hidden`` itself.  Unlike
+    ``rms_norm``, which repeats its reference's BF16 roundings in between, the
+    result is rounded once.  Differentiable in all three tensors.
+    """
+
+    _check_norm(hidden, residual, weight, eps)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
+        normed, summed = _AddRMSNorm.apply(hidden, residual, weight, float(eps))
+        return normed, hidden if summed is None else summed
+    normed, _, summed = _norm_forward(hidden, residual, weight, eps, False)
+    return normed, summed
+
+
+def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor,
+                       eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor]:
+    """``(values, scales, summed)``: ``add_rms_norm`` with MXFP8 rows out, quantised
+    from the FP32 result: E4M3 bytes [..., d] and one E8M0 byte per 32 elements
+    [..., d / 32] (uint8), the layout of ``native.mx_quantize_rows`` and the left
+    operand of ``native.mxfp8_mm_rows``.  d a multiple of 32.  Forward only.
+    """
+
+    d = _check_norm(hidden, residual, weight, eps)
+    if d % 32:
+        raise ValueError("the row length must be a multiple of the block size 32")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, residual, weight)):
+        raise NotImplementedError("add_rms_norm_mxfp8 implements the forward pass only")
+    return _norm_forward(hidden, residual, weight, eps, True)
+
+
+# ---------------------------------------------------------------- rotary positions
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device: torch.device | str | None = None) -> tuple[Tensor, float]:
+    """``(frequencies, factor)`` for ``rotary_embed``: FP64 [rotary_dim / 2] radians per
+    position, ``base ** (-2 p / rotary_dim)``, and the factor on sine and cosine (1 unless "yarn").
+
+    ``scaling`` stretches them for contexts ``factor`` times as long as the
+    trained ``original_length``: ``"linear"`` divides every frequency,
+    ``"ntk"`` raises the base to ``base * factor ** (r / (r - 2))``, and
+    ``"yarn"`` divides those that turn less than ``beta_slow`` times over the
+    trained length, keeps those that turn more than ``beta_fast`` times, blends
+    linearly in between, and scales by ``0.1 ln(factor) + 1``.
+    """
+
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError("scaling must be None, 'linear', 'ntk' or 'yarn'")
+    if not base > 1 or not factor >= 1 or original_length < 1:
+        raise ValueError("base > 1, factor >= 1 and original_length >= 1 are required")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs rotary_dim >= 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    p = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    freq = base ** (-p / max(rotary_dim, 1))
+    mult = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        def pair_of(turns: float) -> float:  # the pair that turns `turns` times over the trained length
+            return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim // 2 - 1)
+        ramp = ((p / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        mult = 0.1 * math.log(factor) + 1.0
+    return freq.to(device) if device is not None else freq, mult
+
+
+def _token_heads(t: Tensor, name: str) -> tuple[Tensor, Tensor]:
+    """``t`` [..., heads, d] as (the tensor kept alive, a [tokens, heads, d] view with unit inner stride)."""
+
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    return t.reshape(-1, t.shape[-2], t.shape[-1])  # a view wherever the leading dimensions merge
+
+
+def _rotate(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Tensor, interleaved: bool, factor: float,
+            inverse: bool) -> tuple[Tensor, Tensor | None]:
+    dev = q.device
+    qt = _token_heads(q, "q")
+    kt = None if k is None else _token_heads(k, "k")
+    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    k_out = None if k is None else torch.empty(k.shape, dtype=torch.bfloat16, device=dev)
+    n = qt.shape[0]
+    if n == 0:
+        return q_out, k_out
+    hq = _lib.Heads(qt.data_ptr(), 0, qt.stride(0), qt.stride(1))
+    hk = None if kt is None else _lib.Heads(kt.data_ptr(), 0, kt.stride(0), kt.stride(1))
+    pos = positions.contiguous()
+    freq = frequencies.contiguous()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.spx_rotary(
+            hq, qt.shape[1], hk, 0 if kt is None else kt.shape[1], n, q.shape[-1], freq.shape[0], pos.data_ptr(),
+            int(pos.dtype == torch.int64), pos.numel(), freq.data_ptr(), factor, int(interleaved), int(inverse),
+            q_out.data_ptr(), _lib.ptr(k_out), _stream(dev)), "spx_rotary")
+    return q_out, k_out
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, interleaved, factor):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.args = (interleaved, factor)
+        ctx.has_k = k is not None
+        return _rotate(q, k, positions, frequencies, interleaved, factor, False)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, frequencies = ctx.saved_tensors
+        interleaved, factor = ctx.args
+        gq, gk = _rotate(dq, dk if ctx.has_k else None, positions, frequencies, interleaved, factor, True)
+        return gq, gk, None, None, None, None
+
+
+def rotary_embed(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Tensor, *, interleaved: bool = False,
+                 factor: float = 1.0) -> tuple[Tensor, Tensor | None]:
+    """Rotary positions: ``(q, k)`` with the first ``2 * len(frequencies)`` elements of
+    every head turned by ``position * frequency`` and scaled by ``factor``.
+
+    ``q`` [..., heads, d] and ``k`` [..., kv_heads, d] (or None) BF16, views of a
+    fused projection included; ``positions`` int32 or int64, one per token or
+    one per token of the last leading dimension (shared by the batch);
+    ``frequencies`` FP64 [pairs] (``rotary_frequencies``).  Pairs are halves of
+    the rotated part, or neighbours with ``interleaved``.  New contiguous
+    tensors come back.  Differentiable in q and k.
+    """
+
+    _require(q, "q", torch.bfloat16)
+    dev = q.device
+    if q.ndim < 3:
+        raise ValueError("q must be [..., tokens, heads, head_dim]")
+    if k is not None:
+        _require(k, "k", torch.bfloat16, dev)
+        if k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ValueError("k must be [..., kv_heads, head_dim] over q's tokens")
+    _require(positions, "positions", (torch.int32, torch.int64), dev)
+    _require(frequencies, "frequencies", torch.float64, dev)
+    if frequencies.ndim != 1 or 2 * frequencies.shape[0] > q.shape[-1]:
+        raise ValueError("frequencies must be [pairs] with 2 * pairs <= head_dim")
+    tokens = math.prod(q.shape[:-2])
+    if positions.numel() not in (tokens, q.shape[-3]) or (positions.numel() != tokens and positions.ndim != 1):
+        raise ValueError(f"positions must hold one position per token ({tokens}, or {q.shape[-3]} shared by the batch)")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, frequencies, bool(interleaved), float(factor))
+    return _rotate(q, k, positions, frequencies, bool(interleaved), float(factor), False)
+
+
+# ---------------------------------------------------------------- linear attention
+_status: dict[torch.device, Tensor] = {}
+
+
+def _status_word(device: torch.device) -> Tensor:
+    word = _status.get(device)
+    if word is None:
+        word = _status[device] = torch.zeros(4, dtype=torch.int32, device=device)
+    return word
+
+
+def linear_attention_status(device: torch.device | str | int | None = None, clear: bool = True) -> int:
+    """The device status word of ``linear_attention`` (synchronises); 0 means no kernel reported an error."""
+
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.empty(0, device=device).device
+    word = _status.get(dev)
+    if word is None:
+        return 0
+    value = int(word[0].item())
+    if clear:
+        word.zero_()
+    return value
+
+
+def _aligned_heads(t: Tensor) -> Tensor:
+    """``t`` [B, T, H, d] with unit inner stride and heads on 16 bytes (a copy only if it must be)."""
+
+    sizes, strides = t.shape, t.stride()
+    if (t.data_ptr() % 16 or (strides[-1] != 1 and sizes[-1] > 1)
+            or any(st % 8 and n > 1 for st, n in zip(strides[:-1], sizes[:-1]))):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _heads(t: Tensor) -> _lib.Heads:
+    # the stride of a dimension of one element is never used; views may carry any value there
+    b, n, h = (st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape[:3]))
+    return _lib.Heads(t.data_ptr(), b, n, h)
+
+
+def _decays(g: Tensor) -> _lib.Decays:
+    return _lib.Decays(g.data_ptr(), *g.stride())
+
+
+def _dims(q: Tensor, k: Tensor, v: Tensor, g: Tensor, cu: Tensor | None, scale: float) -> _lib.LinAttnDims:
+    return _lib.LinAttnDims(q.shape[0] if cu is None else cu.shape[0] - 1, q.shape[1], q.shape[2], k.shape[2],
+                            q.shape[3], v.shape[3], int(cu is not None), int(g.dtype == torch.float32), scale)
+
+
+def _attend(q: Tensor, k: Tensor, v: Tensor, g: Tensor, cu: Tensor | None, state: Tensor | None, scale: float,
+            want_state: bool) -> tuple[Tensor, Tensor | None]:
+    dev = q.device
+    dims = _dims(q, k, v, g, cu, scale)
+    out = torch.empty(*q.shape[:3], v.shape[3], dtype=torch.bfloat16, device=dev)
+    last = None
+    if want_state:
+        last = torch.empty(dims.batch, q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.spx_linear_attention_workspace(dims)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.spx_linear_attention(dims, _heads(q), _heads(k), _heads(v), _decays(g), _lib.ptr(cu),
+                                            _lib.ptr(state), out.data_ptr(), _lib.ptr(last), _lib.ptr(ws), nbytes,
+                                            _status_word(dev).data_ptr(), _stream(dev)), "spx_linear_attention")
+    return out, last
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, state, cu, scale, want_state):
+        ctx.set_materialize_grads(False)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, g, state, cu)
+        return _attend(q, k, v, g, cu, state, scale, want_state)
+
+    @staticmethod
+    def backward(ctx, d_out, d_last):
+        q, k, v, g, state, cu = ctx.saved_tensors
+        dev = q.device
+        dims = _dims(q, k, v, g, cu, ctx.scale)
+        if d_out is None:
+            d_out = torch.zeros(*q.shape[:3], v.shape[3], dtype=torch.bfloat16, device=dev)
+        d_out = _aligned_heads(d_out.to(torch.bfloat16))
+        d_last = None if d_last is None else d_last.float().contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+        dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
+        d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
+        lib = _lib.load()
+        nbytes = lib.spx_linear_attention_backward_workspace(dims)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with torch.cuda.device(dev):
+            _lib.check(lib.spx_linear_attention_backward(
+                dims, _heads(q), _heads(k), _heads(v), _decays(g), _lib.ptr(cu), _lib.ptr(state), _heads(d_out),
+                _lib.ptr(d_last), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), _lib.ptr(d_state),
+                _lib.ptr(ws), nbytes, _status_word(dev).data_ptr(), _stream(dev)), "spx_linear_attention_backward")
+        return dq, dk, dv, dg, d_state, None, None, None
+
+
+def _check_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, scale: float, lead: int, layout: str) -> None:
+    _require(q, "q", torch.bfloat16)
+    dev = q.device
+    for name, t in (("k", k), ("v", v)):
+        _require(t, name, torch.bfloat16, dev)
+    _require(g, "log_decay", (torch.float32, torch.bfloat16), dev)
+    if q.ndim != lead + 2 or k.ndim != lead + 2 or v.ndim != lead + 2 or g.ndim != lead + 1:
+        raise ValueError(f"q, k, v must be [{layout}, heads, dim] and log_decay [{layout}, heads]")
+    if k.shape[:lead] != q.shape[:lead] or v.shape[:lead] != q.shape[:lead] or g.shape != q.shape[:lead + 1]:
+        raise ValueError("q, k, v and log_decay must share their leading dimensions, log_decay q's heads too")
+    if k.shape[-1] != q.shape[-1] or v.shape[lead] != k.shape[lead]:
+        raise ValueError("k must have q's head dimension and v the heads of k")
+    if k.shape[lead] < 1 or q.shape[lead] % k.shape[lead] or q.shape[lead] < 1:
+        raise ValueError("the query heads must be a multiple of the key/value heads")
+    for name, n in (("key", q.shape[-1]), ("value", v.shape[-1])):
+        if n < 8 or n % 8 or n > _MAX_HEAD_DIM:
+            raise ValueError(f"the {name} dimension of a head must be a multiple of 8 up to {_MAX_HEAD_DIM}")
+    if not (math.isfinite(scale) and scale != 0):
+        raise ValueError("scale must be finite and not zero")
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scale: float | None = None,
+                     initial_state: Tensor | None = None, cu_seqlens: Tensor | None = None,
+                     return_state: bool = False) -> tuple[Tensor, Tensor | None]:
+    """Causal linear attention with a decay per head: ``(out, last_state or None)``.
+
+    Per sequence and query head, with the FP32 state S [key_dim, value_dim]:
+    ``S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T`` and ``out_t = scale * S_t^T q_t``.
+
+    ``q`` [B, T, heads, key_dim], ``k`` [B, T, kv_heads, key_dim], ``v`` [B, T,
+    kv_heads, value_dim] BF16 (views of a fused projection included; query head
+    h reads head ``h // (heads // kv_heads)``), ``log_decay`` [B, T, heads]
+    FP32 or BF16, natural logarithms meant to be <= 0.  Head dimensions are
+    multiples of 8 up to 128; ``scale`` defaults to ``key_dim ** -0.5``.
+    ``cu_seqlens`` (int32 [n + 1], from 0 to T, B = 1) packs n sequences into
+    one row; an entry that is out of order skips its sequence and shows in
+    ``linear_attention_status``.  ``initial_state`` and the returned last state
+    are FP32 [B or n, heads, key_dim, value_dim].  Nothing passes from one
+    sequence to another, non-finite values included.
+
+    Differentiable in q, k, v, log_decay and initial_state, through the output
+    and the last state; the backward keeps nothing but the inputs.
+    """
+
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    _check_attention(q, k, v, log_decay, scale, 2, "batch, tokens")
+    dev = q.device
+    n = q.shape[0]
+    if cu_seqlens is not None:
+        _require(cu_seqlens, "cu_seqlens", torch.int32, dev)
+        if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1 or q.shape[0] != 1:
+            raise ValueError("cu_seqlens must be [sequences + 1] over one packed row (B = 1)")
+        cu_seqlens = cu_seqlens.contiguous()
+        n = cu_seqlens.shape[0] - 1
+    if initial_state is not None:
+        _require(initial_state, "initial_state", torch.float32, dev)
+        want = (n, q.shape[2], q.shape[3], v.shape[3])
+        if tuple(initial_state.shape) != want:
+            raise ValueError(f"initial_state must be {list(want)}")
+        initial_state = initial_state.contiguous()
+    q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
+        return _LinearAttention.apply(q, k, v, log_decay, initial_state, cu_seqlens, scale, return_state)
+    return _attend(q, k, v, log_decay, cu_seqlens, initial_state, scale, return_state)
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, *,
+                          slots: Tensor | None = None, scale: float | None = None) -> Tensor:
+    """One token of each request: updates ``state`` in place, returns ``out`` [B, heads, value_dim].
+
+    ``q`` [B, heads, key_dim], ``k`` and ``v`` [B, kv_heads, ...] BF16,
+    ``log_decay`` [B, heads] FP32 or BF16, ``state`` FP32 [slots, heads, key_dim,
+    value_dim] contiguous.  Request i uses state ``slots[i]`` (int64 [B]; None:
+    i); an index outside the cache (-1, say) marks an empty row, which returns
+    zeros and touches nothing.  No index may appear twice.  Forward only.
+    """
+
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    _check_attention(q, k, v, log_decay, scale, 1, "batch")
+    dev = q.device
+    _require(state, "state", torch.float32, dev)
+    B, H, dk = q.shape
+    dv = v.shape[-1]
+    if state.ndim != 4 or tuple(state.shape[1:]) != (H, dk, dv) or not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError(f"state must be a contiguous, 16-byte aligned [slots, {H}, {dk}, {dv}]")
+    if slots is None:
+        if state.shape[0] < B:
+            raise ValueError("state holds fewer slots than there are requests")
+    else:
+        _require(slots, "slots", torch.int64, dev)
+        if slots.shape != (B,):
+            raise ValueError(f"slots must be [{B}]")
+        slots = slots.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise NotImplementedError("linear_attention_step implements the forward pass only")
+    q, k, v = (_aligned_heads(t[:, None]) for t in (q, k, v))
+    out = torch.empty(B, H, dv, dtype=torch.bfloat16, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.spx_linear_attention_step(
+            _heads(q), _heads(k), _heads(v), _lib.Decays(log_decay.data_ptr(), log_decay.stride(0), 0, log_decay.stride(1)),
+            int(log_decay.dtype == torch.float32), B, H, k.shape[2], dk, dv, scale, state.data_ptr(), state.shape[0],
+            _lib.ptr(slots), out.data_ptr(), _stream(dev)), "spx_linear_attention_step")
+    return out
+
+
+__all__ = [
+    "add_rms_norm",
+    "add_rms_norm_mxfp8",
+    "linear_attention",
+    "linear_attention_status",
+    "linear_attention_step",
+    "rotary_embed",
+    "rotary_frequencies",
+]
