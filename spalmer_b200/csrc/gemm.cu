@@ -1248,6 +1248,8 @@ int encode_3d(CUtensorMap* map, const void* base, int64_t groups, int64_t rows, 
 int encode_heads(CUtensorMap* map, const void* base, int64_t d, int64_t heads, int64_t tokens, int64_t batch,
                  int64_t head_stride, int64_t token_stride, int64_t batch_stride, int box_tokens) {
   if (int rc = get_encoder(); rc != SPX_OK) return rc;
+  // a driver call: in a thread whose first CUDA work this is (autograd's), no context is current yet
+  if (int dev = 0; cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return SPX_ERR_CUDA;
   const int64_t extent[3] = {heads, tokens, batch}, stride[3] = {head_stride, token_stride, batch_stride};
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens),
                         static_cast<cuuint64_t>(batch)};

@@ -1,0 +1,936 @@
+// Linear attention with a decay per head on tcgen05 tensor cores: the chunked
+// form of a job of LaArgs (kernels.h).  For a chunk of 128 tokens with G_i =
+// the sum of the log decays up to token i inside the chunk,
+//
+//   out = scale ( tril(e^{G_i - G_j} a_i . b_j) C + e^{G_i} a_i S )
+//   S'  = e^{G_128} S + sum_j e^{G_128 - G_j} b_j c_j^T
+//
+// (reverse: triu, e^{G_j - G_i}, e^{G_128 - G_i} and e^{G_j}).  The forward
+// pass and the three gradients are jobs of this one form, so a backward pass is
+// one launch of three times the work and stores no states.
+//
+// A CTA walks its chunks in order for one (job, sequence, head, 64 columns of
+// C); the FP32 state stays in registers from chunk to chunk.  64 columns leave
+// room in shared memory to load the next chunk (two or three stages) and twice
+// as many CTAs at 128-wide heads; a . b is then computed once per 64 columns,
+// which the tensor cores have time for while HBM is the bound (at 128-wide
+// heads about 2,000 tensor cycles a chunk against 2,800 of memory time).
+//
+// Operand precision.  a, b, c are exact BF16.  What is not is split into BF16
+// parts that are multiplied one after another into the same FP32 accumulator:
+//   c scaled by its decay (into the state): three parts in the forward pass,
+//     whose state a caller keeps (2^-26), two in the gradients (2^-18);
+//   the decayed a . b matrix and the state (into out): one part in the forward
+//     pass, whose output is rounded to BF16 as coarsely, two in the gradients,
+//     because d decay is a long sum of q . dq - k . dk that cancels.
+//
+// Decay factors are exponentials of differences <= 0, never quotients, so no
+// decay overflows: inside a 32-token block e^{G_i - G_j} directly, across
+// blocks e^{G_i - G_end} * e^{G_end - G_j} with the end of j's block between
+// them.  Sums run from the block's start, so a token that forgets everything
+// (clamped to 2^-150, which is zero in FP32) costs its neighbours no digits.
+//
+// When (job, sequence, head, slice) fill too few SMs, the sequence is cut into
+// segments: a pass over b and c alone gives each segment's state from zero, a
+// small kernel chains them, and the full pass starts every segment from its
+// own first state.
+//
+// Warps: 0-3 the decayed a . b matrix (TMEM -> registers -> TMEM operand),
+// 4-7 the state, 8-11 scaled c and the epilogue, 12 TMA, 13 MMA, 14 decays.
+// Every wait is bounded (status word, then return).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "sm100.cuh"
+
+namespace spx {
+
+namespace {
+
+constexpr int kC = 128;              // tokens of a chunk
+constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
+constexpr int kLaThreads = 15 * 32;
+constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
+
+struct alignas(64) LaChunkArgs {
+  CUtensorMap map[3][3];
+  LaArgs la;
+  int lanes[4];          // first lane of each job; lanes[njobs] = all of them
+  int slices[3];
+  int nseg, state_only, run_segs;
+  float* seg_state;      // [lane][nseg][128][64]
+  float* seg_decay;      // [lane][nseg]
+};
+
+struct DecayTable {
+  float lg[kC];  // log2 decay from the start of the token's 32-token block, inclusive
+  float cf[kC];  // from the token to its block's end (forward) / from the block's start to it (reverse)
+  float total[4];
+};
+
+template <int DKB, bool PRECISE>
+struct Cfg {
+  static constexpr int kStages = DKB == 1 ? 3 : 2;
+  static constexpr int kParts = PRECISE ? 2 : 3;  // of scaled c
+  static constexpr int kSParts = PRECISE ? 2 : 1; // of the state
+  static constexpr uint32_t kStage = (2 * DKB + 1) * kTile;
+  static constexpr uint32_t kSTile = DKB * 64 * 128;
+  static constexpr uint32_t kOffS = kStages * kStage;
+  static constexpr uint32_t kOffV = kOffS + kSParts * kSTile;
+  static constexpr uint32_t kOffT = kOffV + kParts * kTile;
+  static constexpr uint32_t kOffBar = kOffT + 2 * sizeof(DecayTable);
+  static constexpr uint32_t kBytes = kOffBar + 256;
+};
+static_assert(Cfg<2, false>::kBytes <= 232448 && Cfg<2, true>::kBytes <= 232448, "shared memory of a CTA");
+
+struct Item {
+  int job, seq, h, slice, seg, lane;
+  int64_t start, len;  // tokens of the sequence in the flattened order
+  int nch, p0, n;      // chunks of the sequence; this item's: p0 .. p0 + n in processing order
+};
+
+__device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
+  const int all = a.lanes[a.la.njobs];
+  it->seg = idx / all;
+  it->lane = idx - it->seg * all;
+  int j = 0;
+  while (j + 1 < a.la.njobs && it->lane >= a.lanes[j + 1]) ++j;
+  it->job = j;
+  int r = it->lane - a.lanes[j];
+  it->slice = r % a.slices[j];
+  r /= a.slices[j];
+  it->h = r % a.la.H;
+  it->seq = r / a.la.H;
+  bool ok = true;
+  if (a.la.cu == nullptr) {
+    it->start = it->seq * a.la.T;
+    it->len = a.la.T;
+  } else {
+    const int64_t lo = __ldg(a.la.cu + it->seq), hi = __ldg(a.la.cu + it->seq + 1);
+    ok = lo >= 0 && hi >= lo && hi <= a.la.total;
+    it->start = ok ? lo : 0;
+    it->len = ok ? hi - lo : 0;
+  }
+  it->nch = static_cast<int>((it->len + kC - 1) / kC);
+  const int per = (it->nch + a.nseg - 1) / a.nseg;
+  it->p0 = min(it->seg * per, it->nch);
+  it->n = min(per, it->nch - it->p0);
+  return ok;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float lo_of(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float hi_of(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+
+// Every lane polls; the warp goes on together, or gives up together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, status, code)) != 0;
+}
+
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]^T, BF16: A holds two K elements per column.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major operand of [128-byte rows along K][64 MN elements] tiles, 128-byte
+// swizzle; the next 64 MN elements are `lbo` bytes on.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// Byte offset of 16-byte chunk `c` of 128-byte row `row` in a 128B-swizzled tile.
+__device__ __forceinline__ uint32_t swz(int row, int c) {
+  return static_cast<uint32_t>(row) * 128u + static_cast<uint32_t>((c ^ (row & 7)) << 4);
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Split two floats into NP packed BF16 parts, each the rounding of what the ones before leave.
+template <int NP>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&part)[NP]) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    part[p] = pack_bf16(x, y);
+    if (p + 1 < NP) {
+      x -= lo_of(part[p]);
+      y -= hi_of(part[p]);
+    }
+  }
+}
+
+struct Bars {
+  uint64_t full[3], empty[3];
+  uint64_t gfull[2], gfree[2];
+  uint64_t pacc[2], pop[2];
+  uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
+  uint64_t vp, kv, kvfree, sop, qs, o, ofree, drained;
+  uint32_t tmem;
+};
+static_assert(sizeof(Bars) <= 256, "barriers");
+
+}  // namespace
+
+template <int DKB, bool PRECISE>
+__global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_constant__ LaChunkArgs args) {
+  using K = Cfg<DKB, PRECISE>;
+  extern __shared__ __align__(1024) uint8_t la_smem[];
+  const uint32_t base = smem_u32(la_smem);
+  int* const status = args.la.status;
+  if ((base & 1023u) != 0u) {  // the swizzled tiles need it; uniform over the CTA
+    if (threadIdx.x == 0) record_error(status, SPX_DEV_BAD_TILE);
+    return;
+  }
+  Bars& bar = *reinterpret_cast<Bars*>(la_smem + K::kOffBar);
+  DecayTable* const tables = reinterpret_cast<DecayTable*>(la_smem + K::kOffT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool full_pass = args.state_only == 0;
+  const int items = args.lanes[args.la.njobs] * args.run_segs;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&bar.full[s], 1);
+      mbar_init(&bar.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar.gfull[s], 1);
+      mbar_init(&bar.gfree[s], full_pass ? 12 : 8);
+      mbar_init(&bar.pacc[s], 1);
+      mbar_init(&bar.pop[s], 4);
+      mbar_init(&bar.tail[s], 4);
+    }
+    mbar_init(&bar.vp, 4);
+    mbar_init(&bar.kv, 1);
+    mbar_init(&bar.kvfree, 4);
+    mbar_init(&bar.sop, 4);
+    mbar_init(&bar.qs, 1);
+    mbar_init(&bar.o, 1);
+    mbar_init(&bar.ofree, 4);
+    mbar_init(&bar.drained, 1);
+    fence_mbar_init();
+  }
+  if (warp == 13) {
+    tmem_alloc(&bar.tmem, kTmCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const int quad = warp & 3;
+  const uint32_t tm_lane = static_cast<uint32_t>(quad * 32) << 16;
+  const int row = quad * 32 + lane;  // this thread's TMEM lane / tile row
+  bool ok = true;
+  uint32_t it = 0;  // chunks so far, the same count in every role
+
+  if (warp < 4) {
+    // ---------------- the decayed a . b matrix
+    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
+      Item w;
+      item_of(args, idx, &w);
+      const bool rev = args.la.job[w.job].reverse != 0;
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u, ph = (it >> 1) & 1u;
+        const DecayTable& t = tables[b];
+        if (!(ok = warp_wait(&bar.gfull[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const float lg = t.lg[row];
+        // factor of a whole off-diagonal block, between this row and the block's near edge
+        float rf[4];
+        {
+          float run = rev ? t.total[quad] - lg : lg;
+          if (!rev) {
+#pragma unroll
+            for (int j = 3; j >= 0; --j)
+              if (j < quad) {
+                rf[j] = ex2(run);
+                run += t.total[j];
+              }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j > quad) {
+                rf[j] = ex2(run);
+                run += t.total[j];
+              }
+          }
+        }
+        if (!(ok = warp_wait(&bar.pacc[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + kTmP + b * 128u + tm_lane;
+        constexpr int kLo = PRECISE ? 2 : 1;
+        // one 32-column block: TMEM -> kLo x 16 packed words
+        auto block = [&](int j, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+          if (rev ? j < quad : j > quad) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) hi[q] = lo[q] = 0u;
+            return;
+          }
+          uint32_t s[32];
+          tmem_ld32(acc + 32u * j, s);
+          tmem_wait_ld();
+          const float4* f4 = reinterpret_cast<const float4*>(j == quad ? t.lg + 32 * j : t.cf + 32 * j);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 f = f4[q];
+            float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = 4 * q + e;
+              const float x = __uint_as_float(s[c]);
+              if (j == quad)  // lane = the row inside the block; a masked entry is zero whatever it holds
+                v[e] = (rev ? c >= lane : c <= lane) ? x * ex2(rev ? v[e] - lg : lg - v[e]) : 0.0f;
+              else
+                v[e] = x * (v[e] * rf[j]);
+            }
+            uint32_t p0[kLo], p1[kLo];
+            split2<kLo>(v[0], v[1], p0);
+            split2<kLo>(v[2], v[3], p1);
+            hi[2 * q] = p0[0];
+            hi[2 * q + 1] = p1[0];
+            if constexpr (PRECISE) {
+              lo[2 * q] = p0[1];
+              lo[2 * q + 1] = p1[1];
+            }
+          }
+        };
+        // The operand (64 columns, PRECISE: 128) takes the accumulator's place: a
+        // block is written only where every accumulator column under it has been read.
+        if constexpr (!PRECISE) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            block(j, hi, lo);
+            tmem_st16(acc + 16u * j, hi);
+          }
+        } else {
+          uint32_t h2[16], l2[16], h3[16], l3[16], hi[16], lo[16];
+          block(2, h2, l2);
+          block(3, h3, l3);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            block(j, hi, lo);
+            tmem_st16(acc + 16u * j, hi);
+            tmem_st16(acc + 64u + 16u * j, lo);
+          }
+          tmem_st16(acc + 32u, h2);
+          tmem_st16(acc + 96u, l2);
+          tmem_st16(acc + 48u, h3);
+          tmem_st16(acc + 112u, l3);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&bar.gfree[b], lane);
+        warp_arrive(&bar.pop[b], lane);
+      }
+    }
+  } else if (warp < 8) {
+    // ---------------- the state: one row of da, 64 columns, in registers
+    const bool rows_in = quad < 2 * DKB;
+    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+      Item w;
+      const bool sound = item_of(args, idx, &w);
+      const LaJob& j = args.la.job[w.job];
+      if (!sound && threadIdx.x == 128) record_error(status, SPX_DEV_BAD_TILE);
+      float s[64];
+      const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
+      const int col0 = w.slice * 64;
+      const bool live = row < j.da;
+      if (args.nseg > 1 && full_pass) {
+        const float4* f = reinterpret_cast<const float4*>(
+            args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float4 v = live ? f[q] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          s[4 * q] = v.x, s[4 * q + 1] = v.y, s[4 * q + 2] = v.z, s[4 * q + 3] = v.w;
+        }
+      } else {
+        const bool some = j.init != nullptr && args.nseg == 1 && live;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          s[c] = some && col0 + c < j.dc ? j.init_scale * j.init[st0 + row * j.s_row + (col0 + c) * j.s_col] : 0.0f;
+      }
+      float decay = 1.0f;
+      auto write_operand = [&]() {  // BF16 parts of the state for the next chunk's a . S
+        if (rows_in) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t q[4][K::kSParts];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split2<K::kSParts>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1], q[e]);
+#pragma unroll
+            for (int part = 0; part < K::kSParts; ++part)
+              sts16(base + K::kOffS + part * K::kSTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
+          }
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&bar.sop, lane);
+      };
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u;
+        if (full_pass) {
+          // the operand before this chunk; its last reader was the chunk before
+          if (it > 0 && !(ok = warp_wait(&bar.qs, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+          write_operand();
+        }
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const float* tt = tables[b].total;
+        const float gamma = ex2((tt[0] + tt[1]) + (tt[2] + tt[3]));
+        warp_arrive(&bar.gfree[b], lane);
+        decay *= gamma;
+        if (!(ok = warp_wait(&bar.kv, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        if (rows_in) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t x[32];
+            tmem_ld32(tmem + kTmKV + 32u * half + tm_lane, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[32 * half + c] = fmaf(gamma, s[32 * half + c], __uint_as_float(x[c]));
+          }
+        }
+        tc_fence_before();
+        warp_arrive(&bar.kvfree, lane);
+      }
+      if (!ok) break;
+      if (!full_pass) {
+        float4* f = reinterpret_cast<float4*>(
+            args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64);
+        if (live) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) f[q] = make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]);
+        }
+        if (threadIdx.x == 128) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
+      } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (col0 + c < j.dc) j.fin[st0 + row * j.s_row + (col0 + c) * j.s_col] = j.fin_scale * s[c];
+      }
+    }
+  } else if (warp < 12) {
+    // ---------------- scaled c, and the epilogue one chunk behind it
+    uint32_t tails = 0;
+    struct Pending {
+      float row_factor;
+      int64_t token;  // flattened; < 0: nothing to store
+    } pend{};
+    Item pw{};
+    uint32_t pit = 0;
+    bool have = false;
+    auto epilogue = [&]() {  // chunk `pit` of item `pw`
+      const LaJob& j = args.la.job[pw.job];
+      const bool in = pend.token >= 0;
+      const int col0 = pw.slice * 64;
+      const int valid = min(64, j.dc - col0);  // a multiple of 8
+      uint4 e[8];
+      if (j.e.p != nullptr && in) {
+        const bool packed = args.la.cu != nullptr;
+        const uint16_t* pe = j.e.p + (packed ? 0 : pw.seq) * j.e.sb +
+                             (packed ? pend.token : pend.token - pw.start) * j.e.st + (pw.h / j.e.group) * j.e.sh + col0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (8 * q < valid) e[q] = __ldg(reinterpret_cast<const uint4*>(pe) + q);
+      }
+      if (!warp_wait(&bar.o, pit & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
+      tc_fence_after();
+      const float sc = args.la.scale, sx = args.la.scale * pend.row_factor;
+      const int64_t at = (pend.token * args.la.H + pw.h) * j.dc + col0;
+      float dot = 0.0f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t x[32], y[32];
+        tmem_ld32(tmem + kTmOI + 32u * half + tm_lane, x);
+        tmem_ld32(tmem + kTmOX + 32u * half + tm_lane, y);
+        tmem_wait_ld();
+        if (half == 1) {
+          tc_fence_before();
+          warp_arrive(&bar.ofree, lane);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = fmaf(sx, __uint_as_float(y[8 * q + i]), sc * __uint_as_float(x[8 * q + i]));
+          const int c = 32 * half + 8 * q;
+          if (!in || c >= valid) continue;
+          if (j.out_f32 != 0) {
+            float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(j.out) + at + c);
+            o[0] = make_float4(v[0], v[1], v[2], v[3]);
+            o[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at + c) =
+                make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+          }
+          if (j.e.p != nullptr) {
+            const uint4 u = e[4 * half + q];
+            const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(v[2 * i], lo_of(ew[i]), fmaf(v[2 * i + 1], hi_of(ew[i]), dot));
+          }
+        }
+      }
+      if (j.e.p != nullptr && in)
+        j.dots[(static_cast<int64_t>(pw.slice) * args.la.H + pw.h) * args.la.total + pend.token] = dot;
+      return true;
+    };
+    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+      Item w;
+      item_of(args, idx, &w);
+      const bool rev = args.la.job[w.job].reverse != 0;
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u;
+        const int st = static_cast<int>(it % K::kStages);
+        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+        const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
+        if (!(ok = warp_wait(&bar.full[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const uint32_t stage = base + st * K::kStage;
+        const uint32_t sc = stage + 2 * DKB * kTile;
+        if (len < kC && args.la.cu != nullptr) {
+          // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
+          if (row >= len) {
+#pragma unroll
+            for (int x = 0; x < DKB + 1; ++x)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) sts16(stage + (DKB + x) * kTile + row * 128 + c * 16, 0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          warp_arrive(&bar.tail[tails++ & 1u], lane);
+        }
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        float fwd, back;  // decay from the chunk's start to this token, from it to the chunk's end
+        {
+          const DecayTable& t = tables[b];
+          float before = 0.0f, after = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            before += q < quad ? t.total[q] : 0.0f;
+            after += q > quad ? t.total[q] : 0.0f;
+          }
+          const float lg = t.lg[row];
+          fwd = ex2(before + lg);
+          back = ex2((t.total[quad] - lg) + after);
+        }
+        warp_arrive(&bar.gfree[b], lane);
+        const float wgt = rev ? fwd : back;
+        // the parts' last reader: the state product of the chunk before
+        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 u = lds16(sc + swz(row, c));
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+          uint32_t q[4][K::kParts];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) split2<K::kParts>(lo_of(uw[e]) * wgt, hi_of(uw[e]) * wgt, q[e]);
+#pragma unroll
+          for (int part = 0; part < K::kParts; ++part)
+            sts16(base + K::kOffV + part * kTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&bar.vp, lane);
+        if (full_pass) {
+          if (have && !(ok = epilogue())) break;
+          have = true;
+          pw = w;
+          pit = it;
+          pend.row_factor = rev ? back : fwd;
+          pend.token = row < len ? w.start + static_cast<int64_t>(chunk) * kC + row : -1;
+        }
+      }
+    }
+    if (ok && have) ok = epilogue();
+  } else if (warp == 12) {
+    // ---------------- TMA
+    if (lane == 0) {
+      for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+        Item w;
+        item_of(args, idx, &w);
+        const LaJob& j = args.la.job[w.job];
+        const bool packed = args.la.cu != nullptr;
+        const int batch = packed ? 0 : w.seq;
+        const int t0 = packed ? static_cast<int>(w.start) : 0;
+        for (int p = 0; p < w.n; ++p, ++it) {
+          const int st = static_cast<int>(it % K::kStages);
+          const int chunk = j.reverse != 0 ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+          if (!(ok = mbar_wait(&bar.empty[st], ((it / K::kStages) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+          const uint32_t stage = base + st * K::kStage;
+          const int t = t0 + chunk * kC;
+          mbar_arrive_expect_tx(&bar.full[st], (full_pass ? 2 * DKB + 1 : DKB + 1) * kTile);
+          if (full_pass) {
+            for (int x = 0; x < DKB; ++x)
+              tma_load_4d(stage + x * kTile, &args.map[w.job][0], &bar.full[st], 64 * x, w.h / j.a.group, t, batch);
+          }
+          for (int x = 0; x < DKB; ++x)
+            tma_load_4d(stage + (DKB + x) * kTile, &args.map[w.job][1], &bar.full[st], 64 * x, w.h / j.b.group, t, batch);
+          tma_load_4d(stage + 2 * DKB * kTile, &args.map[w.job][2], &bar.full[st], 64 * w.slice, w.h / j.c.group, t, batch);
+        }
+      }
+      if (!ok) {  // leave no copy in flight behind an abandoned pipeline
+        for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
+          const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
+          mbar_wait(&bar.full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
+        }
+      }
+    }
+  } else if (warp == 13) {
+    // ---------------- MMA
+    if (lane == 0) {
+      const uint32_t id_ab = idesc_bf16_f32(128, 128);
+      const uint32_t id_o = idesc_bf16_f32(128, 64) | (1u << 16);               // B MN-major
+      const uint32_t id_kv = idesc_bf16_f32(128, 64) | (1u << 15) | (1u << 16);  // A and B MN-major
+      uint32_t tails = 0;
+      auto fixed = [&](const Item& w, int p) {  // whether the chunk's tail rows are zeroed first
+        const bool rev = args.la.job[w.job].reverse != 0;
+        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+        return args.la.cu != nullptr && w.len - static_cast<int64_t>(chunk) * kC < kC;
+      };
+      auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
+        const int st = static_cast<int>(n % K::kStages);
+        if (!mbar_wait(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+        if (fixed(w, p)) {
+          if (!mbar_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          ++tails;
+        }
+        tc_fence_after();
+        return true;
+      };
+      auto product_ab = [&](uint32_t n) {  // a . b of chunk n
+        const uint32_t sa = base + (n % K::kStages) * K::kStage, sb = sa + DKB * kTile;
+        const uint32_t acc = tmem + kTmP + (n & 1u) * 128u;
+#pragma unroll
+        for (uint32_t x = 0; x < DKB; ++x)
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q)
+            mma_bf16_ss(acc, desc_kmajor_sw128(sa + x * kTile + q * 32u), desc_kmajor_sw128(sb + x * kTile + q * 32u), id_ab,
+                        (x | q) != 0u ? 1u : 0u);
+        mma_commit(&bar.pacc[n & 1u]);
+      };
+      // a . b runs one chunk ahead, over item borders
+      int nidx = blockIdx.x, np = 0;  // the next chunk to start
+      Item nw{};
+      bool more = nidx < items;
+      if (more) item_of(args, nidx, &nw);
+      auto settle = [&]() {
+        while (more && np >= nw.n) {
+          nidx += gridDim.x;
+          np = 0;
+          if ((more = nidx < items)) item_of(args, nidx, &nw);
+        }
+      };
+      settle();
+      uint32_t ahead = 0;  // chunks whose tiles are known to be ready
+      auto start_next = [&]() {
+        if (!more) return true;
+        if (!ready(nw, np, ahead)) return false;
+        if (full_pass) {
+          // the buffer's last reader: the product with c two chunks before
+          if (ahead >= 2 && !mbar_wait(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          product_ab(ahead);
+        }
+        ++ahead;
+        ++np;
+        settle();
+        return true;
+      };
+      ok = start_next();
+      while (ok && it < ahead) {
+        const int st = static_cast<int>(it % K::kStages);
+        const uint32_t stage = base + st * K::kStage;
+        // state product b^T (scaled c)
+        if (!(ok = mbar_wait(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (it > 0 && !(ok = mbar_wait(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        tc_fence_after();
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) {
+          const uint64_t da = desc_mn(stage + DKB * kTile + q * 2048u, kTile);
+#pragma unroll
+          for (uint32_t part = 0; part < K::kParts; ++part)
+            mma_bf16_ss(tmem + kTmKV, da, desc_mn(base + K::kOffV + part * kTile + q * 2048u, kTile), id_kv,
+                        (part | q) != 0u ? 1u : 0u);
+        }
+        mma_commit(&bar.kv);
+        if (!(ok = start_next())) break;
+        if (full_pass) {
+          // a . S
+          if (!(ok = mbar_wait(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (it > 0 && !(ok = mbar_wait(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int part = 0; part < K::kSParts; ++part)
+#pragma unroll
+            for (uint32_t x = 0; x < DKB; ++x)
+#pragma unroll
+              for (uint32_t q = 0; q < 4; ++q)
+                mma_bf16_ss(tmem + kTmOX, desc_kmajor_sw128(stage + x * kTile + q * 32u),
+                            desc_mn(base + K::kOffS + part * K::kSTile + (x * 4u + q) * 2048u, kTile), id_o,
+                            (part | x | q) != 0u ? 1u : 0u);
+          mma_commit(&bar.qs);
+          // (decayed a . b) c
+          const uint32_t b = it & 1u;
+          if (!(ok = mbar_wait(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          tc_fence_after();
+#pragma unroll
+          for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q)
+              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + part * 64u + q * 8u,
+                          desc_mn(stage + 2 * DKB * kTile + q * 2048u, kTile), id_o, (part | q) != 0u ? 1u : 0u);
+          mma_commit(&bar.o);
+        }
+        mma_commit(&bar.empty[st]);
+        ++it;
+      }
+      mma_commit(&bar.drained);  // arrives once everything issued above has completed
+    }
+  } else {
+    // ---------------- decay tables: lane l of block b is token 32 b + l
+    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+      Item w;
+      item_of(args, idx, &w);
+      const bool rev = args.la.job[w.job].reverse != 0;
+      const bool packed = args.la.cu != nullptr;
+      const int64_t g0 = (packed ? 0 : w.seq) * args.la.g_sb + (packed ? w.start : 0) * args.la.g_st + w.h * args.la.g_sh;
+      float next[4];
+      auto fetch = [&](int p) {
+        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t t = static_cast<int64_t>(chunk) * kC + 32 * q + lane;
+          float x = 0.0f;  // past the sequence: no decay
+          if (t < w.len) {
+            const int64_t at = g0 + t * args.la.g_st;
+            x = args.la.g_f32 != 0 ? __ldg(reinterpret_cast<const float*>(args.la.g) + at)
+                                   : bf16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(args.la.g) + at));
+          }
+          next[q] = x;
+        }
+      };
+      if (w.n > 0) fetch(0);
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u;
+        float lg[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float x = next[q] * 1.44269504088896340736f;  // log2 e
+          lg[q] = x < -150.0f ? -150.0f : x;                  // a NaN stays
+        }
+        if (p + 1 < w.n) fetch(p + 1);
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float u = __shfl_up_sync(0xFFFFFFFFu, lg[q], off);
+            if (lane >= off) lg[q] += u;
+          }
+        }
+        if (!(ok = warp_wait(&bar.gfree[b], ((it >> 1) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+        DecayTable& t = tables[b];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float total = __shfl_sync(0xFFFFFFFFu, lg[q], 31);
+          t.lg[32 * q + lane] = lg[q];
+          t.cf[32 * q + lane] = ex2(rev ? lg[q] : total - lg[q]);
+          if (lane == q) t.total[q] = total;
+        }
+        warp_arrive(&bar.gfull[b], lane);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    // no MMA may still write the accumulators when they are freed
+    if (lane == 0) mbar_wait(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmCols);
+  }
+}
+
+// Segment states from zero -> each segment's first state, in place.
+__global__ void __launch_bounds__(256) la_chain_kernel(const __grid_constant__ LaChunkArgs args) {
+  const int lane_id = blockIdx.x;
+  Item w;
+  item_of(args, lane_id, &w);
+  const LaJob& j = args.la.job[w.job];
+  const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
+  float* seg = args.seg_state + static_cast<int64_t>(lane_id) * args.nseg * 8192;
+  for (int i = (blockIdx.y * 256 + threadIdx.x) * 4; i < j.da * 64; i += gridDim.y * 1024) {
+    const int r = i / 64, c = w.slice * 64 + (i & 63);
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x[e] = j.init != nullptr && c + e < j.dc ? j.init_scale * j.init[st0 + r * j.s_row + (c + e) * j.s_col] : 0.0f;
+    for (int s = 0; s < args.nseg; ++s) {
+      float4* p = reinterpret_cast<float4*>(seg + static_cast<int64_t>(s) * 8192 + i);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float d = 0.0f;
+      if (s + 1 < args.nseg) {
+        v = *p;
+        d = args.seg_decay[static_cast<int64_t>(lane_id) * args.nseg + s];
+      }
+      *p = make_float4(x[0], x[1], x[2], x[3]);
+      x[0] = fmaf(d, x[0], v.x);
+      x[1] = fmaf(d, x[1], v.y);
+      x[2] = fmaf(d, x[2], v.z);
+      x[3] = fmaf(d, x[3], v.w);
+    }
+  }
+}
+
+namespace {
+
+int64_t lanes_of(const LaArgs& a, int (&slices)[3], int64_t (&first)[4]) {
+  int64_t n = 0;
+  for (int i = 0; i < a.njobs; ++i) {
+    slices[i] = (a.job[i].dc + 63) / 64;
+    first[i] = n;
+    n += static_cast<int64_t>(a.nseq) * a.H * slices[i];
+  }
+  first[a.njobs] = n;
+  return n;
+}
+
+// Segments per sequence that leave the shortest time, in units of one chunk
+// of the full pass (the state-only pass costs about 0.6 of it, the chaining and
+// the two extra launches about ten).
+int segments_for(int64_t lanes, int64_t tokens, int sms) {
+  const int64_t chunks = (tokens + kC - 1) / kC;
+  auto waves = [&](int64_t n) { return (n + sms - 1) / sms; };
+  int best = 1;
+  double least = static_cast<double>(waves(lanes) * chunks);
+  for (int s = 2; s <= 64 && s <= chunks; ++s) {
+    const int64_t per = (chunks + s - 1) / s;
+    const double t = static_cast<double>(waves(lanes * s) * per) + 0.6 * static_cast<double>(waves(lanes * (s - 1)) * per) + 10.0;
+    if (t < 0.95 * least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total + a.nseq - 1) / (a.nseq > 0 ? a.nseq : 1); }
+
+}  // namespace
+
+size_t la_chunk_workspace(const LaArgs& a) {
+  int slices[3];
+  int64_t first[4];
+  const int64_t lanes = lanes_of(a, slices, first);
+  const int nseg = segments_for(lanes, mean_tokens(a), device_sm_count());
+  return nseg == 1 ? 0 : static_cast<size_t>(lanes) * nseg * (8192 + 1) * sizeof(float);
+}
+
+int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream) {
+  LaChunkArgs c{};
+  int64_t first[4];
+  const int64_t lanes = lanes_of(a, c.slices, first);
+  if (lanes == 0) return SPX_OK;
+  const int sms = device_sm_count();
+  c.nseg = segments_for(lanes, mean_tokens(a), sms);
+  if (lanes * c.nseg > 0x7FFFFFFF) return SPX_ERR_UNSUPPORTED;
+  c.la = a;
+  int dkb = 1;
+  for (int i = 0; i < a.njobs; ++i) {
+    const LaJob& j = a.job[i];
+    if (j.da > 64) dkb = 2;
+    const LaOperand* op[3] = {&j.a, &j.b, &j.c};
+    const int width[3] = {j.da, j.da, j.dc};
+    for (int x = 0; x < 3; ++x) {
+      if (a.total == 0) continue;  // only empty sequences: no tile is loaded
+      if (int rc = encode_heads(&c.map[i][x], op[x]->p, width[x], a.H / op[x]->group, a.cu != nullptr ? a.total : a.T,
+                                a.cu != nullptr ? 1 : a.nseq, op[x]->sh, op[x]->st, op[x]->sb, kC);
+          rc != SPX_OK)
+        return rc;
+    }
+  }
+  for (int i = 0; i <= a.njobs; ++i) c.lanes[i] = static_cast<int>(first[i]);
+  if (c.nseg > 1) {
+    if (workspace == nullptr) return SPX_ERR_WORKSPACE;
+    c.seg_state = static_cast<float*>(workspace);
+    c.seg_decay = c.seg_state + lanes * c.nseg * 8192;
+  }
+  auto run = [&](auto kernel, size_t smem) {
+    if (int rc = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel)); rc != SPX_OK) return rc;
+    const int64_t items = lanes * c.run_segs;
+    kernel<<<static_cast<unsigned>(std::min<int64_t>(items, sms)), kLaThreads, smem, stream>>>(c);
+    return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
+  };
+  auto pass = [&]() {
+    if (dkb == 1)
+      return precise ? run(la_chunk_kernel<1, true>, Cfg<1, true>::kBytes) : run(la_chunk_kernel<1, false>, Cfg<1, false>::kBytes);
+    return precise ? run(la_chunk_kernel<2, true>, Cfg<2, true>::kBytes) : run(la_chunk_kernel<2, false>, Cfg<2, false>::kBytes);
+  };
+  if (c.nseg > 1) {
+    c.state_only = 1;
+    c.run_segs = c.nseg - 1;
+    if (int rc = pass(); rc != SPX_OK) return rc;
+    la_chain_kernel<<<dim3(static_cast<unsigned>(lanes), 2), 256, 0, stream>>>(c);
+    if (cudaGetLastError() != cudaSuccess) return SPX_ERR_CUDA;
+  }
+  c.state_only = 0;
+  c.run_segs = c.nseg;
+  return pass();
+}
+
+}  // namespace spx

@@ -64,8 +64,35 @@ LaArgs base_args(const spx_linattn_dims& d, const spx_decays* g, const int32_t* 
 
 int slices_of(int width) { return (width + 63) / 64; }
 
+template <typename T>
+T* at(void* base, size_t off) {
+  return reinterpret_cast<T*>(static_cast<uint8_t*>(base) + off);
+}
+
+// A few tokens go one by one: the chunked form would pad them to 128.
+constexpr int64_t kRecurrentMax = 8;
+bool recurrent(const LaArgs& a) { return a.cu == nullptr && a.T <= kRecurrentMax; }
+
+// The widths, counts and lengths alone, for workspace sizes.
+LaArgs shape_args(const spx_linattn_dims& d, bool backward) {
+  static const int32_t some = 0;
+  const spx_decays none{};
+  LaArgs a = base_args(d, &none, &some, nullptr);
+  a.njobs = backward ? 3 : 1;
+  a.job[0].dc = backward ? d.key_dim : d.value_dim;
+  a.job[1].dc = d.key_dim;
+  a.job[2].dc = d.value_dim;
+  return a;
+}
+
+size_t jobs_workspace(const LaArgs& a) { return a.nseq == 0 || recurrent(a) ? 0 : la_chunk_workspace(a); }
+
+int run_jobs(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream) {
+  return recurrent(a) ? launch_la_recurrent(a, stream) : launch_la_chunk(a, precise, workspace, stream);
+}
+
 struct BackwardLayout {
-  size_t q_dots, k_dots, last, dk, dv, total;
+  size_t q_dots, k_dots, last, dk, dv, segments, total;
 };
 
 BackwardLayout backward_layout(const spx_linattn_dims& d) {
@@ -85,16 +112,10 @@ BackwardLayout backward_layout(const spx_linattn_dims& d) {
     L.dk = take(n * h * d.key_dim * 4);
     L.dv = take(n * h * d.value_dim * 4);
   }
+  L.segments = take(jobs_workspace(shape_args(d, true)));
   L.total = off;
   return L;
 }
-
-template <typename T>
-T* at(void* base, size_t off) {
-  return reinterpret_cast<T*>(static_cast<uint8_t*>(base) + off);
-}
-
-int run_jobs(const LaArgs& a, cudaStream_t stream) { return launch_la_recurrent(a, stream); }
 
 }  // namespace
 
@@ -210,7 +231,7 @@ int spx_rotary(const spx_heads* q, int32_t q_heads, const spx_heads* k, int32_t 
 
 size_t spx_linear_attention_workspace(const spx_linattn_dims* dims) {
   if (check_dims(dims) != SPX_OK) return 0;
-  return 0;
+  return jobs_workspace(shape_args(*dims, false));
 }
 
 int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const spx_heads* k, const spx_heads* v,
@@ -229,7 +250,9 @@ int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const
     return SPX_ERR_INVALID_ARG;
   }
   if (!aligned(out) || !aligned(initial_state) || !aligned(final_state)) return SPX_ERR_ALIGNMENT;
-  if (workspace_bytes < spx_linear_attention_workspace(dims)) return SPX_ERR_WORKSPACE;
+  const size_t need = spx_linear_attention_workspace(dims);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SPX_ERR_WORKSPACE;
+  if (!aligned(workspace)) return SPX_ERR_ALIGNMENT;
   const int group = d.heads / d.kv_heads;
   LaArgs a = base_args(d, decays, cu_seqlens, status);
   LaJob& j = a.job[0];
@@ -245,7 +268,7 @@ int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const
   j.s_row = d.value_dim;
   j.s_col = 1;
   j.init_scale = j.fin_scale = 1.0f;
-  return run_jobs(a, as_stream(stream));
+  return run_jobs(a, false, workspace, as_stream(stream));
 }
 
 size_t spx_linear_attention_backward_workspace(const spx_linattn_dims* dims) {
@@ -330,11 +353,11 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   jv.s_col = 1;
   jv.init_scale = 1.0f / d.scale;
   jv.fin_scale = d.scale;
-  if (int rc = run_jobs(a, st); rc != SPX_OK) return rc;
+  if (int rc = run_jobs(a, true, at<void>(workspace, L.segments), st); rc != SPX_OK) return rc;
   LaDecayGradArgs g{};
   g.q_dots = jq.dots;
   g.k_dots = jk.dots;
-  g.q_slices = g.k_slices = 1;
+  g.q_slices = g.k_slices = recurrent(a) ? 1 : slices_of(K);
   g.last = jq.fin;
   g.d_last = d_final_state;
   g.dg = d_decay;
