@@ -137,9 +137,35 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float lo_of(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_of(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
 
+// mbar_wait whose polls sleep up to 20 us each: most of this kernel's warps wait
+// at any time, and polling at full speed takes the issue slots of those that work.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status, int code) {
+  const uint32_t addr = smem_u32(bar);
+  auto poll = [&]() {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity), "r"(20000u)
+        : "memory");
+    return done != 0u;
+  };
+  if (poll()) return true;
+  const uint64_t start = global_ns();
+  while (!poll()) {
+    if (global_ns() - start > SPX_WAIT_NS) {
+      record_error(status, code);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Every lane polls; the warp goes on together, or gives up together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, status, code)) != 0;
+  return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, status, code)) != 0;
 }
 
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -292,88 +318,63 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const DecayTable& t = tables[b];
         if (!(ok = warp_wait(&bar.gfull[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const float lg = t.lg[row];
-        // factor of a whole off-diagonal block, between this row and the block's near edge
-        float rf[4];
-        {
-          float run = rev ? t.total[quad] - lg : lg;
-          if (!rev) {
-#pragma unroll
-            for (int j = 3; j >= 0; --j)
-              if (j < quad) {
-                rf[j] = ex2(run);
-                run += t.total[j];
-              }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j > quad) {
-                rf[j] = ex2(run);
-                run += t.total[j];
-              }
-          }
-        }
         if (!(ok = warp_wait(&bar.pacc[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
+        // The operand takes the accumulator's place, block by block: 32 FP32 columns
+        // become 16 of BF16 pairs (PRECISE: 16 more of their second parts).
+        // From the diagonal block outwards; `run` is the decay between this row and
+        // the near edge of the block.  One copy of the code serves all blocks: a warp
+        // passes through it once a chunk, so its size is fetched, not cached.
         const uint32_t acc = tmem + kTmP + b * 128u + tm_lane;
-        constexpr int kLo = PRECISE ? 2 : 1;
-        // one 32-column block: TMEM -> kLo x 16 packed words
-        auto block = [&](int j, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
-          if (rev ? j < quad : j > quad) {
+        float run = rev ? t.total[quad] - lg : lg;
+#pragma unroll 1
+        for (int n = 0; n < 4; ++n) {
+          const int j = rev ? (quad + n) & 3 : (quad - n) & 3;
+          const bool zero = rev ? j < quad : j > quad;
+          uint32_t s[32];
+          if (!zero) {
+            tmem_ld32(acc + 32u * j, s);
+            tmem_wait_ld();
+          }
+          uint32_t hi[16], lo[16];
+          if (zero) {
 #pragma unroll
             for (int q = 0; q < 16; ++q) hi[q] = lo[q] = 0u;
-            return;
-          }
-          uint32_t s[32];
-          tmem_ld32(acc + 32u * j, s);
-          tmem_wait_ld();
-          const float4* f4 = reinterpret_cast<const float4*>(j == quad ? t.lg + 32 * j : t.cf + 32 * j);
+          } else {
+            float f[32];
+            const float4* f4 = reinterpret_cast<const float4*>(n == 0 ? t.lg + 32 * j : t.cf + 32 * j);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float4 f = f4[q];
-            float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int c = 4 * q + e;
-              const float x = __uint_as_float(s[c]);
-              if (j == quad)  // lane = the row inside the block; a masked entry is zero whatever it holds
-                v[e] = (rev ? c >= lane : c <= lane) ? x * ex2(rev ? v[e] - lg : lg - v[e]) : 0.0f;
-              else
-                v[e] = x * (v[e] * rf[j]);
+            for (int q = 0; q < 8; ++q) {
+              const float4 v = f4[q];
+              f[4 * q] = v.x, f[4 * q + 1] = v.y, f[4 * q + 2] = v.z, f[4 * q + 3] = v.w;
             }
-            uint32_t p0[kLo], p1[kLo];
-            split2<kLo>(v[0], v[1], p0);
-            split2<kLo>(v[2], v[3], p1);
-            hi[2 * q] = p0[0];
-            hi[2 * q + 1] = p1[0];
-            if constexpr (PRECISE) {
-              lo[2 * q] = p0[1];
-              lo[2 * q + 1] = p1[1];
+            if (n == 0) {  // lane = the row inside the block
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const float d = rev ? f[c] - lg : lg - f[c];
+                f[c] = ex2((rev ? c >= lane : c <= lane) ? d : 0.0f);
+              }
+            } else {
+              const float rf = ex2(run);
+              run += t.total[j];
+#pragma unroll
+              for (int c = 0; c < 32; ++c) f[c] *= rf;
+            }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              float x = __uint_as_float(s[2 * q]) * f[2 * q], y = __uint_as_float(s[2 * q + 1]) * f[2 * q + 1];
+              if (n == 0) {  // a masked entry is zero whatever it holds
+                x = (rev ? 2 * q >= lane : 2 * q <= lane) ? x : 0.0f;
+                y = (rev ? 2 * q + 1 >= lane : 2 * q + 1 <= lane) ? y : 0.0f;
+              }
+              uint32_t part[PRECISE ? 2 : 1];
+              split2<PRECISE ? 2 : 1>(x, y, part);
+              hi[q] = part[0];
+              lo[q] = PRECISE ? part[PRECISE ? 1 : 0] : 0u;
             }
           }
-        };
-        // The operand (64 columns, PRECISE: 128) takes the accumulator's place: a
-        // block is written only where every accumulator column under it has been read.
-        if constexpr (!PRECISE) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            block(j, hi, lo);
-            tmem_st16(acc + 16u * j, hi);
-          }
-        } else {
-          uint32_t h2[16], l2[16], h3[16], l3[16], hi[16], lo[16];
-          block(2, h2, l2);
-          block(3, h3, l3);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            block(j, hi, lo);
-            tmem_st16(acc + 16u * j, hi);
-            tmem_st16(acc + 64u + 16u * j, lo);
-          }
-          tmem_st16(acc + 32u, h2);
-          tmem_st16(acc + 96u, l2);
-          tmem_st16(acc + 48u, h3);
-          tmem_st16(acc + 112u, l3);
+          tmem_st16(acc + 32u * j, hi);
+          if constexpr (PRECISE) tmem_st16(acc + 32u * j + 16u, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const float wgt = rev ? fwd : back;
         // the parts' last reader: the state product of the chunk before
         if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-#pragma unroll
+#pragma unroll 2
         for (int c = 0; c < 8; ++c) {
           const uint4 u = lds16(sc + swz(row, c));
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         for (int p = 0; p < w.n; ++p, ++it) {
           const int st = static_cast<int>(it % K::kStages);
           const int chunk = j.reverse != 0 ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-          if (!(ok = mbar_wait(&bar.empty[st], ((it / K::kStages) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+          if (!(ok = wait_for(&bar.empty[st], ((it / K::kStages) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
           const uint32_t stage = base + st * K::kStage;
           const int t = t0 + chunk * kC;
           mbar_arrive_expect_tx(&bar.full[st], (full_pass ? 2 * DKB + 1 : DKB + 1) * kTile);
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       if (!ok) {  // leave no copy in flight behind an abandoned pipeline
         for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
           const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
-          mbar_wait(&bar.full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
+          wait_for(&bar.full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
         }
       }
     }
@@ -644,9 +645,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       };
       auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
         const int st = static_cast<int>(n % K::kStages);
-        if (!mbar_wait(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+        if (!wait_for(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
         if (fixed(w, p)) {
-          if (!mbar_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (!wait_for(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
         }
         tc_fence_after();
@@ -682,7 +683,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!ready(nw, np, ahead)) return false;
         if (full_pass) {
           // the buffer's last reader: the product with c two chunks before
-          if (ahead >= 2 && !mbar_wait(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (ahead >= 2 && !wait_for(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
           product_ab(ahead);
         }
         ++ahead;
@@ -695,8 +696,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t stage = base + st * K::kStage;
         // state product b^T (scaled c)
-        if (!(ok = mbar_wait(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-        if (it > 0 && !(ok = mbar_wait(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = wait_for(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (it > 0 && !(ok = wait_for(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
 #pragma unroll
         for (uint32_t q = 0; q < 8; ++q) {
@@ -710,8 +711,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!(ok = start_next())) break;
         if (full_pass) {
           // a . S
-          if (!(ok = mbar_wait(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-          if (it > 0 && !(ok = mbar_wait(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = wait_for(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (it > 0 && !(ok = wait_for(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
 #pragma unroll
           for (int part = 0; part < K::kSParts; ++part)
@@ -725,13 +726,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           mma_commit(&bar.qs);
           // (decayed a . b) c
           const uint32_t b = it & 1u;
-          if (!(ok = mbar_wait(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = wait_for(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
 #pragma unroll
           for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
 #pragma unroll
             for (uint32_t q = 0; q < 8; ++q)
-              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + part * 64u + q * 8u,
+              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + (q >> 1) * 32u + (q & 1u) * 8u + part * 16u,
                           desc_mn(stage + 2 * DKB * kTile + q * 2048u, kTile), id_o, (part | q) != 0u ? 1u : 0u);
           mma_commit(&bar.o);
         }
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   __syncthreads();
   if (warp == 13) {
     // no MMA may still write the accumulators when they are freed
-    if (lane == 0) mbar_wait(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
+    if (lane == 0) wait_for(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, kTmCols);
