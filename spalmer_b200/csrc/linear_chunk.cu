@@ -36,7 +36,7 @@
 // own first state.
 //
 // Warps: 0-3 the decayed a . b matrix (TMEM -> registers -> TMEM operand),
-// 4-7 the state, 8-11 scaled c and the epilogue, 12 TMA, 13 MMA, 14 decays.
+// 4-7 the state, 8-11 scaled c, 12-15 the epilogue, 16 TMA, 17 MMA, 18 decays.
 // Every wait is bounded (status word, then return).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -54,7 +54,7 @@ namespace {
 
 constexpr int kC = 128;              // tokens of a chunk
 constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
-constexpr int kLaThreads = 15 * 32;
+constexpr int kLaThreads = 19 * 32;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -73,10 +73,26 @@ struct DecayTable {
   float total[4];
 };
 
-template <int DKB, bool PRECISE>
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Decay from the chunk's start to a token (inclusive), and from it to the chunk's end.
+__device__ __forceinline__ float from_start(const DecayTable& t, int quad, int row) {
+  const float x = quad == 0 ? 0.0f : quad == 1 ? t.total[0] : quad == 2 ? t.total[0] + t.total[1] : t.total[0] + t.total[1] + t.total[2];
+  return ex2(x + t.lg[row]);
+}
+__device__ __forceinline__ float to_end(const DecayTable& t, int quad, int row) {
+  const float x = quad == 3 ? 0.0f : quad == 2 ? t.total[3] : quad == 1 ? t.total[3] + t.total[2] : t.total[3] + t.total[2] + t.total[1];
+  return ex2((t.total[quad] - t.lg[row]) + x);
+}
+
+template <int DKB, bool PRECISE, int PARTS>
 struct Cfg {
   static constexpr int kStages = DKB == 1 ? 3 : 2;
-  static constexpr int kParts = PRECISE ? 2 : 3;  // of scaled c
+  static constexpr int kParts = PARTS;            // of scaled c
   static constexpr int kSParts = PRECISE ? 2 : 1; // of the state
   static constexpr uint32_t kStage = (2 * DKB + 1) * kTile;
   static constexpr uint32_t kSTile = DKB * 64 * 128;
@@ -86,7 +102,7 @@ struct Cfg {
   static constexpr uint32_t kOffBar = kOffT + 2 * sizeof(DecayTable);
   static constexpr uint32_t kBytes = kOffBar + 256;
 };
-static_assert(Cfg<2, false>::kBytes <= 232448 && Cfg<2, true>::kBytes <= 232448, "shared memory of a CTA");
+static_assert(Cfg<2, false, 3>::kBytes <= 232448 && Cfg<2, true, 2>::kBytes <= 232448, "shared memory of a CTA");
 
 struct Item {
   int job, seq, h, slice, seg, lane;
@@ -94,7 +110,7 @@ struct Item {
   int nch, p0, n;      // chunks of the sequence; this item's: p0 .. p0 + n in processing order
 };
 
-__device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
+__device__ __noinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
   const int all = a.lanes[a.la.njobs];
   it->seg = idx / all;
   it->lane = idx - it->seg * all;
@@ -123,44 +139,20 @@ __device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it)
   return ok;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float lo_of(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float hi_of(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
-
-// mbar_wait whose polls sleep up to 20 us each: most of this kernel's warps wait
-// at any time, and polling at full speed takes the issue slots of those that work.
+// mbar_wait with its timed part out of line.  The 19 warps run through a dozen
+// different loops at once, so the kernel's hot code has to stay small: what the
+// instruction cache does not hold is fetched again for every chunk (inlined
+// waits and item decoding, and unrolled blocks, once cost 12,700 cycles a chunk).
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return mbar_wait(bar, parity, status, code);
+}
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status, int code) {
-  const uint32_t addr = smem_u32(bar);
-  auto poll = [&]() {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity), "r"(20000u)
-        : "memory");
-    return done != 0u;
-  };
-  if (poll()) return true;
-  const uint64_t start = global_ns();
-  while (!poll()) {
-    if (global_ns() - start > SPX_WAIT_NS) {
-      record_error(status, code);
-      return false;
-    }
-  }
-  return true;
+  return mbar_try_wait(bar, parity) || wait_slow(bar, parity, status, code);
 }
 
 // Every lane polls; the warp goes on together, or gives up together.
@@ -182,6 +174,16 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// One lane of the warp.  The MMA role branches on this and not on a lane number:
+// only then is the branch known to be one thread's, and descriptors go to the
+// uniform registers that the instruction wants directly -- an MMA of 64, 128 or
+// 256 columns then issues every 48, 64 or 126 cycles, else every 75 at best.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0u;
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]^T, BF16: A holds two K elements per column.
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -193,13 +195,10 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -230,15 +229,54 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t x, uint32_t y, uin
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// Split two floats into NP packed BF16 parts, each the rounding of what the ones before leave.
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y) { return pair(__uint_as_float(x), __uint_as_float(y)); }
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Two floats as NP packed BF16 parts whose sum they are: one part is the
+// rounding, two leave 2^-18 of the value, three are exact (three truncations of
+// eight bits each).
 template <int NP>
-__device__ __forceinline__ void split2(float x, float y, uint32_t (&part)[NP]) {
+__device__ __forceinline__ void split2(uint64_t v, uint32_t (&part)[NP]) {
+  float x, y;
+  unpair(v, x, y);
+  if constexpr (NP < 3) {
+    part[0] = pack_bf16(x, y);
+    if constexpr (NP == 2) {
+      unpair(add2(v, pair((part[0] << 16) ^ 0x80000000u, (part[0] & 0xFFFF0000u) ^ 0x80000000u)), x, y);
+      part[1] = pack_bf16(x, y);
+    }
+  } else {
 #pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    part[p] = pack_bf16(x, y);
-    if (p + 1 < NP) {
-      x -= lo_of(part[p]);
-      y -= hi_of(part[p]);
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
+      part[p] = __byte_perm(ux, uy, 0x7632);
+      if (p < 2) {
+        v = add2(v, pair((ux & 0xFFFF0000u) ^ 0x80000000u, (uy & 0xFFFF0000u) ^ 0x80000000u));
+        unpair(v, x, y);
+      }
     }
   }
 }
@@ -255,9 +293,9 @@ static_assert(sizeof(Bars) <= 256, "barriers");
 
 }  // namespace
 
-template <int DKB, bool PRECISE>
+template <int DKB, bool PRECISE, int PARTS>
 __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_constant__ LaChunkArgs args) {
-  using K = Cfg<DKB, PRECISE>;
+  using K = Cfg<DKB, PRECISE, PARTS>;
   extern __shared__ __align__(1024) uint8_t la_smem[];
   const uint32_t base = smem_u32(la_smem);
   int* const status = args.la.status;
@@ -267,7 +305,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   }
   Bars& bar = *reinterpret_cast<Bars*>(la_smem + K::kOffBar);
   DecayTable* const tables = reinterpret_cast<DecayTable*>(la_smem + K::kOffT);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform to the compiler
   const bool full_pass = args.state_only == 0;
   const int items = args.lanes[args.la.njobs] * args.run_segs;
 
@@ -278,7 +316,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.gfull[s], 1);
-      mbar_init(&bar.gfree[s], full_pass ? 12 : 8);
+      mbar_init(&bar.gfree[s], full_pass ? 16 : 8);
       mbar_init(&bar.pacc[s], 1);
       mbar_init(&bar.pop[s], 4);
       mbar_init(&bar.tail[s], 4);
@@ -293,7 +331,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     mbar_init(&bar.drained, 1);
     fence_mbar_init();
   }
-  if (warp == 13) {
+  if (warp == 17) {
     tmem_alloc(&bar.tmem, kTmCols);
     tmem_relinquish();
   }
@@ -320,61 +358,75 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const float lg = t.lg[row];
         if (!(ok = warp_wait(&bar.pacc[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        // The operand takes the accumulator's place, block by block: 32 FP32 columns
-        // become 16 of BF16 pairs (PRECISE: 16 more of their second parts).
-        // From the diagonal block outwards; `run` is the decay between this row and
-        // the near edge of the block.  One copy of the code serves all blocks: a warp
-        // passes through it once a chunk, so its size is fetched, not cached.
+        // The operand takes the accumulator's place: 16 FP32 columns become 8 of BF16
+        // pairs (PRECISE: 8 more of their second parts).  From the diagonal block
+        // outwards; `run` is the decay between this row and the near edge of the block.
         const uint32_t acc = tmem + kTmP + b * 128u + tm_lane;
-        float run = rev ? t.total[quad] - lg : lg;
+        const float own = t.total[quad];
+        // inside the diagonal block the two factors are on either side of 1; a block
+        // that decays by more than 2^100 takes the exponential of each difference
+        float run = rev ? -lg : lg - own;
+        const bool steep = !(own >= -100.0f);
+        const int first = 2 * quad;
+        const int live = 2 * (rev ? 4 - quad : quad + 1);  // groups of 16 columns that are not all masked
+        uint32_t x[16];
+        tmem_ld16(acc + 16u * first, x);
+        float rf = 0.0f;
 #pragma unroll 1
-        for (int n = 0; n < 4; ++n) {
-          const int j = rev ? (quad + n) & 3 : (quad - n) & 3;
-          const bool zero = rev ? j < quad : j > quad;
-          uint32_t s[32];
-          if (!zero) {
-            tmem_ld32(acc + 32u * j, s);
-            tmem_wait_ld();
-          }
-          uint32_t hi[16], lo[16];
-          if (zero) {
+        for (int n = 0; n < 8; ++n) {
+          const int g = ((rev ? first + (n & ~1) : first - (n & ~1)) & 7) + (n & 1);
+          uint32_t hi[8], lo[8];
+          if (n >= live) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) hi[q] = lo[q] = 0u;
+            for (int q = 0; q < 8; ++q) hi[q] = lo[q] = 0u;
           } else {
-            float f[32];
-            const float4* f4 = reinterpret_cast<const float4*>(n == 0 ? t.lg + 32 * j : t.cf + 32 * j);
+            tmem_wait_ld();
+            uint32_t y[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) y[q] = x[q];
+            if (n + 1 < live) {
+              const int g1 = ((rev ? first + ((n + 1) & ~1) : first - ((n + 1) & ~1)) & 7) + ((n + 1) & 1);
+              tmem_ld16(acc + 16u * g1, x);
+            }
+            if ((n & 1) == 0) {
+              rf = ex2(run);
+              run += t.total[g >> 1];
+            }
+            uint64_t v[8];
+            if (n < 2 && steep) {
+              const float sg = rev ? 1.0f : -1.0f;
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                v[q] = mul2(pair(y[2 * q], y[2 * q + 1]), pair(ex2((t.lg[16 * g + 2 * q] - lg) * sg), ex2((t.lg[16 * g + 2 * q + 1] - lg) * sg)));
+            } else {
+              const uint64_t rf2 = pair(rf, rf);
+              const ulonglong2* f4 = reinterpret_cast<const ulonglong2*>(t.cf + 16 * g);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const ulonglong2 f = f4[q];
+                v[2 * q] = mul2(pair(y[4 * q], y[4 * q + 1]), mul2(f.x, rf2));
+                v[2 * q + 1] = mul2(pair(y[4 * q + 2], y[4 * q + 3]), mul2(f.y, rf2));
+              }
+            }
+            if (n < 2) {  // the diagonal block: a masked entry is zero whatever it holds
+              const int d = lane - 16 * (g & 1);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                float a, c;
+                unpair(v[q], a, c);
+                v[q] = pair((rev ? 2 * q >= d : 2 * q <= d) ? a : 0.0f, (rev ? 2 * q + 1 >= d : 2 * q + 1 <= d) ? c : 0.0f);
+              }
+            }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-              const float4 v = f4[q];
-              f[4 * q] = v.x, f[4 * q + 1] = v.y, f[4 * q + 2] = v.z, f[4 * q + 3] = v.w;
-            }
-            if (n == 0) {  // lane = the row inside the block
-#pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const float d = rev ? f[c] - lg : lg - f[c];
-                f[c] = ex2((rev ? c >= lane : c <= lane) ? d : 0.0f);
-              }
-            } else {
-              const float rf = ex2(run);
-              run += t.total[j];
-#pragma unroll
-              for (int c = 0; c < 32; ++c) f[c] *= rf;
-            }
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              float x = __uint_as_float(s[2 * q]) * f[2 * q], y = __uint_as_float(s[2 * q + 1]) * f[2 * q + 1];
-              if (n == 0) {  // a masked entry is zero whatever it holds
-                x = (rev ? 2 * q >= lane : 2 * q <= lane) ? x : 0.0f;
-                y = (rev ? 2 * q + 1 >= lane : 2 * q + 1 <= lane) ? y : 0.0f;
-              }
               uint32_t part[PRECISE ? 2 : 1];
-              split2<PRECISE ? 2 : 1>(x, y, part);
+              split2<PRECISE ? 2 : 1>(v[q], part);
               hi[q] = part[0];
-              lo[q] = PRECISE ? part[PRECISE ? 1 : 0] : 0u;
+              lo[q] = part[PRECISE ? 1 : 0];
             }
           }
-          tmem_st16(acc + 32u * j, hi);
-          if constexpr (PRECISE) tmem_st16(acc + 32u * j + 16u, lo);
+          tmem_st8(acc + 16u * g, hi);
+          if constexpr (PRECISE) tmem_st8(acc + 16u * g + 8u, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -403,10 +455,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           s[4 * q] = v.x, s[4 * q + 1] = v.y, s[4 * q + 2] = v.z, s[4 * q + 3] = v.w;
         }
       } else {
-        const bool some = j.init != nullptr && args.nseg == 1 && live;
+        const float* f = j.init + st0 + row * j.s_row + col0 * j.s_col;
+        const int n = j.init != nullptr && args.nseg == 1 && live ? j.dc - col0 : 0;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          s[c] = some && col0 + c < j.dc ? j.init_scale * j.init[st0 + row * j.s_row + (col0 + c) * j.s_col] : 0.0f;
+        for (int c = 0; c < 64; ++c, f += j.s_col) s[c] = c < n ? j.init_scale * *f : 0.0f;
       }
       float decay = 1.0f;
       auto write_operand = [&]() {  // BF16 parts of the state for the next chunk's a . S
@@ -415,7 +467,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           for (int c = 0; c < 8; ++c) {
             uint32_t q[4][K::kSParts];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split2<K::kSParts>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1], q[e]);
+            for (int e = 0; e < 4; ++e) split2<K::kSParts>(pair(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]), q[e]);
 #pragma unroll
             for (int part = 0; part < K::kSParts; ++part)
               sts16(base + K::kOffS + part * K::kSTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
@@ -440,12 +492,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         tc_fence_after();
         if (rows_in) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t x[32];
-            tmem_ld32(tmem + kTmKV + 32u * half + tm_lane, x);
+          for (int part = 0; part < 4; ++part) {
+            uint32_t x[16];
+            tmem_ld16(tmem + kTmKV + 16u * part + tm_lane, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) s[32 * half + c] = fmaf(gamma, s[32 * half + c], __uint_as_float(x[c]));
+            for (int c = 0; c < 16; ++c) s[16 * part + c] = fmaf(gamma, s[16 * part + c], __uint_as_float(x[c]));
           }
         }
         tc_fence_before();
@@ -461,78 +513,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
         if (threadIdx.x == 128) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
+        float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
+        const int n = j.dc - col0;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (col0 + c < j.dc) j.fin[st0 + row * j.s_row + (col0 + c) * j.s_col] = j.fin_scale * s[c];
+        for (int c = 0; c < 64; ++c, f += j.s_col)
+          if (c < n) *f = j.fin_scale * s[c];
       }
     }
   } else if (warp < 12) {
-    // ---------------- scaled c, and the epilogue one chunk behind it
+    // ---------------- scaled c
     uint32_t tails = 0;
-    struct Pending {
-      float row_factor;
-      int64_t token;  // flattened; < 0: nothing to store
-    } pend{};
-    Item pw{};
-    uint32_t pit = 0;
-    bool have = false;
-    auto epilogue = [&]() {  // chunk `pit` of item `pw`
-      const LaJob& j = args.la.job[pw.job];
-      const bool in = pend.token >= 0;
-      const int col0 = pw.slice * 64;
-      const int valid = min(64, j.dc - col0);  // a multiple of 8
-      uint4 e[8];
-      if (j.e.p != nullptr && in) {
-        const bool packed = args.la.cu != nullptr;
-        const uint16_t* pe = j.e.p + (packed ? 0 : pw.seq) * j.e.sb +
-                             (packed ? pend.token : pend.token - pw.start) * j.e.st + (pw.h / j.e.group) * j.e.sh + col0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (8 * q < valid) e[q] = __ldg(reinterpret_cast<const uint4*>(pe) + q);
-      }
-      if (!warp_wait(&bar.o, pit & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
-      tc_fence_after();
-      const float sc = args.la.scale, sx = args.la.scale * pend.row_factor;
-      const int64_t at = (pend.token * args.la.H + pw.h) * j.dc + col0;
-      float dot = 0.0f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t x[32], y[32];
-        tmem_ld32(tmem + kTmOI + 32u * half + tm_lane, x);
-        tmem_ld32(tmem + kTmOX + 32u * half + tm_lane, y);
-        tmem_wait_ld();
-        if (half == 1) {
-          tc_fence_before();
-          warp_arrive(&bar.ofree, lane);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = fmaf(sx, __uint_as_float(y[8 * q + i]), sc * __uint_as_float(x[8 * q + i]));
-          const int c = 32 * half + 8 * q;
-          if (!in || c >= valid) continue;
-          if (j.out_f32 != 0) {
-            float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(j.out) + at + c);
-            o[0] = make_float4(v[0], v[1], v[2], v[3]);
-            o[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at + c) =
-                make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-          }
-          if (j.e.p != nullptr) {
-            const uint4 u = e[4 * half + q];
-            const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dot = fmaf(v[2 * i], lo_of(ew[i]), fmaf(v[2 * i + 1], hi_of(ew[i]), dot));
-          }
-        }
-      }
-      if (j.e.p != nullptr && in)
-        j.dots[(static_cast<int64_t>(pw.slice) * args.la.H + pw.h) * args.la.total + pend.token] = dot;
-      return true;
-    };
     for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
       Item w;
       item_of(args, idx, &w);
@@ -557,21 +547,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           warp_arrive(&bar.tail[tails++ & 1u], lane);
         }
         if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        float fwd, back;  // decay from the chunk's start to this token, from it to the chunk's end
-        {
-          const DecayTable& t = tables[b];
-          float before = 0.0f, after = 0.0f;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            before += q < quad ? t.total[q] : 0.0f;
-            after += q > quad ? t.total[q] : 0.0f;
-          }
-          const float lg = t.lg[row];
-          fwd = ex2(before + lg);
-          back = ex2((t.total[quad] - lg) + after);
-        }
+        const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
         warp_arrive(&bar.gfree[b], lane);
-        const float wgt = rev ? fwd : back;
+        const uint64_t wgt2 = pair(wgt, wgt);
         // the parts' last reader: the state product of the chunk before
         if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
 #pragma unroll 2
@@ -580,25 +558,105 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
           uint32_t q[4][K::kParts];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) split2<K::kParts>(lo_of(uw[e]) * wgt, hi_of(uw[e]) * wgt, q[e]);
+          for (int e = 0; e < 4; ++e) split2<K::kParts>(mul2(pair(uw[e] << 16, uw[e] & 0xFFFF0000u), wgt2), q[e]);
 #pragma unroll
           for (int part = 0; part < K::kParts; ++part)
             sts16(base + K::kOffV + part * kTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
         }
         fence_proxy_async_smem();
         warp_arrive(&bar.vp, lane);
-        if (full_pass) {
-          if (have && !(ok = epilogue())) break;
-          have = true;
-          pw = w;
-          pit = it;
-          pend.row_factor = rev ? back : fwd;
-          pend.token = row < len ? w.start + static_cast<int64_t>(chunk) * kC + row : -1;
+      }
+    }
+  } else if (warp < 16) {
+    // ---------------- epilogue: one token of 64 columns a thread
+    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
+      Item w;
+      item_of(args, idx, &w);
+      const LaJob& j = args.la.job[w.job];
+      const bool rev = j.reverse != 0, f32 = PRECISE && j.out_f32 != 0;
+      const int col0 = w.slice * 64;
+      const int valid = min(64, j.dc - col0);  // a multiple of 8
+      const bool packed = args.la.cu != nullptr;
+      const uint16_t* pe = nullptr;
+      if constexpr (PRECISE) {
+        if (j.e.p != nullptr)
+          pe = j.e.p + (packed ? 0 : w.seq) * j.e.sb + (packed ? w.start : 0) * j.e.st + (w.h / j.e.group) * j.e.sh + col0;
+      }
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u;
+        const int64_t t = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC + row;  // in the sequence
+        const bool in = t < w.len;
+        uint4 e[8];
+        if constexpr (PRECISE) {
+          if (pe != nullptr && in) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (8 * q < valid) e[q] = __ldg(reinterpret_cast<const uint4*>(pe + t * j.e.st) + q);
+          }
+        }
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const float factor = rev ? to_end(tables[b], quad, row) : from_start(tables[b], quad, row);
+        warp_arrive(&bar.gfree[b], lane);
+        const float sc = args.la.scale, sx = sc * factor;
+        const uint64_t sc2 = pair(sc, sc), sx2 = pair(sx, sx);
+        const int64_t at = ((w.start + t) * args.la.H + w.h) * j.dc + col0;
+        if (!(ok = warp_wait(&bar.o, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        uint32_t o[32];
+        uint64_t dot = 0;  // two FP32 sums
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          uint32_t x[16], y[16];
+          tmem_ld16(tmem + kTmOI + 16u * part + tm_lane, x);
+          tmem_ld16(tmem + kTmOX + 16u * part + tm_lane, y);
+          tmem_wait_ld();
+          uint64_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = fma2(sx2, pair(y[2 * i], y[2 * i + 1]), mul2(sc2, pair(x[2 * i], x[2 * i + 1])));
+            uint32_t one[1];
+            split2<1>(v[i], one);
+            o[8 * part + i] = one[0];
+          }
+          if constexpr (PRECISE) {
+            if (f32 && in) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (16 * part + 4 * q < valid)
+                  *reinterpret_cast<ulonglong2*>(reinterpret_cast<float*>(j.out) + at + 16 * part + 4 * q) =
+                      make_ulonglong2(v[2 * q], v[2 * q + 1]);
+            }
+            if (pe != nullptr && in) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                if (16 * part + 8 * q >= valid) continue;
+                const uint4 u = e[2 * part + q];
+                const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dot = fma2(v[4 * q + i], pair(ew[i] << 16, ew[i] & 0xFFFF0000u), dot);
+              }
+            }
+          }
+        }
+        // the accumulators are free before the stores: the next chunk's products wait for them
+        tc_fence_before();
+        warp_arrive(&bar.ofree, lane);
+        if (in && !f32) {
+          uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (8 * q < valid) out[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+        if constexpr (PRECISE) {
+          if (pe != nullptr && in) {
+            float d0, d1;
+            unpair(dot, d0, d1);
+            j.dots[(static_cast<int64_t>(w.slice) * args.la.H + w.h) * args.la.total + w.start + t] = d0 + d1;
+          }
         }
       }
     }
-    if (ok && have) ok = epilogue();
-  } else if (warp == 12) {
+  } else if (warp == 16) {
     // ---------------- TMA
     if (lane == 0) {
       for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
@@ -631,9 +689,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == 17) {
     // ---------------- MMA
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t id_ab = idesc_bf16_f32(128, 128);
       const uint32_t id_o = idesc_bf16_f32(128, 64) | (1u << 16);               // B MN-major
       const uint32_t id_kv = idesc_bf16_f32(128, 64) | (1u << 15) | (1u << 16);  // A and B MN-major
@@ -654,16 +712,17 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         return true;
       };
       auto product_ab = [&](uint32_t n) {  // a . b of chunk n
-        const uint32_t sa = base + (n % K::kStages) * K::kStage, sb = sa + DKB * kTile;
+        const uint32_t sa = base + (n % K::kStages) * K::kStage;
+        const uint64_t da = desc_kmajor_sw128(sa), db = desc_kmajor_sw128(sa + DKB * kTile);
         const uint32_t acc = tmem + kTmP + (n & 1u) * 128u;
-#pragma unroll
-        for (uint32_t x = 0; x < DKB; ++x)
-#pragma unroll
-          for (uint32_t q = 0; q < 4; ++q)
-            mma_bf16_ss(acc, desc_kmajor_sw128(sa + x * kTile + q * 32u), desc_kmajor_sw128(sb + x * kTile + q * 32u), id_ab,
-                        (x | q) != 0u ? 1u : 0u);
+#pragma unroll 1
+        for (uint32_t n = 0; n < 4 * DKB; ++n) {
+          const uint32_t at = ((n >> 2) * kTile + (n & 3u) * 32u) >> 4;
+          mma_bf16_ss(acc, da + at, db + at, id_ab, n != 0u ? 1u : 0u);
+        }
         mma_commit(&bar.pacc[n & 1u]);
       };
+      // Loops stay rolled: a chunk passes through each once, and what is unrolled is fetched anew every time.
       // a . b runs one chunk ahead, over item borders
       int nidx = blockIdx.x, np = 0;  // the next chunk to start
       Item nw{};
@@ -699,13 +758,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!(ok = wait_for(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
         if (it > 0 && !(ok = wait_for(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
-#pragma unroll
+        const uint64_t db = desc_mn(stage + DKB * kTile, kTile), dv = desc_mn(base + K::kOffV, kTile);
+#pragma unroll 1
         for (uint32_t q = 0; q < 8; ++q) {
-          const uint64_t da = desc_mn(stage + DKB * kTile + q * 2048u, kTile);
 #pragma unroll
           for (uint32_t part = 0; part < K::kParts; ++part)
-            mma_bf16_ss(tmem + kTmKV, da, desc_mn(base + K::kOffV + part * kTile + q * 2048u, kTile), id_kv,
-                        (part | q) != 0u ? 1u : 0u);
+            mma_bf16_ss(tmem + kTmKV, db + q * 128u, dv + (part * (kTile >> 4) + q * 128u), id_kv,
+                   (part | q) != 0u ? 1u : 0u);
         }
         mma_commit(&bar.kv);
         if (!(ok = start_next())) break;
@@ -714,26 +773,27 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           if (!(ok = wait_for(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           if (it > 0 && !(ok = wait_for(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
+          const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
+#pragma unroll 1
+          for (uint32_t n = 0; n < 4 * DKB; ++n) {
 #pragma unroll
-          for (int part = 0; part < K::kSParts; ++part)
-#pragma unroll
-            for (uint32_t x = 0; x < DKB; ++x)
-#pragma unroll
-              for (uint32_t q = 0; q < 4; ++q)
-                mma_bf16_ss(tmem + kTmOX, desc_kmajor_sw128(stage + x * kTile + q * 32u),
-                            desc_mn(base + K::kOffS + part * K::kSTile + (x * 4u + q) * 2048u, kTile), id_o,
-                            (part | x | q) != 0u ? 1u : 0u);
+            for (uint32_t part = 0; part < K::kSParts; ++part)
+              mma_bf16_ss(tmem + kTmOX, da + (((n >> 2) * kTile + (n & 3u) * 32u) >> 4),
+                     ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
+          }
           mma_commit(&bar.qs);
           // (decayed a . b) c
           const uint32_t b = it & 1u;
+          const uint64_t dc = desc_mn(stage + 2 * DKB * kTile, kTile);
           if (!(ok = wait_for(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
+#pragma unroll 1
+          for (uint32_t q = 0; q < 8; ++q) {
 #pragma unroll
-          for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
-#pragma unroll
-            for (uint32_t q = 0; q < 8; ++q)
-              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + (q >> 1) * 32u + (q & 1u) * 8u + part * 16u,
-                          desc_mn(stage + 2 * DKB * kTile + q * 2048u, kTile), id_o, (part | q) != 0u ? 1u : 0u);
+            for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
+              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + q * 16u + part * 8u, dc + q * 128u,
+                     id_o, (part | q) != 0u ? 1u : 0u);
+          }
           mma_commit(&bar.o);
         }
         mma_commit(&bar.empty[st]);
@@ -749,19 +809,22 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       const bool rev = args.la.job[w.job].reverse != 0;
       const bool packed = args.la.cu != nullptr;
       const int64_t g0 = (packed ? 0 : w.seq) * args.la.g_sb + (packed ? w.start : 0) * args.la.g_st + w.h * args.la.g_sh;
-      float next[4];
+      uint32_t next[4];  // raw: nothing of a load is used before the next chunk
+      const bool f32 = args.la.g_f32 != 0;
       auto fetch = [&](int p) {
         const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+        const int64_t t0 = static_cast<int64_t>(chunk) * kC + lane;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int64_t t = static_cast<int64_t>(chunk) * kC + 32 * q + lane;
-          float x = 0.0f;  // past the sequence: no decay
+          const int64_t t = t0 + 32 * q;
+          next[q] = 0u;  // past the sequence: no decay
           if (t < w.len) {
             const int64_t at = g0 + t * args.la.g_st;
-            x = args.la.g_f32 != 0 ? __ldg(reinterpret_cast<const float*>(args.la.g) + at)
-                                   : bf16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(args.la.g) + at));
+            if (f32)
+              next[q] = __ldg(reinterpret_cast<const uint32_t*>(args.la.g) + at);
+            else
+              next[q] = __ldg(reinterpret_cast<const uint16_t*>(args.la.g) + at);
           }
-          next[q] = x;
         }
       };
       if (w.n > 0) fetch(0);
@@ -770,7 +833,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         float lg[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float x = next[q] * 1.44269504088896340736f;  // log2 e
+          const float x = __uint_as_float(f32 ? next[q] : next[q] << 16) * 1.44269504088896340736f;  // log2 e
           lg[q] = x < -150.0f ? -150.0f : x;                  // a NaN stays
         }
         if (p + 1 < w.n) fetch(p + 1);
@@ -798,7 +861,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     // no MMA may still write the accumulators when they are freed
     if (lane == 0) wait_for(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
     __syncwarp();
@@ -917,10 +980,17 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
     kernel<<<static_cast<unsigned>(std::min<int64_t>(items, sms)), kLaThreads, smem, stream>>>(c);
     return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
   };
+  // a last state that the caller keeps is FP32 to the end; one that only feeds BF16 outputs needs two parts
+  const int parts = !precise && a.job[0].fin != nullptr ? 3 : 2;
   auto pass = [&]() {
-    if (dkb == 1)
-      return precise ? run(la_chunk_kernel<1, true>, Cfg<1, true>::kBytes) : run(la_chunk_kernel<1, false>, Cfg<1, false>::kBytes);
-    return precise ? run(la_chunk_kernel<2, true>, Cfg<2, true>::kBytes) : run(la_chunk_kernel<2, false>, Cfg<2, false>::kBytes);
+    if (dkb == 1) {
+      if (precise) return run(la_chunk_kernel<1, true, 2>, Cfg<1, true, 2>::kBytes);
+      return parts == 3 ? run(la_chunk_kernel<1, false, 3>, Cfg<1, false, 3>::kBytes)
+                        : run(la_chunk_kernel<1, false, 2>, Cfg<1, false, 2>::kBytes);
+    }
+    if (precise) return run(la_chunk_kernel<2, true, 2>, Cfg<2, true, 2>::kBytes);
+    return parts == 3 ? run(la_chunk_kernel<2, false, 3>, Cfg<2, false, 3>::kBytes)
+                      : run(la_chunk_kernel<2, false, 2>, Cfg<2, false, 2>::kBytes);
   };
   if (c.nseg > 1) {
     c.state_only = 1;
