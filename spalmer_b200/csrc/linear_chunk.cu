@@ -35,8 +35,10 @@
 // small kernel chains them, and the full pass starts every segment from its
 // own first state.
 //
-// Warps: 0-3 the decayed a . b matrix (TMEM -> registers -> TMEM operand),
-// 4-7 the state, 8-11 scaled c, 12-15 the epilogue, 16 TMA, 17 MMA, 18 decays.
+// Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
+// scaled c, 16-19 the state, 20-23 the epilogue, 24 TMA, 25 MMA, 26 decays.  One
+// warp gets through an instruction every three or four cycles here, so the
+// longer roles have two warpgroups, and registers move between warpgroups.
 // Every wait is bounded (status word, then return).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -54,7 +56,11 @@ namespace {
 
 constexpr int kC = 128;              // tokens of a chunk
 constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
-constexpr int kLaThreads = 19 * 32;
+constexpr int kLaThreads = 28 * 32;  // seven warpgroups
+constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
+// Registers of the warpgroups' threads: the launch gives each 72 (896 x 72 = 64,512 of 65,536).
+constexpr int kRegsAB = 64, kRegsC = 56, kRegsState = 128, kRegsOut = 88, kRegsRest = 40;
+static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + kRegsOut + kRegsRest <= 7 * 72, "registers of a CTA");
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -110,7 +116,7 @@ struct Item {
   int nch, p0, n;      // chunks of the sequence; this item's: p0 .. p0 + n in processing order
 };
 
-__device__ __noinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
+__device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
   const int all = a.lanes[a.la.njobs];
   it->seg = idx / all;
   it->lane = idx - it->seg * all;
@@ -144,15 +150,27 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// mbar_wait with its timed part out of line.  The 19 warps run through a dozen
-// different loops at once, so the kernel's hot code has to stay small: what the
-// instruction cache does not hold is fetched again for every chunk (inlined
-// waits and item decoding, and unrolled blocks, once cost 12,700 cycles a chunk).
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return mbar_wait(bar, parity, status, code);
-}
+// mbar_wait that counts cycles instead of reading the timer: the kernel's 28
+// warps run through a dozen loops at once, and what the instruction cache does
+// not hold is fetched again for every chunk, so its hot code has to stay small.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return mbar_try_wait(bar, parity) || wait_slow(bar, parity, status, code);
+  if (mbar_try_wait(bar, parity)) return true;
+  const int64_t start = clock64();
+  do {
+    if (mbar_try_wait(bar, parity)) return true;
+  } while (clock64() - start < kWaitCycles);
+  record_error(status, code);
+  return false;
+}
+
+// Registers move between warpgroups; every warp of one executes the same instruction.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Every lane polls; the warp goes on together, or gives up together.
@@ -174,10 +192,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// One lane of the warp.  The MMA role branches on this and not on a lane number:
-// only then is the branch known to be one thread's, and descriptors go to the
-// uniform registers that the instruction wants directly -- an MMA of 64, 128 or
-// 256 columns then issues every 48, 64 or 126 cycles, else every 75 at best.
+// One lane of the warp, the same one every time.  MMAs are issued in branches on
+// this and not on a lane number, and everything around them runs in the whole
+// warp: only then does the compiler know the branch as one thread's and the
+// descriptors as uniform, and an MMA of 64, 128 or 256 columns issues every 48,
+// 64 or 126 cycles instead of every 75 and more.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -312,16 +331,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   if (threadIdx.x == 0) {
     for (int s = 0; s < 3; ++s) {
       mbar_init(&bar.full[s], 1);
-      mbar_init(&bar.empty[s], 1);
+      mbar_init(&bar.empty[s], full_pass ? 5 : 1);  // the MMAs, and the epilogue's warps
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.gfull[s], 1);
-      mbar_init(&bar.gfree[s], full_pass ? 16 : 8);
+      mbar_init(&bar.gfree[s], full_pass ? 24 : 12);
       mbar_init(&bar.pacc[s], 1);
-      mbar_init(&bar.pop[s], 4);
-      mbar_init(&bar.tail[s], 4);
+      mbar_init(&bar.pop[s], 8);
+      mbar_init(&bar.tail[s], 8);
     }
-    mbar_init(&bar.vp, 4);
+    mbar_init(&bar.vp, 8);
     mbar_init(&bar.kv, 1);
     mbar_init(&bar.kvfree, 4);
     mbar_init(&bar.sop, 4);
@@ -331,7 +350,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     mbar_init(&bar.drained, 1);
     fence_mbar_init();
   }
-  if (warp == 17) {
+  if (warp == 25) {
     tmem_alloc(&bar.tmem, kTmCols);
     tmem_relinquish();
   }
@@ -345,8 +364,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   bool ok = true;
   uint32_t it = 0;  // chunks so far, the same count in every role
 
-  if (warp < 4) {
-    // ---------------- the decayed a . b matrix
+  if (warp < 8) {
+    regs_down<kRegsAB>();
+    // ---------------- the decayed a . b matrix: 16 columns of each 32-token block
+    const int half = warp >> 2;
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
       Item w;
       item_of(args, idx, &w);
@@ -367,66 +388,57 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         // that decays by more than 2^100 takes the exponential of each difference
         float run = rev ? -lg : lg - own;
         const bool steep = !(own >= -100.0f);
-        const int first = 2 * quad;
-        const int live = 2 * (rev ? 4 - quad : quad + 1);  // groups of 16 columns that are not all masked
-        uint32_t x[16];
-        tmem_ld16(acc + 16u * first, x);
-        float rf = 0.0f;
 #pragma unroll 1
-        for (int n = 0; n < 8; ++n) {
-          const int g = ((rev ? first + (n & ~1) : first - (n & ~1)) & 7) + (n & 1);
+        for (int n = 0; n < 4; ++n) {
+          const int j = rev ? (quad + n) & 3 : (quad - n) & 3;
+          const uint32_t at = acc + 32u * j + 16u * half;
           uint32_t hi[8], lo[8];
-          if (n >= live) {
+          if (rev ? j < quad : j > quad) {
 #pragma unroll
             for (int q = 0; q < 8; ++q) hi[q] = lo[q] = 0u;
           } else {
-            tmem_wait_ld();
-            uint32_t y[16];
-#pragma unroll
-            for (int q = 0; q < 16; ++q) y[q] = x[q];
-            if (n + 1 < live) {
-              const int g1 = ((rev ? first + ((n + 1) & ~1) : first - ((n + 1) & ~1)) & 7) + ((n + 1) & 1);
-              tmem_ld16(acc + 16u * g1, x);
-            }
-            if ((n & 1) == 0) {
-              rf = ex2(run);
-              run += t.total[g >> 1];
-            }
-            uint64_t v[8];
-            if (n < 2 && steep) {
+            uint32_t x[16];
+            tmem_ld16(at, x);
+            const int c0 = 32 * j + 16 * half;
+            const float rf = ex2(run);
+            run += t.total[j];
+            uint64_t f[8];
+            if (n == 0 && steep) {
               const float sg = rev ? 1.0f : -1.0f;
 #pragma unroll
-              for (int q = 0; q < 8; ++q)
-                v[q] = mul2(pair(y[2 * q], y[2 * q + 1]), pair(ex2((t.lg[16 * g + 2 * q] - lg) * sg), ex2((t.lg[16 * g + 2 * q + 1] - lg) * sg)));
+              for (int q = 0; q < 8; ++q) f[q] = pair(ex2((t.lg[c0 + 2 * q] - lg) * sg), ex2((t.lg[c0 + 2 * q + 1] - lg) * sg));
             } else {
               const uint64_t rf2 = pair(rf, rf);
-              const ulonglong2* f4 = reinterpret_cast<const ulonglong2*>(t.cf + 16 * g);
+              const ulonglong2* f4 = reinterpret_cast<const ulonglong2*>(t.cf + c0);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const ulonglong2 f = f4[q];
-                v[2 * q] = mul2(pair(y[4 * q], y[4 * q + 1]), mul2(f.x, rf2));
-                v[2 * q + 1] = mul2(pair(y[4 * q + 2], y[4 * q + 3]), mul2(f.y, rf2));
+                const ulonglong2 v = f4[q];
+                f[2 * q] = mul2(v.x, rf2);
+                f[2 * q + 1] = mul2(v.y, rf2);
               }
             }
-            if (n < 2) {  // the diagonal block: a masked entry is zero whatever it holds
-              const int d = lane - 16 * (g & 1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = mul2(pair(x[2 * q], x[2 * q + 1]), f[q]);
+            if (n == 0) {  // the diagonal block: a masked entry is zero whatever it holds
+              const int d = lane - 16 * half;
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 float a, c;
-                unpair(v[q], a, c);
-                v[q] = pair((rev ? 2 * q >= d : 2 * q <= d) ? a : 0.0f, (rev ? 2 * q + 1 >= d : 2 * q + 1 <= d) ? c : 0.0f);
+                unpair(f[q], a, c);
+                f[q] = pair((rev ? 2 * q >= d : 2 * q <= d) ? a : 0.0f, (rev ? 2 * q + 1 >= d : 2 * q + 1 <= d) ? c : 0.0f);
               }
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               uint32_t part[PRECISE ? 2 : 1];
-              split2<PRECISE ? 2 : 1>(v[q], part);
+              split2<PRECISE ? 2 : 1>(f[q], part);
               hi[q] = part[0];
               lo[q] = part[PRECISE ? 1 : 0];
             }
           }
-          tmem_st8(acc + 16u * g, hi);
-          if constexpr (PRECISE) tmem_st8(acc + 16u * g + 8u, lo);
+          tmem_st8(at, hi);
+          if constexpr (PRECISE) tmem_st8(at + 8u, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -434,14 +446,64 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         warp_arrive(&bar.pop[b], lane);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 16) {
+    regs_down<kRegsC>();
+    const int half = warp >> 2 & 1;  // 32 of the 64 columns
+    // ---------------- scaled c
+    uint32_t tails = 0;
+    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+      Item w;
+      item_of(args, idx, &w);
+      const bool rev = args.la.job[w.job].reverse != 0;
+      for (int p = 0; p < w.n; ++p, ++it) {
+        const uint32_t b = it & 1u;
+        const int st = static_cast<int>(it % K::kStages);
+        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+        const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
+        if (!(ok = warp_wait(&bar.full[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const uint32_t stage = base + st * K::kStage;
+        const uint32_t sc = stage + 2 * DKB * kTile;
+        if (len < kC && args.la.cu != nullptr) {
+          // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
+          if (row >= len) {
+#pragma unroll
+            for (int x = 0; x < DKB + 1; ++x)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sts16(stage + (DKB + x) * kTile + row * 128 + (4 * half + c) * 16, 0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          warp_arrive(&bar.tail[tails++ & 1u], lane);
+        }
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
+        warp_arrive(&bar.gfree[b], lane);
+        const uint64_t wgt2 = pair(wgt, wgt);
+        // the parts' last reader: the state product of the chunk before
+        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+#pragma unroll 2
+        for (int c = 4 * half; c < 4 * half + 4; ++c) {
+          const uint4 u = lds16(sc + swz(row, c));
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+          uint32_t q[4][K::kParts];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) split2<K::kParts>(mul2(pair(uw[e] << 16, uw[e] & 0xFFFF0000u), wgt2), q[e]);
+#pragma unroll
+          for (int part = 0; part < K::kParts; ++part)
+            sts16(base + K::kOffV + part * kTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&bar.vp, lane);
+      }
+    }
+  } else if (warp < 20) {
+    regs_up<kRegsState>();
     // ---------------- the state: one row of da, 64 columns, in registers
     const bool rows_in = quad < 2 * DKB;
     for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
       Item w;
       const bool sound = item_of(args, idx, &w);
       const LaJob& j = args.la.job[w.job];
-      if (!sound && threadIdx.x == 128) record_error(status, SPX_DEV_BAD_TILE);
+      if (!sound && threadIdx.x == 512) record_error(status, SPX_DEV_BAD_TILE);
       float s[64];
       const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
       const int col0 = w.slice * 64;
@@ -493,11 +555,15 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (rows_in) {
 #pragma unroll
           for (int part = 0; part < 4; ++part) {
-            uint32_t x[16];
+            uint32_t x[16], y[16];
             tmem_ld16(tmem + kTmKV + 16u * part + tm_lane, x);
+            if constexpr (K::kParts == 2) tmem_ld16(tmem + kTmKV + 64u + 16u * part + tm_lane, y);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s[16 * part + c] = fmaf(gamma, s[16 * part + c], __uint_as_float(x[c]));
+            for (int c = 0; c < 16; ++c) {
+              const float add = K::kParts == 2 ? __uint_as_float(x[c]) + __uint_as_float(y[c]) : __uint_as_float(x[c]);
+              s[16 * part + c] = fmaf(gamma, s[16 * part + c], add);
+            }
           }
         }
         tc_fence_before();
@@ -511,7 +577,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
 #pragma unroll
           for (int q = 0; q < 16; ++q) f[q] = make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]);
         }
-        if (threadIdx.x == 128) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
+        if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
@@ -520,55 +586,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           if (c < n) *f = j.fin_scale * s[c];
       }
     }
-  } else if (warp < 12) {
-    // ---------------- scaled c
-    uint32_t tails = 0;
-    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
-      Item w;
-      item_of(args, idx, &w);
-      const bool rev = args.la.job[w.job].reverse != 0;
-      for (int p = 0; p < w.n; ++p, ++it) {
-        const uint32_t b = it & 1u;
-        const int st = static_cast<int>(it % K::kStages);
-        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-        const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
-        if (!(ok = warp_wait(&bar.full[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const uint32_t stage = base + st * K::kStage;
-        const uint32_t sc = stage + 2 * DKB * kTile;
-        if (len < kC && args.la.cu != nullptr) {
-          // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
-          if (row >= len) {
-#pragma unroll
-            for (int x = 0; x < DKB + 1; ++x)
-#pragma unroll
-              for (int c = 0; c < 8; ++c) sts16(stage + (DKB + x) * kTile + row * 128 + c * 16, 0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          warp_arrive(&bar.tail[tails++ & 1u], lane);
-        }
-        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
-        warp_arrive(&bar.gfree[b], lane);
-        const uint64_t wgt2 = pair(wgt, wgt);
-        // the parts' last reader: the state product of the chunk before
-        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-#pragma unroll 2
-        for (int c = 0; c < 8; ++c) {
-          const uint4 u = lds16(sc + swz(row, c));
-          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
-          uint32_t q[4][K::kParts];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) split2<K::kParts>(mul2(pair(uw[e] << 16, uw[e] & 0xFFFF0000u), wgt2), q[e]);
-#pragma unroll
-          for (int part = 0; part < K::kParts; ++part)
-            sts16(base + K::kOffV + part * kTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
-        }
-        fence_proxy_async_smem();
-        warp_arrive(&bar.vp, lane);
-      }
-    }
-  } else if (warp < 16) {
-    // ---------------- epilogue: one token of 64 columns a thread
+  } else if (warp < 24) {
+    regs_up<kRegsOut>();
+    // ---------------- epilogue: 64 columns of one token a thread
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
       Item w;
       item_of(args, idx, &w);
@@ -585,13 +605,22 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       for (int p = 0; p < w.n; ++p, ++it) {
         const uint32_t b = it & 1u;
         const int64_t t = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC + row;  // in the sequence
-        const bool in = t < w.len;
+        // Rows go through shared memory on their way to and from global memory (eight
+        // lanes a row of 128 bytes): a thread's own row would touch 32 lines an
+        // instruction and hold up every barrier and shared-memory access of the CTA.
+        // The chunk's tiles serve: their last reader is done when its output is.
+        const uint32_t stage = base + (it % K::kStages) * K::kStage;
+        const uint32_t s_e = stage, s_out = stage + DKB * kTile;
+        const int64_t t0 = t - lane + (lane >> 3);  // rows t0, t0 + 4, ... of this warp's 32
+        const int c8 = lane & 7;
         uint4 e[8];
         if constexpr (PRECISE) {
-          if (pe != nullptr && in) {
+          if (pe != nullptr) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-              if (8 * q < valid) e[q] = __ldg(reinterpret_cast<const uint4*>(pe + t * j.e.st) + q);
+              e[q] = t0 + 4 * q < w.len && 8 * c8 < valid
+                         ? __ldg(reinterpret_cast<const uint4*>(pe + (t0 + 4 * q) * j.e.st) + c8)
+                         : make_uint4(0u, 0u, 0u, 0u);
           }
         }
         if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
@@ -599,9 +628,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         warp_arrive(&bar.gfree[b], lane);
         const float sc = args.la.scale, sx = sc * factor;
         const uint64_t sc2 = pair(sc, sc), sx2 = pair(sx, sx);
-        const int64_t at = ((w.start + t) * args.la.H + w.h) * j.dc + col0;
         if (!(ok = warp_wait(&bar.o, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
+        const int r0 = quad * 32 + (lane >> 3);
+        if constexpr (PRECISE) {
+          if (pe != nullptr) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) sts16(s_e + swz(r0 + 4 * q, c8), e[q].x, e[q].y, e[q].z, e[q].w);
+            __syncwarp();
+          }
+        }
         uint32_t o[32];
         uint64_t dot = 0;  // two FP32 sums
 #pragma unroll
@@ -619,18 +655,20 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             o[8 * part + i] = one[0];
           }
           if constexpr (PRECISE) {
-            if (f32 && in) {
+            if (f32) {  // two tiles of 32 columns
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (16 * part + 4 * q < valid)
-                  *reinterpret_cast<ulonglong2*>(reinterpret_cast<float*>(j.out) + at + 16 * part + 4 * q) =
-                      make_ulonglong2(v[2 * q], v[2 * q + 1]);
+              for (int q = 0; q < 4; ++q) {
+                float z[4];
+                unpair(v[2 * q], z[0], z[1]);
+                unpair(v[2 * q + 1], z[2], z[3]);
+                sts16(s_out + (part >> 1) * kTile + swz(row, 4 * (part & 1) + q), __float_as_uint(z[0]), __float_as_uint(z[1]),
+                      __float_as_uint(z[2]), __float_as_uint(z[3]));
+              }
             }
-            if (pe != nullptr && in) {
+            if (pe != nullptr) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                if (16 * part + 8 * q >= valid) continue;
-                const uint4 u = e[2 * part + q];
+                const uint4 u = lds16(s_e + swz(row, 2 * part + q));
                 const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dot = fma2(v[4 * q + i], pair(ew[i] << 16, ew[i] & 0xFFFF0000u), dot);
@@ -641,14 +679,32 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         // the accumulators are free before the stores: the next chunk's products wait for them
         tc_fence_before();
         warp_arrive(&bar.ofree, lane);
-        if (in && !f32) {
-          uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at);
+        if (!f32) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) sts16(s_out + swz(row, q), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+        __syncwarp();
+        const int64_t stride = static_cast<int64_t>(args.la.H) * j.dc;
+        const int64_t at = (w.start + t0) * stride + w.h * j.dc + col0;
+        if (f32) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const int c = 32 * (q & 1) + 4 * c8;
+            if (t0 + 4 * (q >> 1) < w.len && c < valid)
+              *reinterpret_cast<uint4*>(reinterpret_cast<float*>(j.out) + at + 4 * (q >> 1) * stride + c) =
+                  lds16(s_out + (q & 1) * kTile + swz(r0 + 4 * (q >> 1), c8));
+          }
+        } else {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            if (8 * q < valid) out[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            if (t0 + 4 * q < w.len && 8 * c8 < valid)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at + 4 * q * stride + 8 * c8) =
+                  lds16(s_out + swz(r0 + 4 * q, c8));
         }
+        fence_proxy_async_smem();  // before the next chunk's copies land here
+        warp_arrive(&bar.empty[it % K::kStages], lane);
         if constexpr (PRECISE) {
-          if (pe != nullptr && in) {
+          if (pe != nullptr && t < w.len) {
             float d0, d1;
             unpair(dot, d0, d1);
             j.dots[(static_cast<int64_t>(w.slice) * args.la.H + w.h) * args.la.total + w.start + t] = d0 + d1;
@@ -656,7 +712,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
       }
     }
-  } else if (warp == 16) {
+  } else {
+    regs_down<kRegsRest>();
+    if (warp == 24) {
     // ---------------- TMA
     if (lane == 0) {
       for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
@@ -689,12 +747,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
       }
     }
-  } else if (warp == 17) {
+    } else if (warp == 25) {
     // ---------------- MMA
-    if (elect_one()) {
+    {
       const uint32_t id_ab = idesc_bf16_f32(128, 128);
       const uint32_t id_o = idesc_bf16_f32(128, 64) | (1u << 16);               // B MN-major
-      const uint32_t id_kv = idesc_bf16_f32(128, 64) | (1u << 15) | (1u << 16);  // A and B MN-major
+      const uint32_t id_kv = idesc_bf16_f32(128, K::kParts == 3 ? 64 : 128) | (1u << 15) | (1u << 16);  // A and B MN-major
       uint32_t tails = 0;
       auto fixed = [&](const Item& w, int p) {  // whether the chunk's tail rows are zeroed first
         const bool rev = args.la.job[w.job].reverse != 0;
@@ -703,9 +761,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       };
       auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
         const int st = static_cast<int>(n % K::kStages);
-        if (!wait_for(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+        if (!warp_wait(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
         if (fixed(w, p)) {
-          if (!wait_for(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
         }
         tc_fence_after();
@@ -715,14 +773,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const uint32_t sa = base + (n % K::kStages) * K::kStage;
         const uint64_t da = desc_kmajor_sw128(sa), db = desc_kmajor_sw128(sa + DKB * kTile);
         const uint32_t acc = tmem + kTmP + (n & 1u) * 128u;
-#pragma unroll 1
-        for (uint32_t n = 0; n < 4 * DKB; ++n) {
-          const uint32_t at = ((n >> 2) * kTile + (n & 3u) * 32u) >> 4;
-          mma_bf16_ss(acc, da + at, db + at, id_ab, n != 0u ? 1u : 0u);
+        if (elect_one()) {
+#pragma unroll
+          for (uint32_t k = 0; k < 4 * DKB; ++k) {
+            const uint32_t at = ((k >> 2) * kTile + (k & 3u) * 32u) >> 4;
+            mma_bf16_ss(acc, da + at, db + at, id_ab, k != 0u ? 1u : 0u);
+          }
+          mma_commit(&bar.pacc[n & 1u]);
         }
-        mma_commit(&bar.pacc[n & 1u]);
+        __syncwarp();
       };
-      // Loops stay rolled: a chunk passes through each once, and what is unrolled is fetched anew every time.
       // a . b runs one chunk ahead, over item borders
       int nidx = blockIdx.x, np = 0;  // the next chunk to start
       Item nw{};
@@ -742,7 +802,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!ready(nw, np, ahead)) return false;
         if (full_pass) {
           // the buffer's last reader: the product with c two chunks before
-          if (ahead >= 2 && !wait_for(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (ahead >= 2 && !warp_wait(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
           product_ab(ahead);
         }
         ++ahead;
@@ -755,53 +815,66 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t stage = base + st * K::kStage;
         // state product b^T (scaled c)
-        if (!(ok = wait_for(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-        if (it > 0 && !(ok = wait_for(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = warp_wait(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (it > 0 && !(ok = warp_wait(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
         const uint64_t db = desc_mn(stage + DKB * kTile, kTile), dv = desc_mn(base + K::kOffV, kTile);
-#pragma unroll 1
-        for (uint32_t q = 0; q < 8; ++q) {
+        if (elect_one()) {
 #pragma unroll
-          for (uint32_t part = 0; part < K::kParts; ++part)
-            mma_bf16_ss(tmem + kTmKV, db + q * 128u, dv + (part * (kTile >> 4) + q * 128u), id_kv,
-                   (part | q) != 0u ? 1u : 0u);
+          for (uint32_t q = 0; q < 8; ++q) {
+            // two parts side by side are one MMA of 128 columns, which reads b once; three go one after another
+            // into the same 64 (MMAs of different shapes on one accumulator have no order)
+#pragma unroll
+            for (uint32_t part = 0; part < (K::kParts == 3 ? 3u : 1u); ++part)
+              mma_bf16_ss(tmem + kTmKV, db + q * 128u, dv + (part * (kTile >> 4) + q * 128u), id_kv,
+                          (part | q) != 0u ? 1u : 0u);
+          }
+          mma_commit(&bar.kv);
         }
-        mma_commit(&bar.kv);
+        __syncwarp();
         if (!(ok = start_next())) break;
         if (full_pass) {
           // a . S
-          if (!(ok = wait_for(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-          if (it > 0 && !(ok = wait_for(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = warp_wait(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (it > 0 && !(ok = warp_wait(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
           const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
-#pragma unroll 1
-          for (uint32_t n = 0; n < 4 * DKB; ++n) {
+          if (elect_one()) {
 #pragma unroll
-            for (uint32_t part = 0; part < K::kSParts; ++part)
-              mma_bf16_ss(tmem + kTmOX, da + (((n >> 2) * kTile + (n & 3u) * 32u) >> 4),
-                     ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
+            for (uint32_t n = 0; n < 4 * DKB; ++n) {
+#pragma unroll
+              for (uint32_t part = 0; part < K::kSParts; ++part)
+                mma_bf16_ss(tmem + kTmOX, da + (((n >> 2) * kTile + (n & 3u) * 32u) >> 4),
+                            ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
+            }
+            mma_commit(&bar.qs);
           }
-          mma_commit(&bar.qs);
+          __syncwarp();
           // (decayed a . b) c
           const uint32_t b = it & 1u;
           const uint64_t dc = desc_mn(stage + 2 * DKB * kTile, kTile);
-          if (!(ok = wait_for(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = warp_wait(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
-#pragma unroll 1
-          for (uint32_t q = 0; q < 8; ++q) {
+          if (elect_one()) {
 #pragma unroll
-            for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
-              mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + q * 16u + part * 8u, dc + q * 128u,
-                     id_o, (part | q) != 0u ? 1u : 0u);
+            for (uint32_t q = 0; q < 8; ++q) {
+#pragma unroll
+              for (uint32_t part = 0; part < (PRECISE ? 2u : 1u); ++part)
+                mma_bf16_ts(tmem + kTmOI, tmem + kTmP + b * 128u + q * 16u + part * 8u, dc + q * 128u, id_o,
+                            (part | q) != 0u ? 1u : 0u);
+            }
+            mma_commit(&bar.o);
           }
-          mma_commit(&bar.o);
+          __syncwarp();
         }
-        mma_commit(&bar.empty[st]);
+        if (elect_one()) mma_commit(&bar.empty[st]);
+        __syncwarp();
         ++it;
       }
-      mma_commit(&bar.drained);  // arrives once everything issued above has completed
+      if (elect_one()) mma_commit(&bar.drained);  // arrives once everything issued above has completed
+      __syncwarp();
     }
-  } else {
+    } else if (warp == 26) {
     // ---------------- decay tables: lane l of block b is token 32 b + l
     for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
       Item w;
@@ -857,11 +930,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         warp_arrive(&bar.gfull[b], lane);
       }
     }
+    }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 25) {
     // no MMA may still write the accumulators when they are freed
     if (lane == 0) wait_for(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
     __syncwarp();
