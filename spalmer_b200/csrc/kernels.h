@@ -537,7 +537,7 @@ struct LaOperand {
 };
 struct LaJob {
   LaOperand a, b, c;
-  LaOperand e;         // e.p: dots[h][token] = sum over the columns of e . out (the decay's gradient) | null
+  LaOperand e;         // e.p: dots[h][token] = sum over the columns of e . out (the decay's gradient; BF16 out only) | null
   float* dots;         // [slices of 64 columns][H][total]
   void* out;           // [total][H][dc] BF16 / FP32
   const float* init;   // [nseq][H][da * dc], strides s_row, s_col | null = zero
@@ -583,7 +583,16 @@ struct LaDecayGradArgs {
   int nseq, H, g_f32;
 };
 int launch_la_decay_grad(const LaDecayGradArgs& a, cudaStream_t stream);
-// out[t][kv][d] = bf16(sum over the group's query heads of in[t][h][d])
-int launch_la_group_sum(const float* in, uint16_t* out, int64_t total, int H, int group, int d, cudaStream_t stream);
+// out[t][kv][d] = bf16(sum over the group's query heads of in[t][h][d]); with
+// e.p, dots[h][t] = in[t][h] . e[t][kv]
+struct LaGroupSumArgs {
+  const float* in;
+  uint16_t* out;
+  LaOperand e;
+  float* dots;
+  int64_t total, T;  // tokens in all, of a batch row
+  int H, group, d;   // d <= 128
+};
+int launch_la_group_sum(const LaGroupSumArgs& a, cudaStream_t stream);
 
 }  // namespace spx

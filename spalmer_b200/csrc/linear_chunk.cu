@@ -36,7 +36,7 @@
 // own first state.
 //
 // Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
-// scaled c, 16-19 the state, 20-23 the epilogue, 24 TMA, 25 MMA, 26 decays.  One
+// scaled c, 16-19 the state, 20-23 the epilogue, 24 and 27 TMA, 25 MMA, 26 decays.  One
 // warp gets through an instruction every three or four cycles here, so the
 // longer roles have two warpgroups, and registers move between warpgroups.
 // Every wait is bounded (status word, then return).
@@ -59,8 +59,9 @@ constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
 constexpr int kLaThreads = 28 * 32;  // seven warpgroups
 constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
 // Registers of the warpgroups' threads: the launch gives each 72 (896 x 72 = 64,512 of 65,536).
-constexpr int kRegsAB = 64, kRegsC = 56, kRegsState = 128, kRegsOut = 88, kRegsRest = 40;
+constexpr int kRegsAB = 64, kRegsC = 56, kRegsState = 120, kRegsOut = 104, kRegsRest = 40;
 static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + kRegsOut + kRegsRest <= 7 * 72, "registers of a CTA");
+constexpr uint32_t kBarBytes = 288;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -104,9 +105,12 @@ struct Cfg {
   static constexpr uint32_t kSTile = DKB * 64 * 128;
   static constexpr uint32_t kOffS = kStages * kStage;
   static constexpr uint32_t kOffV = kOffS + kSParts * kSTile;
-  static constexpr uint32_t kOffT = kOffV + kParts * kTile;
+  // rows on their way to global memory: a tile of their own where there is room, else the chunk's tile of c
+  static constexpr bool kOwnOut = DKB == 1;
+  static constexpr uint32_t kOffOut = kOffV + kParts * kTile;
+  static constexpr uint32_t kOffT = kOffOut + (kOwnOut ? kTile : 0);
   static constexpr uint32_t kOffBar = kOffT + 2 * sizeof(DecayTable);
-  static constexpr uint32_t kBytes = kOffBar + 256;
+  static constexpr uint32_t kBytes = kOffBar + kBarBytes;
 };
 static_assert(Cfg<2, false, 3>::kBytes <= 232448 && Cfg<2, true, 2>::kBytes <= 232448, "shared memory of a CTA");
 
@@ -300,15 +304,24 @@ __device__ __forceinline__ void split2(uint64_t v, uint32_t (&part)[NP]) {
   }
 }
 
+// A load that stays where it is written (the compiler may move others down to their use).
+__device__ __forceinline__ uint4 load_now(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(reinterpret_cast<uint64_t>(p)));
+  return v;
+}
+
 struct Bars {
-  uint64_t full[3], empty[3];
+  uint64_t full_ab[3], full_c[3], empty_a[3], empty_b[3], empty_c[3];  // per stage
   uint64_t gfull[2], gfree[2];
   uint64_t pacc[2], pop[2];
   uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
   uint64_t vp, kv, kvfree, sop, qs, o, ofree, drained;
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 256, "barriers");
+static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 
 }  // namespace
 
@@ -330,8 +343,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 3; ++s) {
-      mbar_init(&bar.full[s], 1);
-      mbar_init(&bar.empty[s], full_pass ? 5 : 1);  // the MMAs, and the epilogue's warps
+      mbar_init(&bar.full_ab[s], 1);
+      mbar_init(&bar.full_c[s], 1);
+      mbar_init(&bar.empty_a[s], 1);
+      mbar_init(&bar.empty_b[s], 1);
+      mbar_init(&bar.empty_c[s], full_pass && !K::kOwnOut ? 5 : 1);  // the MMAs, and the epilogue's warps
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.gfull[s], 1);
@@ -460,11 +476,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
         const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
-        if (!(ok = warp_wait(&bar.full[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.full_c[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const uint32_t stage = base + st * K::kStage;
         const uint32_t sc = stage + 2 * DKB * kTile;
         if (len < kC && args.la.cu != nullptr) {
           // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
+          if (!(ok = warp_wait(&bar.full_ab[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
           if (row >= len) {
 #pragma unroll
             for (int x = 0; x < DKB + 1; ++x)
@@ -602,42 +619,51 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (j.e.p != nullptr)
           pe = j.e.p + (packed ? 0 : w.seq) * j.e.sb + (packed ? w.start : 0) * j.e.st + (w.h / j.e.group) * j.e.sh + col0;
       }
-      for (int p = 0; p < w.n; ++p, ++it) {
-        const uint32_t b = it & 1u;
-        const int64_t t = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC + row;  // in the sequence
+      const int64_t stride = static_cast<int64_t>(args.la.H) * j.dc;
+      const int r0 = quad * 32 + (lane >> 3), c8 = lane & 7;  // rows r0, r0 + 4, ... of this warp's 32
+      // the row's decay for the a . S part; read a chunk ahead, so that this role, the
+      // last to need a table, does not keep the others waiting for the next
+      float factor = 0.0f;
+      auto read_factor = [&](uint32_t n) {
+        const uint32_t b = n & 1u;
+        if (!warp_wait(&bar.gfull[b], (n >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
+        factor = rev ? to_end(tables[b], quad, row) : from_start(tables[b], quad, row);
+        warp_arrive(&bar.gfree[b], lane);
+        return true;
+      };
+      if (w.n > 0) ok = read_factor(it);
+      for (int p = 0; ok && p < w.n; ++p, ++it) {
+        const int64_t first = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC;  // in the sequence
+        const int left = static_cast<int>(min(w.len - first, static_cast<int64_t>(kC)));            // tokens of the chunk
         // Rows go through shared memory on their way to and from global memory (eight
         // lanes a row of 128 bytes): a thread's own row would touch 32 lines an
         // instruction and hold up every barrier and shared-memory access of the CTA.
-        // The chunk's tiles serve: their last reader is done when its output is.
-        const uint32_t stage = base + (it % K::kStages) * K::kStage;
-        const uint32_t s_e = stage, s_out = stage + DKB * kTile;
-        const int64_t t0 = t - lane + (lane >> 3);  // rows t0, t0 + 4, ... of this warp's 32
-        const int c8 = lane & 7;
+        const int st = static_cast<int>(it % K::kStages);
+        const uint32_t tile = base + (K::kOwnOut ? K::kOffOut : st * K::kStage + 2 * DKB * kTile);
         uint4 e[8];
         if constexpr (PRECISE) {
           if (pe != nullptr) {
+            const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c8;
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              e[q] = t0 + 4 * q < w.len && 8 * c8 < valid
-                         ? __ldg(reinterpret_cast<const uint4*>(pe + (t0 + 4 * q) * j.e.st) + c8)
-                         : make_uint4(0u, 0u, 0u, 0u);
+            for (int q = 0; q < 8; ++q, src += 4 * j.e.st) {
+              e[q] = make_uint4(0u, 0u, 0u, 0u);
+              if (r0 + 4 * q < left && 8 * c8 < valid) e[q] = load_now(src);
+            }
           }
         }
-        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const float factor = rev ? to_end(tables[b], quad, row) : from_start(tables[b], quad, row);
-        warp_arrive(&bar.gfree[b], lane);
         const float sc = args.la.scale, sx = sc * factor;
         const uint64_t sc2 = pair(sc, sc), sx2 = pair(sx, sx);
+        if (p + 1 < w.n && !(ok = read_factor(it + 1))) break;
         if (!(ok = warp_wait(&bar.o, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        const int r0 = quad * 32 + (lane >> 3);
         if constexpr (PRECISE) {
           if (pe != nullptr) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) sts16(s_e + swz(r0 + 4 * q, c8), e[q].x, e[q].y, e[q].z, e[q].w);
+            for (int q = 0; q < 8; ++q) sts16(tile + swz(r0 + 4 * q, c8), e[q].x, e[q].y, e[q].z, e[q].w);
             __syncwarp();
           }
         }
+        const int64_t at = (w.start + first + r0) * stride + w.h * j.dc + col0;
         uint32_t o[32];
         uint64_t dot = 0;  // two FP32 sums
 #pragma unroll
@@ -655,20 +681,28 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             o[8 * part + i] = one[0];
           }
           if constexpr (PRECISE) {
-            if (f32) {  // two tiles of 32 columns
+            if (f32) {  // (no dots then) 32 columns at a time fill the tile
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float z[4];
                 unpair(v[2 * q], z[0], z[1]);
                 unpair(v[2 * q + 1], z[2], z[3]);
-                sts16(s_out + (part >> 1) * kTile + swz(row, 4 * (part & 1) + q), __float_as_uint(z[0]), __float_as_uint(z[1]),
-                      __float_as_uint(z[2]), __float_as_uint(z[3]));
+                sts16(tile + swz(row, 4 * (part & 1) + q), __float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]),
+                      __float_as_uint(z[3]));
               }
-            }
-            if (pe != nullptr) {
+              if ((part & 1) != 0) {
+                __syncwarp();
+                const int c = 16 * (part - 1) + 4 * c8;
+                float* dst = reinterpret_cast<float*>(j.out) + at + c;
+#pragma unroll
+                for (int q = 0; q < 8; ++q, dst += 4 * stride)
+                  if (r0 + 4 * q < left && c < valid) *reinterpret_cast<uint4*>(dst) = lds16(tile + swz(r0 + 4 * q, c8));
+                __syncwarp();
+              }
+            } else if (pe != nullptr) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const uint4 u = lds16(s_e + swz(row, 2 * part + q));
+                const uint4 u = lds16(tile + swz(row, 2 * part + q));
                 const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dot = fma2(v[4 * q + i], pair(ew[i] << 16, ew[i] & 0xFFFF0000u), dot);
@@ -679,44 +713,42 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         // the accumulators are free before the stores: the next chunk's products wait for them
         tc_fence_before();
         warp_arrive(&bar.ofree, lane);
+        uint4 rows[8];
         if (!f32) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) sts16(s_out + swz(row, q), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-        }
-        __syncwarp();
-        const int64_t stride = static_cast<int64_t>(args.la.H) * j.dc;
-        const int64_t at = (w.start + t0) * stride + w.h * j.dc + col0;
-        if (f32) {
+          for (int q = 0; q < 8; ++q) sts16(tile + swz(row, q), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const int c = 32 * (q & 1) + 4 * c8;
-            if (t0 + 4 * (q >> 1) < w.len && c < valid)
-              *reinterpret_cast<uint4*>(reinterpret_cast<float*>(j.out) + at + 4 * (q >> 1) * stride + c) =
-                  lds16(s_out + (q & 1) * kTile + swz(r0 + 4 * (q >> 1), c8));
-          }
+          for (int q = 0; q < 8; ++q) rows[q] = lds16(tile + swz(r0 + 4 * q, c8));
+        }
+        if constexpr (K::kOwnOut) {
+          __syncwarp();  // before the next chunk's rows
         } else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (t0 + 4 * q < w.len && 8 * c8 < valid)
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(j.out) + at + 4 * q * stride + 8 * c8) =
-                  lds16(s_out + swz(r0 + 4 * q, c8));
+          fence_proxy_async_smem();  // before the next copy lands here
+          warp_arrive(&bar.empty_c[st], lane);
         }
-        fence_proxy_async_smem();  // before the next chunk's copies land here
-        warp_arrive(&bar.empty[it % K::kStages], lane);
+        if (!f32) {
+          uint16_t* dst = reinterpret_cast<uint16_t*>(j.out) + at + 8 * c8;
+#pragma unroll
+          for (int q = 0; q < 8; ++q, dst += 4 * stride)
+            if (r0 + 4 * q < left && 8 * c8 < valid) *reinterpret_cast<uint4*>(dst) = rows[q];
+        }
         if constexpr (PRECISE) {
-          if (pe != nullptr && t < w.len) {
+          if (pe != nullptr && row < left) {
             float d0, d1;
             unpair(dot, d0, d1);
-            j.dots[(static_cast<int64_t>(w.slice) * args.la.H + w.h) * args.la.total + w.start + t] = d0 + d1;
+            j.dots[(static_cast<int64_t>(w.slice) * args.la.H + w.h) * args.la.total + w.start + first + row] = d0 + d1;
           }
         }
       }
     }
   } else {
     regs_down<kRegsRest>();
-    if (warp == 24) {
-    // ---------------- TMA
+    if (warp == 24 || warp == 27) {
+    // ---------------- TMA: a and b, and in a warp of its own c, whose tile is free later
     if (lane == 0) {
+      const bool ab = warp == 24;
+      uint64_t* const full = ab ? bar.full_ab : bar.full_c;
       for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
         Item w;
         item_of(args, idx, &w);
@@ -726,24 +758,36 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int t0 = packed ? static_cast<int>(w.start) : 0;
         for (int p = 0; p < w.n; ++p, ++it) {
           const int st = static_cast<int>(it % K::kStages);
+          const uint32_t ph = ((it / K::kStages) & 1u) ^ 1u;
           const int chunk = j.reverse != 0 ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-          if (!(ok = wait_for(&bar.empty[st], ((it / K::kStages) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
           const uint32_t stage = base + st * K::kStage;
           const int t = t0 + chunk * kC;
-          mbar_arrive_expect_tx(&bar.full[st], (full_pass ? 2 * DKB + 1 : DKB + 1) * kTile);
-          if (full_pass) {
-            for (int x = 0; x < DKB; ++x)
-              tma_load_4d(stage + x * kTile, &args.map[w.job][0], &bar.full[st], 64 * x, w.h / j.a.group, t, batch);
+          if (!ab) {
+            if (!(ok = wait_for(&bar.empty_c[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+            mbar_arrive_expect_tx(&full[st], kTile);
+            tma_load_4d(stage + 2 * DKB * kTile, &args.map[w.job][2], &full[st], 64 * w.slice, w.h / j.c.group, t, batch);
+            continue;
           }
+          if (!(ok = wait_for(&bar.empty_b[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+          mbar_arrive_expect_tx(&full[st], (full_pass ? 2 * DKB : DKB) * kTile);
           for (int x = 0; x < DKB; ++x)
-            tma_load_4d(stage + (DKB + x) * kTile, &args.map[w.job][1], &bar.full[st], 64 * x, w.h / j.b.group, t, batch);
-          tma_load_4d(stage + 2 * DKB * kTile, &args.map[w.job][2], &bar.full[st], 64 * w.slice, w.h / j.c.group, t, batch);
+            tma_load_4d(stage + (DKB + x) * kTile, &args.map[w.job][1], &full[st], 64 * x, w.h / j.b.group, t, batch);
+          if (full_pass) {
+            // with b's copies on their way the count has to come to its end: a's follow even after a failed wait
+            ok = wait_for(&bar.empty_a[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER);
+            for (int x = 0; x < DKB; ++x)
+              tma_load_4d(stage + x * kTile, &args.map[w.job][0], &full[st], 64 * x, w.h / j.a.group, t, batch);
+            if (!ok) {
+              ++it;
+              break;
+            }
+          }
         }
       }
       if (!ok) {  // leave no copy in flight behind an abandoned pipeline
         for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
           const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
-          wait_for(&bar.full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
+          wait_for(&full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
         }
       }
     }
@@ -761,7 +805,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       };
       auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
         const int st = static_cast<int>(n % K::kStages);
-        if (!warp_wait(&bar.full[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+        if (!warp_wait(&bar.full_ab[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
         if (fixed(w, p)) {
           if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
@@ -830,6 +874,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
                           (part | q) != 0u ? 1u : 0u);
           }
           mma_commit(&bar.kv);
+          mma_commit(&bar.empty_b[st]);  // a . b of this chunk was issued before
+          if (!full_pass) mma_commit(&bar.empty_c[st]);
         }
         __syncwarp();
         if (!(ok = start_next())) break;
@@ -848,6 +894,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
                             ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
             }
             mma_commit(&bar.qs);
+            mma_commit(&bar.empty_a[st]);
           }
           __syncwarp();
           // (decayed a . b) c
@@ -864,11 +911,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
                             (part | q) != 0u ? 1u : 0u);
             }
             mma_commit(&bar.o);
+            mma_commit(&bar.empty_c[st]);
           }
           __syncwarp();
         }
-        if (elect_one()) mma_commit(&bar.empty[st]);
-        __syncwarp();
         ++it;
       }
       if (elect_one()) mma_commit(&bar.drained);  // arrives once everything issued above has completed
@@ -952,27 +998,26 @@ __global__ void __launch_bounds__(256) la_chain_kernel(const __grid_constant__ L
   const LaJob& j = args.la.job[w.job];
   const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
   float* seg = args.seg_state + static_cast<int64_t>(lane_id) * args.nseg * 8192;
-  for (int i = (blockIdx.y * 256 + threadIdx.x) * 4; i < j.da * 64; i += gridDim.y * 1024) {
-    const int r = i / 64, c = w.slice * 64 + (i & 63);
-    float x[4];
+  const int i = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (i >= j.da * 64) return;
+  const int r = i / 64, c = w.slice * 64 + (i & 63);
+  float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x[e] = j.init != nullptr && c + e < j.dc ? j.init_scale * j.init[st0 + r * j.s_row + (c + e) * j.s_col] : 0.0f;
-    for (int s = 0; s < args.nseg; ++s) {
-      float4* p = reinterpret_cast<float4*>(seg + static_cast<int64_t>(s) * 8192 + i);
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float d = 0.0f;
-      if (s + 1 < args.nseg) {
-        v = *p;
-        d = args.seg_decay[static_cast<int64_t>(lane_id) * args.nseg + s];
-      }
-      *p = make_float4(x[0], x[1], x[2], x[3]);
-      x[0] = fmaf(d, x[0], v.x);
-      x[1] = fmaf(d, x[1], v.y);
-      x[2] = fmaf(d, x[2], v.z);
-      x[3] = fmaf(d, x[3], v.w);
-    }
+  for (int e = 0; e < 4; ++e)
+    x[e] = j.init != nullptr && c + e < j.dc ? j.init_scale * j.init[st0 + r * j.s_row + (c + e) * j.s_col] : 0.0f;
+  float4 next = *reinterpret_cast<const float4*>(seg + i);
+  for (int s = 0; s + 1 < args.nseg; ++s) {
+    const float4 v = next;
+    float4* p = reinterpret_cast<float4*>(seg + static_cast<int64_t>(s) * 8192 + i);
+    if (s + 2 < args.nseg) next = p[2048];  // the next segment's, before this one's place is written
+    const float d = args.seg_decay[static_cast<int64_t>(lane_id) * args.nseg + s];
+    *p = make_float4(x[0], x[1], x[2], x[3]);
+    x[0] = fmaf(d, x[0], v.x);
+    x[1] = fmaf(d, x[1], v.y);
+    x[2] = fmaf(d, x[2], v.z);
+    x[3] = fmaf(d, x[3], v.w);
   }
+  *reinterpret_cast<float4*>(seg + static_cast<int64_t>(args.nseg - 1) * 8192 + i) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
 namespace {
@@ -1070,7 +1115,7 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
     c.state_only = 1;
     c.run_segs = c.nseg - 1;
     if (int rc = pass(); rc != SPX_OK) return rc;
-    la_chain_kernel<<<dim3(static_cast<unsigned>(lanes), 2), 256, 0, stream>>>(c);
+    la_chain_kernel<<<dim3(static_cast<unsigned>(lanes), 8), 256, 0, stream>>>(c);
     if (cudaGetLastError() != cudaSuccess) return SPX_ERR_CUDA;
   }
   c.state_only = 0;

@@ -201,29 +201,49 @@ int launch_la_decay_grad(const LaDecayGradArgs& a, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- shared heads
-__global__ void __launch_bounds__(256) la_group_sum_kernel(const float* __restrict__ in, uint16_t* __restrict__ out,
-                                                           int64_t total, int kv, int group, int d) {
-  const int64_t n4 = total * kv * (d / 4);
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n4; i += gridDim.x * 256ll) {
-    const int64_t row = i / (d / 4);  // (token, shared head)
-    const int c = static_cast<int>(i - row * (d / 4)) * 4;
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int q = 0; q < group; ++q) {
-      const float4 v = *reinterpret_cast<const float4*>(in + (row * group + q) * d + c);
-      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+// One warp per (token, shared head): the sum over its query heads' gradients,
+// and with `e` (the shared tensor itself) each query head's dot with it.
+__global__ void __launch_bounds__(256) la_group_sum_kernel(const LaGroupSumArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int kv = a.H / a.group;
+  const int64_t n = a.total * kv;
+  const bool col = 4 * lane < a.d;
+  for (int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < n; i += gridDim.x * 8ll) {
+    const int64_t t = i / kv;
+    const int h = static_cast<int>(i - t * kv);
+    float4 ev = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.e.p != nullptr && col) {
+      const int64_t b = t / a.T;
+      const uint2 u = *reinterpret_cast<const uint2*>(a.e.p + b * a.e.sb + (t - b * a.T) * a.e.st + h * a.e.sh + 4 * lane);
+      ev = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xFFFF0000u));
     }
-    const uint2 b = make_uint2(f32_to_bf16_rne(s.x) | (static_cast<uint32_t>(f32_to_bf16_rne(s.y)) << 16),
-                               f32_to_bf16_rne(s.z) | (static_cast<uint32_t>(f32_to_bf16_rne(s.w)) << 16));
-    *reinterpret_cast<uint2*>(out + row * d + c) = b;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int q = 0; q < a.group; ++q) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (col) v = *reinterpret_cast<const float4*>(a.in + (i * a.group + q) * a.d + 4 * lane);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      if (a.e.p != nullptr) {
+        float d = fmaf(v.x, ev.x, fmaf(v.y, ev.y, fmaf(v.z, ev.z, v.w * ev.w)));
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, off);
+        if (lane == 0) a.dots[static_cast<int64_t>(h * a.group + q) * a.total + t] = d;
+      }
+    }
+    if (col) {
+      const uint2 b = make_uint2(f32_to_bf16_rne(s.x) | (static_cast<uint32_t>(f32_to_bf16_rne(s.y)) << 16),
+                                 f32_to_bf16_rne(s.z) | (static_cast<uint32_t>(f32_to_bf16_rne(s.w)) << 16));
+      *reinterpret_cast<uint2*>(a.out + i * a.d + 4 * lane) = b;
+    }
   }
 }
 
-int launch_la_group_sum(const float* in, uint16_t* out, int64_t total, int H, int group, int d, cudaStream_t stream) {
-  const int64_t n4 = total * (H / group) * (d / 4);
-  if (n4 <= 0) return SPX_OK;
-  int64_t blocks = (n4 + 255) / 256;
+int launch_la_group_sum(const LaGroupSumArgs& a, cudaStream_t stream) {
+  const int64_t n = a.total * (a.H / a.group);
+  if (n <= 0) return SPX_OK;
+  int64_t blocks = (n + 7) / 8;
   if (blocks > 148 * 16) blocks = 148 * 16;
-  la_group_sum_kernel<<<static_cast<int>(blocks), 256, 0, stream>>>(in, out, total, H / group, group, d);
+  la_group_sum_kernel<<<static_cast<int>(blocks), 256, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
 }
 

@@ -335,8 +335,10 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   jk.s_col = V;
   jk.init_scale = 1.0f / d.scale;  // the last state's gradient enters without `scale`
   jk.fin_scale = d.scale;
-  jk.e = operand(k, group);
-  jk.dots = at<float>(workspace, L.k_dots);
+  if (group == 1) {  // else the sum over the group takes k . dk per query head
+    jk.e = operand(k, 1);
+    jk.dots = at<float>(workspace, L.k_dots);
+  }
   // d v_j = scale sum_{i >= j} w_ij (k_j . q_i) d out_i, and the first state's gradient
   LaJob& jv = a.job[2];
   jv.a = operand(k, group);
@@ -354,10 +356,29 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   jv.init_scale = 1.0f / d.scale;
   jv.fin_scale = d.scale;
   if (int rc = run_jobs(a, true, at<void>(workspace, L.segments), st); rc != SPX_OK) return rc;
+  if (group > 1) {
+    LaGroupSumArgs sum{};
+    sum.total = total;
+    sum.T = d.packed != 0 ? total : d.seq_len;
+    sum.H = d.heads;
+    sum.group = group;
+    sum.in = at<float>(workspace, L.dk);
+    sum.out = d_k;
+    sum.d = K;
+    sum.e = operand(k, group);
+    sum.dots = at<float>(workspace, L.k_dots);
+    if (int rc = launch_la_group_sum(sum, st); rc != SPX_OK) return rc;
+    sum.in = at<float>(workspace, L.dv);
+    sum.out = d_v;
+    sum.d = V;
+    sum.e = LaOperand{};
+    if (int rc = launch_la_group_sum(sum, st); rc != SPX_OK) return rc;
+  }
   LaDecayGradArgs g{};
   g.q_dots = jq.dots;
-  g.k_dots = jk.dots;
-  g.q_slices = g.k_slices = recurrent(a) ? 1 : slices_of(K);
+  g.k_dots = at<float>(workspace, L.k_dots);
+  g.q_slices = recurrent(a) ? 1 : slices_of(K);
+  g.k_slices = group > 1 ? 1 : g.q_slices;
   g.last = jq.fin;
   g.d_last = d_final_state;
   g.dg = d_decay;
@@ -369,10 +390,6 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   g.H = a.H;
   g.g_f32 = a.g_f32;
   if (int rc = launch_la_decay_grad(g, st); rc != SPX_OK) return rc;
-  if (group > 1) {
-    if (int rc = launch_la_group_sum(at<float>(workspace, L.dk), d_k, total, d.heads, group, K, st); rc != SPX_OK) return rc;
-    if (int rc = launch_la_group_sum(at<float>(workspace, L.dv), d_v, total, d.heads, group, V, st); rc != SPX_OK) return rc;
-  }
   return SPX_OK;
 }
 
