@@ -538,7 +538,7 @@ struct LaOperand {
 struct LaJob {
   LaOperand a, b, c;
   LaOperand e;         // e.p: dots[h][token] = sum over the columns of e . out (the decay's gradient; BF16 out only) | null
-  float* dots;         // [slices of 64 columns][H][total]
+  float* dots;         // [planes of 32 columns][H][total]
   void* out;           // [total][H][dc] BF16 / FP32
   const float* init;   // [nseq][H][da * dc], strides s_row, s_col | null = zero
   float* fin;          // the last state, same layout | null
@@ -570,7 +570,7 @@ struct LaStepArgs {
 int launch_la_step(const LaStepArgs& a, cudaStream_t stream);
 int launch_la_recurrent(const LaArgs& a, cudaStream_t stream);
 size_t la_chunk_workspace(const LaArgs& a);
-// precise: more parts of the rounded operands (the gradients); dots then hold one plane per 64 columns
+// precise: more parts of the rounded operands (the gradients); dots then hold one plane per 32 columns
 int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream);
 // dg[t, h] = <last state, its gradient> + sum over t' >= t of (q . dq - k . dk), from the jobs' dots
 struct LaDecayGradArgs {

@@ -36,9 +36,9 @@
 // own first state.
 //
 // Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
-// scaled c, 16-19 the state, 20-23 the epilogue, 24 and 27 TMA, 25 MMA, 26 decays.  One
-// warp gets through an instruction every three or four cycles here, so the
-// longer roles have two warpgroups, and registers move between warpgroups.
+// scaled c, 16-19 the state, 20-27 the epilogue, 28 and 31 TMA, 29 MMA, 30
+// decays.  One warp gets through an instruction every three or four cycles here,
+// so the longer roles have two warpgroups, and registers move between them.
 // Every wait is bounded (status word, then return).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -56,12 +56,12 @@ namespace {
 
 constexpr int kC = 128;              // tokens of a chunk
 constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
-constexpr int kLaThreads = 28 * 32;  // seven warpgroups
+constexpr int kLaThreads = 32 * 32;  // eight warpgroups
 constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
-// Registers of the warpgroups' threads: the launch gives each 72 (896 x 72 = 64,512 of 65,536).
-constexpr int kRegsAB = 64, kRegsC = 56, kRegsState = 120, kRegsOut = 104, kRegsRest = 40;
-static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + kRegsOut + kRegsRest <= 7 * 72, "registers of a CTA");
-constexpr uint32_t kBarBytes = 288;
+// Registers of the warpgroups' threads: the launch gives each 64 (1024 x 64 = 65,536).
+constexpr int kRegsAB = 64, kRegsC = 48, kRegsState = 120, kRegsOut = 64, kRegsRest = 40;
+static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + 2 * kRegsOut + kRegsRest <= 8 * 64, "registers of a CTA");
+constexpr uint32_t kBarBytes = 304;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -157,13 +157,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // mbar_wait that counts cycles instead of reading the timer: the kernel's 28
 // warps run through a dozen loops at once, and what the instruction cache does
 // not hold is fetched again for every chunk, so its hot code has to stay small.
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status, int code) {
+// One that gives up leaves its code in shared memory; the CTA's end records it.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* failed, int code) {
   if (mbar_try_wait(bar, parity)) return true;
   const int64_t start = clock64();
   do {
     if (mbar_try_wait(bar, parity)) return true;
   } while (clock64() - start < kWaitCycles);
-  record_error(status, code);
+  *failed = code;
   return false;
 }
 
@@ -178,8 +179,8 @@ __device__ __forceinline__ void regs_down() {
 }
 
 // Every lane polls; the warp goes on together, or gives up together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, status, code)) != 0;
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* failed, int code) {
+  return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, failed, code)) != 0;
 }
 
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -218,10 +219,19 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[16]) {  // the first eight
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -320,6 +330,7 @@ struct Bars {
   uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
   uint64_t vp, kv, kvfree, sop, qs, o, ofree, drained;
   uint32_t tmem;
+  int failed;
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 
@@ -336,6 +347,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     return;
   }
   Bars& bar = *reinterpret_cast<Bars*>(la_smem + K::kOffBar);
+  int* const failed = &bar.failed;
   DecayTable* const tables = reinterpret_cast<DecayTable*>(la_smem + K::kOffT);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform to the compiler
   const bool full_pass = args.state_only == 0;
@@ -347,11 +359,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       mbar_init(&bar.full_c[s], 1);
       mbar_init(&bar.empty_a[s], 1);
       mbar_init(&bar.empty_b[s], 1);
-      mbar_init(&bar.empty_c[s], full_pass && !K::kOwnOut ? 5 : 1);  // the MMAs, and the epilogue's warps
+      mbar_init(&bar.empty_c[s], full_pass && !K::kOwnOut ? 9 : 1);  // the MMAs, and the epilogue's warps
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.gfull[s], 1);
-      mbar_init(&bar.gfree[s], full_pass ? 24 : 12);
+      mbar_init(&bar.gfree[s], full_pass ? 28 : 12);
       mbar_init(&bar.pacc[s], 1);
       mbar_init(&bar.pop[s], 8);
       mbar_init(&bar.tail[s], 8);
@@ -362,11 +374,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     mbar_init(&bar.sop, 4);
     mbar_init(&bar.qs, 1);
     mbar_init(&bar.o, 1);
-    mbar_init(&bar.ofree, 4);
+    mbar_init(&bar.ofree, 8);
     mbar_init(&bar.drained, 1);
+    bar.failed = 0;
     fence_mbar_init();
   }
-  if (warp == 25) {
+  if (warp == 29) {
     tmem_alloc(&bar.tmem, kTmCols);
     tmem_relinquish();
   }
@@ -381,19 +394,27 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   uint32_t it = 0;  // chunks so far, the same count in every role
 
   if (warp < 8) {
-    regs_down<kRegsAB>();
+    static_assert(kRegsAB == 64, "the launch's own");
     // ---------------- the decayed a . b matrix: 16 columns of each 32-token block
     const int half = warp >> 2;
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
       Item w;
       item_of(args, idx, &w);
       const bool rev = args.la.job[w.job].reverse != 0;
+      const float sign = rev ? 1.0f : -1.0f;
+      // of this row's words in the diagonal block: a masked entry is zero whatever it holds
+      uint32_t mask[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int c = 16 * half + 2 * q;
+        mask[q] = ((rev ? c >= lane : c <= lane) ? 0xFFFFu : 0u) | ((rev ? c + 1 >= lane : c + 1 <= lane) ? 0xFFFF0000u : 0u);
+      }
       for (int p = 0; p < w.n; ++p, ++it) {
         const uint32_t b = it & 1u, ph = (it >> 1) & 1u;
         const DecayTable& t = tables[b];
-        if (!(ok = warp_wait(&bar.gfull[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.gfull[b], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const float lg = t.lg[row];
-        if (!(ok = warp_wait(&bar.pacc[b], ph, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.pacc[b], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         // The operand takes the accumulator's place: 16 FP32 columns become 8 of BF16
         // pairs (PRECISE: 8 more of their second parts).  From the diagonal block
@@ -406,55 +427,50 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const bool steep = !(own >= -100.0f);
 #pragma unroll 1
         for (int n = 0; n < 4; ++n) {
-          const int j = rev ? (quad + n) & 3 : (quad - n) & 3;
-          const uint32_t at = acc + 32u * j + 16u * half;
-          uint32_t hi[8], lo[8];
+          const int j = (rev ? quad + n : quad - n) & 3;
+          const int c0 = 32 * j + 16 * half;
+          uint32_t x[16];  // columns in, words out
           if (rev ? j < quad : j > quad) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) hi[q] = lo[q] = 0u;
+            for (int q = 0; q < 16; ++q) x[q] = 0u;
           } else {
-            uint32_t x[16];
-            tmem_ld16(at, x);
-            const int c0 = 32 * j + 16 * half;
+            tmem_ld16(acc + c0, x);
             const float rf = ex2(run);
+            const uint64_t rf2 = pair(rf, rf);
             run += t.total[j];
+            const ulonglong2* f4 = reinterpret_cast<const ulonglong2*>(t.cf + c0);
             uint64_t f[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const ulonglong2 v = f4[q];
+              f[2 * q] = mul2(v.x, rf2);
+              f[2 * q + 1] = mul2(v.y, rf2);
+            }
             if (n == 0 && steep) {
-              const float sg = rev ? 1.0f : -1.0f;
 #pragma unroll
-              for (int q = 0; q < 8; ++q) f[q] = pair(ex2((t.lg[c0 + 2 * q] - lg) * sg), ex2((t.lg[c0 + 2 * q + 1] - lg) * sg));
-            } else {
-              const uint64_t rf2 = pair(rf, rf);
-              const ulonglong2* f4 = reinterpret_cast<const ulonglong2*>(t.cf + c0);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const ulonglong2 v = f4[q];
-                f[2 * q] = mul2(v.x, rf2);
-                f[2 * q + 1] = mul2(v.y, rf2);
-              }
+              for (int q = 0; q < 8; ++q) f[q] = pair(ex2((t.lg[c0 + 2 * q] - lg) * sign), ex2((t.lg[c0 + 2 * q + 1] - lg) * sign));
             }
             tmem_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 8; ++q) f[q] = mul2(pair(x[2 * q], x[2 * q + 1]), f[q]);
-            if (n == 0) {  // the diagonal block: a masked entry is zero whatever it holds
-              const int d = lane - 16 * half;
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                float a, c;
-                unpair(f[q], a, c);
-                f[q] = pair((rev ? 2 * q >= d : 2 * q <= d) ? a : 0.0f, (rev ? 2 * q + 1 >= d : 2 * q + 1 <= d) ? c : 0.0f);
-              }
-            }
-#pragma unroll
             for (int q = 0; q < 8; ++q) {
               uint32_t part[PRECISE ? 2 : 1];
-              split2<PRECISE ? 2 : 1>(f[q], part);
-              hi[q] = part[0];
-              lo[q] = part[PRECISE ? 1 : 0];
+              split2<PRECISE ? 2 : 1>(mul2(pair(x[2 * q], x[2 * q + 1]), f[q]), part);
+              x[q] = part[0];  // its column has been taken: 2 q >= q
+              if constexpr (PRECISE) f[q] = part[1];
+            }
+            if constexpr (PRECISE) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) x[8 + q] = static_cast<uint32_t>(f[q]);
+            }
+            if (n == 0) {
+#pragma unroll
+              for (int q = 0; q < (PRECISE ? 16 : 8); ++q) x[q] &= mask[q & 7];
             }
           }
-          tmem_st8(at, hi);
-          if constexpr (PRECISE) tmem_st8(at + 8u, lo);
+          if constexpr (PRECISE)
+            tmem_st16(acc + c0, x);
+          else
+            tmem_st8(acc + c0, x);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -476,12 +492,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
         const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
-        if (!(ok = warp_wait(&bar.full_c[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.full_c[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const uint32_t stage = base + st * K::kStage;
         const uint32_t sc = stage + 2 * DKB * kTile;
         if (len < kC && args.la.cu != nullptr) {
           // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
-          if (!(ok = warp_wait(&bar.full_ab[st], (it / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+          if (!(ok = warp_wait(&bar.full_ab[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
           if (row >= len) {
 #pragma unroll
             for (int x = 0; x < DKB + 1; ++x)
@@ -491,13 +507,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           fence_proxy_async_smem();
           warp_arrive(&bar.tail[tails++ & 1u], lane);
         }
-        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
         warp_arrive(&bar.gfree[b], lane);
         const uint64_t wgt2 = pair(wgt, wgt);
         // the parts' last reader: the state product of the chunk before
-        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-#pragma unroll 2
+        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+#pragma unroll 1
         for (int c = 4 * half; c < 4 * half + 4; ++c) {
           const uint4 u = lds16(sc + swz(row, c));
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
@@ -520,8 +536,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       Item w;
       const bool sound = item_of(args, idx, &w);
       const LaJob& j = args.la.job[w.job];
-      if (!sound && threadIdx.x == 512) record_error(status, SPX_DEV_BAD_TILE);
-      float s[64];
+      if (!sound && threadIdx.x == 512) *failed = SPX_DEV_BAD_TILE;
+      uint64_t s[32];  // pairs of columns
       const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
       const int col0 = w.slice * 64;
       const bool live = row < j.da;
@@ -531,13 +547,15 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
           const float4 v = live ? f[q] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          s[4 * q] = v.x, s[4 * q + 1] = v.y, s[4 * q + 2] = v.z, s[4 * q + 3] = v.w;
+          s[2 * q] = pair(v.x, v.y);
+          s[2 * q + 1] = pair(v.z, v.w);
         }
       } else {
         const float* f = j.init + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.init != nullptr && args.nseg == 1 && live ? j.dc - col0 : 0;
 #pragma unroll
-        for (int c = 0; c < 64; ++c, f += j.s_col) s[c] = c < n ? j.init_scale * *f : 0.0f;
+        for (int c = 0; c < 32; ++c, f += 2 * j.s_col)  // widths are even
+          s[c] = 2 * c < n ? pair(j.init_scale * f[0], j.init_scale * f[j.s_col]) : 0;
       }
       float decay = 1.0f;
       auto write_operand = [&]() {  // BF16 parts of the state for the next chunk's a . S
@@ -546,7 +564,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           for (int c = 0; c < 8; ++c) {
             uint32_t q[4][K::kSParts];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split2<K::kSParts>(pair(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]), q[e]);
+            for (int e = 0; e < 4; ++e) split2<K::kSParts>(s[4 * c + e], q[e]);
 #pragma unroll
             for (int part = 0; part < K::kSParts; ++part)
               sts16(base + K::kOffS + part * K::kSTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
@@ -559,15 +577,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const uint32_t b = it & 1u;
         if (full_pass) {
           // the operand before this chunk; its last reader was the chunk before
-          if (it > 0 && !(ok = warp_wait(&bar.qs, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+          if (it > 0 && !(ok = warp_wait(&bar.qs, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
           write_operand();
         }
-        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const float* tt = tables[b].total;
         const float gamma = ex2((tt[0] + tt[1]) + (tt[2] + tt[3]));
         warp_arrive(&bar.gfree[b], lane);
+        const uint64_t gamma2 = pair(gamma, gamma);
         decay *= gamma;
-        if (!(ok = warp_wait(&bar.kv, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.kv, it & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         if (rows_in) {
 #pragma unroll
@@ -577,9 +596,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             if constexpr (K::kParts == 2) tmem_ld16(tmem + kTmKV + 64u + 16u * part + tm_lane, y);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float add = K::kParts == 2 ? __uint_as_float(x[c]) + __uint_as_float(y[c]) : __uint_as_float(x[c]);
-              s[16 * part + c] = fmaf(gamma, s[16 * part + c], add);
+            for (int c = 0; c < 8; ++c) {
+              uint64_t add = pair(x[2 * c], x[2 * c + 1]);
+              if constexpr (K::kParts == 2) add = add2(add, pair(y[2 * c], y[2 * c + 1]));
+              s[8 * part + c] = fma2(gamma2, s[8 * part + c], add);
             }
           }
         }
@@ -592,20 +612,27 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64);
         if (live) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q) f[q] = make_float4(s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]);
+          for (int q = 0; q < 16; ++q) *reinterpret_cast<ulonglong2*>(f + q) = make_ulonglong2(s[2 * q], s[2 * q + 1]);
         }
         if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
 #pragma unroll
-        for (int c = 0; c < 64; ++c, f += j.s_col)
-          if (c < n) *f = j.fin_scale * s[c];
+        for (int c = 0; c < 32; ++c, f += 2 * j.s_col) {
+          float v0, v1;
+          unpair(s[c], v0, v1);
+          if (2 * c < n) {
+            f[0] = j.fin_scale * v0;
+            f[j.s_col] = j.fin_scale * v1;
+          }
+        }
       }
     }
-  } else if (warp < 24) {
-    regs_up<kRegsOut>();
-    // ---------------- epilogue: 64 columns of one token a thread
+  } else if (warp < 28) {
+    static_assert(kRegsOut == 64, "the launch's own");
+    const int half = warp >> 2 & 1;  // 32 of the 64 columns
+    // ---------------- epilogue: 32 columns of one token a thread
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
       Item w;
       item_of(args, idx, &w);
@@ -620,13 +647,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           pe = j.e.p + (packed ? 0 : w.seq) * j.e.sb + (packed ? w.start : 0) * j.e.st + (w.h / j.e.group) * j.e.sh + col0;
       }
       const int64_t stride = static_cast<int64_t>(args.la.H) * j.dc;
-      const int r0 = quad * 32 + (lane >> 3), c8 = lane & 7;  // rows r0, r0 + 4, ... of this warp's 32
+      const int r0 = quad * 32 + (lane >> 2), c4 = 4 * half + (lane & 3);  // rows r0, r0 + 8, ...; 16-byte column
       // the row's decay for the a . S part; read a chunk ahead, so that this role, the
       // last to need a table, does not keep the others waiting for the next
       float factor = 0.0f;
       auto read_factor = [&](uint32_t n) {
         const uint32_t b = n & 1u;
-        if (!warp_wait(&bar.gfull[b], (n >> 1) & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
+        if (!warp_wait(&bar.gfull[b], (n >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
         factor = rev ? to_end(tables[b], quad, row) : from_start(tables[b], quad, row);
         warp_arrive(&bar.gfree[b], lane);
         return true;
@@ -635,91 +662,96 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       for (int p = 0; ok && p < w.n; ++p, ++it) {
         const int64_t first = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC;  // in the sequence
         const int left = static_cast<int>(min(w.len - first, static_cast<int64_t>(kC)));            // tokens of the chunk
-        // Rows go through shared memory on their way to and from global memory (eight
-        // lanes a row of 128 bytes): a thread's own row would touch 32 lines an
+        // Rows go through shared memory on their way to and from global memory (four
+        // lanes this warp's 64 bytes of a row): a thread's own row would touch 32 lines an
         // instruction and hold up every barrier and shared-memory access of the CTA.
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t tile = base + (K::kOwnOut ? K::kOffOut : st * K::kStage + 2 * DKB * kTile);
-        uint4 e[8];
+        uint4 e[4];
         if constexpr (PRECISE) {
           if (pe != nullptr) {
-            const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c8;
+            const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c4;
 #pragma unroll
-            for (int q = 0; q < 8; ++q, src += 4 * j.e.st) {
+            for (int q = 0; q < 4; ++q, src += 8 * j.e.st) {
               e[q] = make_uint4(0u, 0u, 0u, 0u);
-              if (r0 + 4 * q < left && 8 * c8 < valid) e[q] = load_now(src);
+              if (r0 + 8 * q < left && 8 * c4 < valid) e[q] = load_now(src);
             }
           }
         }
         const float sc = args.la.scale, sx = sc * factor;
         const uint64_t sc2 = pair(sc, sc), sx2 = pair(sx, sx);
         if (p + 1 < w.n && !(ok = read_factor(it + 1))) break;
-        if (!(ok = warp_wait(&bar.o, it & 1u, status, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.o, it & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         if constexpr (PRECISE) {
           if (pe != nullptr) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) sts16(tile + swz(r0 + 4 * q, c8), e[q].x, e[q].y, e[q].z, e[q].w);
+            for (int q = 0; q < 4; ++q) sts16(tile + swz(r0 + 8 * q, c4), e[q].x, e[q].y, e[q].z, e[q].w);
             __syncwarp();
           }
         }
         const int64_t at = (w.start + first + r0) * stride + w.h * j.dc + col0;
-        uint32_t o[32];
-        uint64_t dot = 0;  // two FP32 sums
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          uint32_t x[16], y[16];
-          tmem_ld16(tmem + kTmOI + 16u * part + tm_lane, x);
-          tmem_ld16(tmem + kTmOX + 16u * part + tm_lane, y);
+        uint64_t dot[2] = {0, 0};  // four FP32 sums
+        uint32_t x[16], y[16];
+        const uint32_t tm = tmem + tm_lane + 32u * half;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {  // 16 columns
+          tmem_ld16(tm + kTmOI + 16u * part, x);
+          tmem_ld16(tm + kTmOX + 16u * part, y);
           tmem_wait_ld();
+          if (part == 1) {
+            // the accumulators are free before the stores: the next chunk's products wait for them
+            tc_fence_before();
+            warp_arrive(&bar.ofree, lane);
+          }
           uint64_t v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             v[i] = fma2(sx2, pair(y[2 * i], y[2 * i + 1]), mul2(sc2, pair(x[2 * i], x[2 * i + 1])));
-            uint32_t one[1];
-            split2<1>(v[i], one);
-            o[8 * part + i] = one[0];
           }
           if constexpr (PRECISE) {
-            if (f32) {  // (no dots then) 32 columns at a time fill the tile
+            if (f32) {  // (no dots then) 16 columns at a time fill this warp's half of the tile
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float z[4];
                 unpair(v[2 * q], z[0], z[1]);
                 unpair(v[2 * q + 1], z[2], z[3]);
-                sts16(tile + swz(row, 4 * (part & 1) + q), __float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]),
+                sts16(tile + swz(row, 4 * half + q), __float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]),
                       __float_as_uint(z[3]));
               }
-              if ((part & 1) != 0) {
-                __syncwarp();
-                const int c = 16 * (part - 1) + 4 * c8;
-                float* dst = reinterpret_cast<float*>(j.out) + at + c;
+              __syncwarp();
+              const int c = 32 * half + 16 * part + 4 * (lane & 3);
+              float* dst = reinterpret_cast<float*>(j.out) + at + c;
 #pragma unroll
-                for (int q = 0; q < 8; ++q, dst += 4 * stride)
-                  if (r0 + 4 * q < left && c < valid) *reinterpret_cast<uint4*>(dst) = lds16(tile + swz(r0 + 4 * q, c8));
-                __syncwarp();
-              }
+              for (int q = 0; q < 4; ++q, dst += 8 * stride)
+                if (r0 + 8 * q < left && c < valid) *reinterpret_cast<uint4*>(dst) = lds16(tile + swz(r0 + 8 * q, c4));
+              __syncwarp();
             } else if (pe != nullptr) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const uint4 u = lds16(tile + swz(row, 2 * part + q));
+                const uint4 u = lds16(tile + swz(row, 4 * half + 2 * part + q));
                 const uint32_t ew[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dot = fma2(v[4 * q + i], pair(ew[i] << 16, ew[i] & 0xFFFF0000u), dot);
+                for (int i = 0; i < 4; ++i)
+                  dot[i & 1] = fma2(v[4 * q + i], pair(ew[i] << 16, ew[i] & 0xFFFF0000u), dot[i & 1]);
               }
             }
           }
-        }
-        // the accumulators are free before the stores: the next chunk's products wait for them
-        tc_fence_before();
-        warp_arrive(&bar.ofree, lane);
-        uint4 rows[8];
-        if (!f32) {
+          if (!f32) {  // over the e that has just been read
 #pragma unroll
-          for (int q = 0; q < 8; ++q) sts16(tile + swz(row, q), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            for (int q = 0; q < 2; ++q) {
+              uint32_t o[4][1];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) split2<1>(v[4 * q + i], o[i]);
+              sts16(tile + swz(row, 4 * half + 2 * part + q), o[0][0], o[1][0], o[2][0], o[3][0]);
+            }
+          }
+        }
+        uint4 rows[4];
+        if (!f32) {
           __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) rows[q] = lds16(tile + swz(r0 + 4 * q, c8));
+          for (int q = 0; q < 4; ++q) rows[q] = lds16(tile + swz(r0 + 8 * q, c4));
         }
         if constexpr (K::kOwnOut) {
           __syncwarp();  // before the next chunk's rows
@@ -728,26 +760,26 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           warp_arrive(&bar.empty_c[st], lane);
         }
         if (!f32) {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(j.out) + at + 8 * c8;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(j.out) + at + 8 * c4;
 #pragma unroll
-          for (int q = 0; q < 8; ++q, dst += 4 * stride)
-            if (r0 + 4 * q < left && 8 * c8 < valid) *reinterpret_cast<uint4*>(dst) = rows[q];
+          for (int q = 0; q < 4; ++q, dst += 8 * stride)
+            if (r0 + 8 * q < left && 8 * c4 < valid) *reinterpret_cast<uint4*>(dst) = rows[q];
         }
         if constexpr (PRECISE) {
           if (pe != nullptr && row < left) {
             float d0, d1;
-            unpair(dot, d0, d1);
-            j.dots[(static_cast<int64_t>(w.slice) * args.la.H + w.h) * args.la.total + w.start + first + row] = d0 + d1;
+            unpair(add2(dot[0], dot[1]), d0, d1);
+            j.dots[(static_cast<int64_t>(2 * w.slice + half) * args.la.H + w.h) * args.la.total + w.start + first + row] = d0 + d1;
           }
         }
       }
     }
   } else {
     regs_down<kRegsRest>();
-    if (warp == 24 || warp == 27) {
+    if (warp == 28 || warp == 31) {
     // ---------------- TMA: a and b, and in a warp of its own c, whose tile is free later
     if (lane == 0) {
-      const bool ab = warp == 24;
+      const bool ab = warp == 28;
       uint64_t* const full = ab ? bar.full_ab : bar.full_c;
       for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
         Item w;
@@ -763,18 +795,18 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           const uint32_t stage = base + st * K::kStage;
           const int t = t0 + chunk * kC;
           if (!ab) {
-            if (!(ok = wait_for(&bar.empty_c[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+            if (!(ok = wait_for(&bar.empty_c[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
             mbar_arrive_expect_tx(&full[st], kTile);
             tma_load_4d(stage + 2 * DKB * kTile, &args.map[w.job][2], &full[st], 64 * w.slice, w.h / j.c.group, t, batch);
             continue;
           }
-          if (!(ok = wait_for(&bar.empty_b[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+          if (!(ok = wait_for(&bar.empty_b[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
           mbar_arrive_expect_tx(&full[st], (full_pass ? 2 * DKB : DKB) * kTile);
           for (int x = 0; x < DKB; ++x)
             tma_load_4d(stage + (DKB + x) * kTile, &args.map[w.job][1], &full[st], 64 * x, w.h / j.b.group, t, batch);
           if (full_pass) {
             // with b's copies on their way the count has to come to its end: a's follow even after a failed wait
-            ok = wait_for(&bar.empty_a[st], ph, status, SPX_DEV_TIMEOUT_PRODUCER);
+            ok = wait_for(&bar.empty_a[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER);
             for (int x = 0; x < DKB; ++x)
               tma_load_4d(stage + x * kTile, &args.map[w.job][0], &full[st], 64 * x, w.h / j.a.group, t, batch);
             if (!ok) {
@@ -787,11 +819,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       if (!ok) {  // leave no copy in flight behind an abandoned pipeline
         for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
           const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
-          wait_for(&full[s], (last / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_PRODUCER);
+          wait_for(&full[s], (last / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_PRODUCER);
         }
       }
     }
-    } else if (warp == 25) {
+    } else if (warp == 29) {
     // ---------------- MMA
     {
       const uint32_t id_ab = idesc_bf16_f32(128, 128);
@@ -805,9 +837,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       };
       auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
         const int st = static_cast<int>(n % K::kStages);
-        if (!warp_wait(&bar.full_ab[st], (n / K::kStages) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+        if (!warp_wait(&bar.full_ab[st], (n / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
         if (fixed(w, p)) {
-          if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
         }
         tc_fence_after();
@@ -846,7 +878,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!ready(nw, np, ahead)) return false;
         if (full_pass) {
           // the buffer's last reader: the product with c two chunks before
-          if (ahead >= 2 && !warp_wait(&bar.o, (ahead - 2) & 1u, status, SPX_DEV_TIMEOUT_MMA)) return false;
+          if (ahead >= 2 && !warp_wait(&bar.o, (ahead - 2) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
           product_ab(ahead);
         }
         ++ahead;
@@ -859,8 +891,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t stage = base + st * K::kStage;
         // state product b^T (scaled c)
-        if (!(ok = warp_wait(&bar.vp, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-        if (it > 0 && !(ok = warp_wait(&bar.kvfree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = warp_wait(&bar.vp, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+        if (it > 0 && !(ok = warp_wait(&bar.kvfree, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
         const uint64_t db = desc_mn(stage + DKB * kTile, kTile), dv = desc_mn(base + K::kOffV, kTile);
         if (elect_one()) {
@@ -881,8 +913,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         if (!(ok = start_next())) break;
         if (full_pass) {
           // a . S
-          if (!(ok = warp_wait(&bar.sop, it & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
-          if (it > 0 && !(ok = warp_wait(&bar.ofree, (it - 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = warp_wait(&bar.sop, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+          if (it > 0 && !(ok = warp_wait(&bar.ofree, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
           const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
           if (elect_one()) {
@@ -900,7 +932,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           // (decayed a . b) c
           const uint32_t b = it & 1u;
           const uint64_t dc = desc_mn(stage + 2 * DKB * kTile, kTile);
-          if (!(ok = warp_wait(&bar.pop[b], (it >> 1) & 1u, status, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = warp_wait(&bar.pop[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -920,7 +952,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       if (elect_one()) mma_commit(&bar.drained);  // arrives once everything issued above has completed
       __syncwarp();
     }
-    } else if (warp == 26) {
+    } else if (warp == 30) {
     // ---------------- decay tables: lane l of block b is token 32 b + l
     for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
       Item w;
@@ -964,7 +996,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             if (lane >= off) lg[q] += u;
           }
         }
-        if (!(ok = warp_wait(&bar.gfree[b], ((it >> 1) & 1u) ^ 1u, status, SPX_DEV_TIMEOUT_PRODUCER))) break;
+        if (!(ok = warp_wait(&bar.gfree[b], ((it >> 1) & 1u) ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
         DecayTable& t = tables[b];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -981,11 +1013,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 25) {
+  if (warp == 29) {
     // no MMA may still write the accumulators when they are freed
-    if (lane == 0) wait_for(&bar.drained, 0u, status, SPX_DEV_TIMEOUT_MMA);
+    if (lane == 0) wait_for(&bar.drained, 0u, failed, SPX_DEV_TIMEOUT_MMA);
     __syncwarp();
     tc_fence_after();
+    if (lane == 0 && *failed != 0) record_error(status, *failed);
     tmem_dealloc(tmem, kTmCols);
   }
 }

@@ -62,7 +62,8 @@ LaArgs base_args(const spx_linattn_dims& d, const spx_decays* g, const int32_t* 
   return a;
 }
 
-int slices_of(int width) { return (width + 63) / 64; }
+// Planes of the chunked form's dots: two for each 64 columns of an output.
+int planes_of(int width) { return 2 * ((width + 63) / 64); }
 
 template <typename T>
 T* at(void* base, size_t off) {
@@ -105,8 +106,8 @@ BackwardLayout backward_layout(const spx_linattn_dims& d) {
   };
   const size_t n = static_cast<size_t>(total_tokens(d)), h = static_cast<size_t>(d.heads);
   const size_t state = static_cast<size_t>(d.batch) * h * d.key_dim * d.value_dim * 4;
-  L.q_dots = take(n * h * 4 * slices_of(d.key_dim));
-  L.k_dots = take(n * h * 4 * slices_of(d.key_dim));
+  L.q_dots = take(n * h * 4 * planes_of(d.key_dim));
+  L.k_dots = take(n * h * 4 * planes_of(d.key_dim));
   L.last = take(state);
   if (d.heads != d.kv_heads) {
     L.dk = take(n * h * d.key_dim * 4);
@@ -377,7 +378,7 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   LaDecayGradArgs g{};
   g.q_dots = jq.dots;
   g.k_dots = at<float>(workspace, L.k_dots);
-  g.q_slices = recurrent(a) ? 1 : slices_of(K);
+  g.q_slices = recurrent(a) ? 1 : planes_of(K);
   g.k_slices = group > 1 ? 1 : g.q_slices;
   g.last = jq.fin;
   g.d_last = d_final_state;
