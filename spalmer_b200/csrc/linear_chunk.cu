@@ -61,7 +61,7 @@ constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
 // Registers of the warpgroups' threads: the launch gives each 64 (1024 x 64 = 65,536).
 constexpr int kRegsAB = 64, kRegsC = 48, kRegsState = 120, kRegsOut = 64, kRegsRest = 40;
 static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + 2 * kRegsOut + kRegsRest <= 8 * 64, "registers of a CTA");
-constexpr uint32_t kBarBytes = 304;
+constexpr uint32_t kBarBytes = 336;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -157,7 +157,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // mbar_wait that counts cycles instead of reading the timer: the kernel's 28
 // warps run through a dozen loops at once, and what the instruction cache does
 // not hold is fetched again for every chunk, so its hot code has to stay small.
-// One that gives up leaves its code in shared memory; the CTA's end records it.
+// A wait that gives up leaves its code in shared memory; the CTA's end records it.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* failed, int code) {
   if (mbar_try_wait(bar, parity)) return true;
   const int64_t start = clock64();
@@ -314,13 +314,8 @@ __device__ __forceinline__ void split2(uint64_t v, uint32_t (&part)[NP]) {
   }
 }
 
-// A load that stays where it is written (the compiler may move others down to their use).
-__device__ __forceinline__ uint4 load_now(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(reinterpret_cast<uint64_t>(p)));
-  return v;
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst_smem, const void* src, bool copy) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(copy ? 16 : 0) : "memory");
 }
 
 struct Bars {
@@ -328,7 +323,8 @@ struct Bars {
   uint64_t gfull[2], gfree[2];
   uint64_t pacc[2], pop[2];
   uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
-  uint64_t vp, kv, kvfree, sop, qs, o, ofree, drained;
+  uint64_t vp[2], kv[2], kvfree[2];  // by the chunk's parity
+  uint64_t sop, qs, o, ofree, drained;
   uint32_t tmem;
   int failed;
 };
@@ -352,6 +348,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform to the compiler
   const bool full_pass = args.state_only == 0;
   const int items = args.lanes[args.la.njobs] * args.run_segs;
+  // The state-only pass has room for two chunks' parts of scaled c (the second in
+  // the places of a and of the state's operand) and two accumulators, so that
+  // scaling, product and update of neighbouring chunks overlap.
+  const uint32_t depth = full_pass ? 1u : 2u;
+  auto part_at = [&](uint32_t n, uint32_t part) {  // the part's tile for chunk n
+    if (full_pass || (n & 1u) == 0u) return base + K::kOffV + part * kTile;
+    if constexpr (DKB == 1) return base + part * K::kStage;
+    return part < 2u ? base + part * kTile : base + K::kOffS;
+  };
+  auto acc_at = [&](uint32_t n) { return full_pass || (n & 1u) == 0u ? kTmKV : kTmP; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 3; ++s) {
@@ -367,10 +373,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       mbar_init(&bar.pacc[s], 1);
       mbar_init(&bar.pop[s], 8);
       mbar_init(&bar.tail[s], 8);
+      mbar_init(&bar.vp[s], 8);
+      mbar_init(&bar.kv[s], 1);
+      mbar_init(&bar.kvfree[s], 4);
     }
-    mbar_init(&bar.vp, 8);
-    mbar_init(&bar.kv, 1);
-    mbar_init(&bar.kvfree, 4);
     mbar_init(&bar.sop, 4);
     mbar_init(&bar.qs, 1);
     mbar_init(&bar.o, 1);
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
         if (!(ok = warp_wait(&bar.full_c[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const uint32_t stage = base + st * K::kStage;
-        const uint32_t sc = stage + 2 * DKB * kTile;
+        const uint32_t sc_row = stage + 2 * DKB * kTile + swz(row, 0);  // ^ (c << 4): the row's chunk c
         if (len < kC && args.la.cu != nullptr) {
           // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
           if (!(ok = warp_wait(&bar.full_ab[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
@@ -505,27 +511,30 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
               for (int c = 0; c < 4; ++c) sts16(stage + (DKB + x) * kTile + row * 128 + (4 * half + c) * 16, 0u, 0u, 0u, 0u);
           }
           fence_proxy_async_smem();
-          warp_arrive(&bar.tail[tails++ & 1u], lane);
+          if (full_pass) warp_arrive(&bar.tail[tails++ & 1u], lane);  // else the product alone reads them, after vp
         }
         if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
         warp_arrive(&bar.gfree[b], lane);
         const uint64_t wgt2 = pair(wgt, wgt);
-        // the parts' last reader: the state product of the chunk before
-        if (it > 0 && !(ok = warp_wait(&bar.kv, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        // the parts' last reader: the state product of the chunk before (or the one before that)
+        if (it >= depth && !(ok = warp_wait(&bar.kv[(it - depth) & 1u], ((it - depth) >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        uint32_t dst[K::kParts];
+#pragma unroll
+        for (int part = 0; part < K::kParts; ++part) dst[part] = part_at(it, part) + swz(row, 0);
 #pragma unroll 1
         for (int c = 4 * half; c < 4 * half + 4; ++c) {
-          const uint4 u = lds16(sc + swz(row, c));
+          const uint4 u = lds16(sc_row ^ (c << 4));
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
           uint32_t q[4][K::kParts];
 #pragma unroll
           for (int e = 0; e < 4; ++e) split2<K::kParts>(mul2(pair(uw[e] << 16, uw[e] & 0xFFFF0000u), wgt2), q[e]);
 #pragma unroll
           for (int part = 0; part < K::kParts; ++part)
-            sts16(base + K::kOffV + part * kTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
+            sts16(dst[part] ^ (c << 4), q[0][part], q[1][part], q[2][part], q[3][part]);
         }
         fence_proxy_async_smem();
-        warp_arrive(&bar.vp, lane);
+        warp_arrive(&bar.vp[b], lane);
       }
     }
   } else if (warp < 20) {
@@ -586,14 +595,15 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         warp_arrive(&bar.gfree[b], lane);
         const uint64_t gamma2 = pair(gamma, gamma);
         decay *= gamma;
-        if (!(ok = warp_wait(&bar.kv, it & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&bar.kv[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const uint32_t acc = tmem + acc_at(it) + tm_lane;
         tc_fence_after();
         if (rows_in) {
 #pragma unroll
           for (int part = 0; part < 4; ++part) {
             uint32_t x[16], y[16];
-            tmem_ld16(tmem + kTmKV + 16u * part + tm_lane, x);
-            if constexpr (K::kParts == 2) tmem_ld16(tmem + kTmKV + 64u + 16u * part + tm_lane, y);
+            tmem_ld16(acc + 16u * part, x);
+            if constexpr (K::kParts == 2) tmem_ld16(acc + 64u + 16u * part, y);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           }
         }
         tc_fence_before();
-        warp_arrive(&bar.kvfree, lane);
+        warp_arrive(&bar.kvfree[b], lane);
       }
       if (!ok) break;
       if (!full_pass) {
@@ -667,16 +677,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         // instruction and hold up every barrier and shared-memory access of the CTA.
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t tile = base + (K::kOwnOut ? K::kOffOut : st * K::kStage + 2 * DKB * kTile);
-        uint4 e[4];
-        if constexpr (PRECISE) {
-          if (pe != nullptr) {
-            const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c4;
+        auto fetch_e = [&]() {  // rows past the sequence and columns past the width read as zero
+          const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c4;
 #pragma unroll
-            for (int q = 0; q < 4; ++q, src += 8 * j.e.st) {
-              e[q] = make_uint4(0u, 0u, 0u, 0u);
-              if (r0 + 8 * q < left && 8 * c4 < valid) e[q] = load_now(src);
-            }
+          for (int q = 0; q < 4; ++q, src += 8 * j.e.st) {
+            const bool in = r0 + 8 * q < left && 8 * c4 < valid;
+            cp_async16_or_zero(tile + swz(r0 + 8 * q, c4), in ? src : pe, in);
           }
+        };
+        if constexpr (PRECISE && K::kOwnOut) {
+          if (pe != nullptr) fetch_e();
         }
         const float sc = args.la.scale, sx = sc * factor;
         const uint64_t sc2 = pair(sc, sc), sx2 = pair(sx, sx);
@@ -685,8 +695,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         tc_fence_after();
         if constexpr (PRECISE) {
           if (pe != nullptr) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) sts16(tile + swz(r0 + 8 * q, c4), e[q].x, e[q].y, e[q].z, e[q].w);
+            if constexpr (!K::kOwnOut) fetch_e();  // the tile is the chunk's c, free now
+            cp_async_wait_all();
             __syncwarp();
           }
         }
@@ -838,7 +848,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
         const int st = static_cast<int>(n % K::kStages);
         if (!warp_wait(&bar.full_ab[st], (n / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
-        if (fixed(w, p)) {
+        if (full_pass && fixed(w, p)) {
           if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
         }
@@ -891,10 +901,14 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const int st = static_cast<int>(it % K::kStages);
         const uint32_t stage = base + st * K::kStage;
         // state product b^T (scaled c)
-        if (!(ok = warp_wait(&bar.vp, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
-        if (it > 0 && !(ok = warp_wait(&bar.kvfree, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = warp_wait(&bar.vp[it & 1u], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+        if (it >= depth && !(ok = warp_wait(&bar.kvfree[(it - depth) & 1u], ((it - depth) >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
-        const uint64_t db = desc_mn(stage + DKB * kTile, kTile), dv = desc_mn(base + K::kOffV, kTile);
+        const uint64_t db = desc_mn(stage + DKB * kTile, kTile);
+        uint64_t dv[K::kParts];  // (two parts: the first, with the distance to the second)
+#pragma unroll
+        for (uint32_t part = 0; part < K::kParts; ++part) dv[part] = desc_mn(part_at(it, part), part_at(it, 1) - part_at(it, 0));
+        const uint32_t acc = tmem + acc_at(it);
         if (elect_one()) {
 #pragma unroll
           for (uint32_t q = 0; q < 8; ++q) {
@@ -902,10 +916,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             // into the same 64 (MMAs of different shapes on one accumulator have no order)
 #pragma unroll
             for (uint32_t part = 0; part < (K::kParts == 3 ? 3u : 1u); ++part)
-              mma_bf16_ss(tmem + kTmKV, db + q * 128u, dv + (part * (kTile >> 4) + q * 128u), id_kv,
-                          (part | q) != 0u ? 1u : 0u);
+              mma_bf16_ss(acc, db + q * 128u, dv[part] + q * 128u, id_kv, (part | q) != 0u ? 1u : 0u);
           }
-          mma_commit(&bar.kv);
+          mma_commit(&bar.kv[it & 1u]);
           mma_commit(&bar.empty_b[st]);  // a . b of this chunk was issued before
           if (!full_pass) mma_commit(&bar.empty_c[st]);
         }
