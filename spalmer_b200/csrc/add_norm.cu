@@ -15,13 +15,17 @@
 // BF16 roundings between the products of the module it replaces).
 //
 // The pass is bound by HBM: each tensor is read or written once.  A row is
-// held in the registers of 32 * WPR threads (NC 16-byte chunks of BF16 each),
+// held in the registers of 32 * WPR threads (NC chunks of eight elements each),
 // so the statistics cost no second read; a CTA walks rows with a stride, which
-// keeps w in registers for all of them.  MXFP8: four neighbouring lanes hold a
-// block of 32, so its largest magnitude is two shuffles.
+// keeps w in registers for all of them, and a row's loads are issued while the
+// row before is worked on (loads between the stores of one row went one after
+// another: 132 us instead of @FWD@ us for 65,536 rows of 768).  MXFP8: four
+// neighbouring lanes hold a block of 32, so its largest magnitude is two shuffles.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "kernels.h"
 #include "mx.cuh"
@@ -52,13 +56,27 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void load8(const void* base, int64_t at, bool f32, float (&v)[8]) {
-  if (f32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// Eight elements as they are stored: BF16 in one register quad, FP32 in two.
+template <bool F32>
+struct Raw8 {
+  uint4 u[F32 ? 2 : 1];
+};
+
+template <bool F32>
+__device__ __forceinline__ void load_raw(const void* base, int64_t at, Raw8<F32>& r) {
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at * (F32 ? 4 : 2));
+#pragma unroll
+  for (int i = 0; i < (F32 ? 2 : 1); ++i) r.u[i] = __ldg(p + i);
+}
+
+template <bool F32>
+__device__ __forceinline__ void unpack8(const Raw8<F32>& r, float (&v)[8]) {
+  if constexpr (F32) {
+    const uint32_t w[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
   } else {
-    unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + at), v);
+    unpack8(r.u[0], v);
   }
 }
 
@@ -89,7 +107,8 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, i
 #pragma unroll
       for (int j = 0; j < N; ++j) p[wr * N + j] = s[j];
     }
-    __syncthreads();
+    // the row's warps alone
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * WPR) : "memory");
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float t = 0.0f;
@@ -102,15 +121,33 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, i
 
 }  // namespace
 
-template <int WPR, int NC>
-__global__ void __launch_bounds__(kNormThreads) add_norm_kernel(const AddNormArgs a) {
+// RES: 0 no residual, 1 BF16, 2 FP32.
+template <int WPR, int NC, int RES>
+__global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNormArgs a) {
   constexpr int kGroups = kNormThreads / (32 * WPR);
   __shared__ float part[2 * kGroups * WPR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = warp / WPR, wr = warp % WPR;
   const int nchunks = a.d / 8;
   const float inv_d = 1.0f / static_cast<float>(a.d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   uint4 wv[NC];
+  Raw8<false> xr[NC];
+  Raw8<RES == 2> rr[NC];
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * WPR + wr) * 32 + lane;
+      if (c < nchunks) {
+        load_raw<false>(a.x, row * a.ld_x + c * 8, xr[i]);
+        if constexpr (RES != 0) load_raw<RES == 2>(a.res, row * a.ld_res + c * 8, rr[i]);
+      }
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  constexpr bool kAhead = NC <= 2;
+  if (kAhead) fetch(row);
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = (i * WPR + wr) * 32 + lane;
@@ -118,26 +155,24 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_kernel(const AddNormArg
   }
   uint32_t turn = 0;
   // every warp of the CTA runs the same number of rows (row_sum has a barrier)
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups; row0 < a.rows;
-       row0 += static_cast<int64_t>(gridDim.x) * kGroups, ++turn) {
-    const int64_t row = row0 + group;
+  for (int64_t row0 = row - group; row0 < a.rows; row0 += step, row += step, ++turn) {
     const bool live = row < a.rows;
+    if (!kAhead) fetch(row);
     float h[NC][8];
     float s[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = (i * WPR + wr) * 32 + lane;
       if (live && c < nchunks) {
-        load8(a.x, row * a.ld_x + c * 8, false, h[i]);
-        if (a.res != nullptr) {
+        unpack8(xr[i], h[i]);
+        if constexpr (RES != 0) {
           float r[8];
-          load8(a.res, row * a.ld_res + c * 8, a.res_f32 != 0, r);
+          unpack8(rr[i], r);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             h[i][j] += r[j];
-            if (a.res_f32 == 0) h[i][j] = round_bf16(h[i][j]);
+            if (RES == 1) h[i][j] = round_bf16(h[i][j]);
           }
-          store8(a.sum, row * a.d + c * 8, a.res_f32 != 0, h[i]);
         }
       } else {
 #pragma unroll
@@ -145,6 +180,14 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_kernel(const AddNormArg
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[0] = fmaf(h[i][j], h[i][j], s[0]);
+    }
+    if (kAhead) fetch(row + step);
+    if constexpr (RES != 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = (i * WPR + wr) * 32 + lane;
+        if (live && c < nchunks) store8(a.sum, row * a.d + c * 8, RES == 2, h[i]);
+      }
     }
     row_sum<WPR, 1>(s, part, group, wr, lane, turn);
     const float r = 1.0f / sqrtf(s[0] * inv_d + a.eps);
@@ -180,8 +223,8 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_kernel(const AddNormArg
 
 // dw is summed per thread over the CTA's rows, then over the CTA's row groups
 // in shared memory, then over CTAs by norm_dw_kernel: a fixed order, no atomics.
-template <int WPR, int NC>
-__global__ void __launch_bounds__(kNormThreads) add_norm_backward_kernel(const AddNormBackwardArgs a) {
+template <int WPR, int NC, bool F32>
+__global__ void __launch_bounds__(kNormThreads, 1) add_norm_backward_kernel(const AddNormBackwardArgs a) {
   constexpr int kGroups = kNormThreads / (32 * WPR);
   constexpr int kCols = 32 * WPR * 8;  // columns of one chunk index
   __shared__ float part[2 * kGroups * WPR * 2];
@@ -190,8 +233,25 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_backward_kernel(const A
   const int group = warp / WPR, wr = warp % WPR;
   const int nchunks = a.d / 8;
   const float inv_d = 1.0f / static_cast<float>(a.d);
-  uint4 wv[NC];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  uint4 wv[NC], gr[NC];
+  Raw8<F32> hr[NC], sr[NC];
   float dw[NC][8];
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * WPR + wr) * 32 + lane;
+      if (c < nchunks) {
+        gr[i] = __ldg(reinterpret_cast<const uint4*>(a.dy + row * a.ld_dy) + c);
+        load_raw<F32>(a.h, row * a.ld_h + c * 8, hr[i]);
+        if (a.dsum != nullptr) load_raw<F32>(a.dsum, row * a.ld_dsum + c * 8, sr[i]);
+      }
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  constexpr bool kAhead = NC <= 2;
+  if (kAhead) fetch(row);
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = (i * WPR + wr) * 32 + lane;
@@ -200,33 +260,28 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_backward_kernel(const A
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.0f;
   }
   uint32_t turn = 0;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups; row0 < a.rows;
-       row0 += static_cast<int64_t>(gridDim.x) * kGroups, ++turn) {
-    const int64_t row = row0 + group;
+  for (int64_t row0 = row - group; row0 < a.rows; row0 += step, row += step, ++turn) {
     const bool live = row < a.rows;
-    float h[NC][8];
+    if (!kAhead) fetch(row);
+    Raw8<F32> h[NC], ds[NC];
     uint4 g[NC];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = (i * WPR + wr) * 32 + lane;
-      if (live && c < nchunks) {
-        g[i] = *reinterpret_cast<const uint4*>(a.dy + row * a.ld_dy + c * 8);
-        load8(a.h, row * a.ld_h + c * 8, a.res_f32 != 0, h[i]);
-      } else {
-        g[i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
-      }
-      float wf[8], gf[8];
+      h[i] = hr[i], g[i] = gr[i], ds[i] = sr[i];
+      if (!live || c >= nchunks) continue;
+      float wf[8], gf[8], hf[8];
       unpack8(wv[i], wf);
       unpack8(g[i], gf);
+      unpack8(h[i], hf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[0] = fmaf(h[i][j], h[i][j], s[0]);
-        s[1] = fmaf(gf[j] * wf[j], h[i][j], s[1]);
+        s[0] = fmaf(hf[j], hf[j], s[0]);
+        s[1] = fmaf(gf[j] * wf[j], hf[j], s[1]);
       }
     }
+    if (kAhead) fetch(row + step);
     row_sum<WPR, 2>(s, part, group, wr, lane, turn);
     const float r = 1.0f / sqrtf(s[0] * inv_d + a.eps);
     const float k = r * r * s[1] * inv_d;
@@ -234,22 +289,23 @@ __global__ void __launch_bounds__(kNormThreads) add_norm_backward_kernel(const A
     for (int i = 0; i < NC; ++i) {
       const int c = (i * WPR + wr) * 32 + lane;
       if (!live || c >= nchunks) continue;
-      float wf[8], gf[8], dh[8];
+      float wf[8], gf[8], hf[8], dh[8];
       unpack8(wv[i], wf);
       unpack8(g[i], gf);
+      unpack8(h[i], hf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        dw[i][j] = fmaf(gf[j] * h[i][j], r, dw[i][j]);
-        dh[j] = r * (gf[j] * wf[j] - h[i][j] * k);
+        dw[i][j] = fmaf(gf[j] * hf[j], r, dw[i][j]);
+        dh[j] = r * (gf[j] * wf[j] - hf[j] * k);
       }
       if (a.dsum != nullptr) {
-        float ds[8];
-        load8(a.dsum, row * a.ld_dsum + c * 8, a.res_f32 != 0, ds);
+        float sf[8];
+        unpack8(ds[i], sf);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dh[j] += ds[j];
+        for (int j = 0; j < 8; ++j) dh[j] += sf[j];
       }
       store8(a.dx, row * a.d + c * 8, false, dh);
-      if (a.dres != nullptr) store8(a.dres, row * a.d + c * 8, true, dh);
+      if (F32 && a.dres != nullptr) store8(a.dres, row * a.d + c * 8, true, dh);
     }
   }
   if (a.dw_part == nullptr) return;
@@ -317,7 +373,31 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ 
 
 namespace {
 
-int norm_wpr(int d) { return d <= 1024 ? 1 : d <= 4096 ? 4 : 16; }
+// Threads of a row: up to two chunks a thread (registers for this row and the
+// next), from one warp to sixteen; beyond that more chunks, loaded row by row.
+int norm_wpr(int d) {
+  int wpr = 1;
+  while (wpr < 16 && 32 * wpr * 2 < d / 8) wpr *= 2;
+  return wpr;
+}
+
+// kernel(wpr, nc) as compile-time constants
+template <typename F>
+int with_shape(int d, F&& f) {
+  const int wpr = norm_wpr(d);
+  const int nc = (d / 8 + 32 * wpr - 1) / (32 * wpr);
+  using std::integral_constant;
+  auto pick = [&](auto w) {
+    return nc <= 1 ? f(w, integral_constant<int, 1>{}) : f(w, integral_constant<int, 2>{});
+  };
+  switch (wpr) {
+    case 1: return pick(integral_constant<int, 1>{});
+    case 2: return pick(integral_constant<int, 2>{});
+    case 4: return pick(integral_constant<int, 4>{});
+    case 8: return pick(integral_constant<int, 8>{});
+    default: return nc <= 2 ? pick(integral_constant<int, 16>{}) : f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  }
+}
 
 int norm_grid(int64_t rows, int wpr, int per_sm) {
   const int groups = kNormThreads / (32 * wpr);
@@ -329,20 +409,21 @@ int norm_grid(int64_t rows, int wpr, int per_sm) {
 }  // namespace
 
 // Rows of partial dw sums that launch_add_norm_backward writes (d floats each).
-int add_norm_backward_parts(int64_t rows, int d) { return norm_grid(rows, norm_wpr(d), 2); }
+int add_norm_backward_parts(int64_t rows, int d) { return norm_grid(rows, norm_wpr(d), 1); }
 
 int launch_add_norm(const AddNormArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return SPX_OK;
-  const int wpr = norm_wpr(a.d);
-  const int grid = norm_grid(a.rows, wpr, 4);
-  const int nc = (a.d / 8 + 32 * wpr - 1) / (32 * wpr);
-  auto run = [&](auto kernel) {
-    kernel<<<grid, kNormThreads, 0, stream>>>(a);
+  const int grid = norm_grid(a.rows, norm_wpr(a.d), 2);
+  return with_shape(a.d, [&](auto w, auto n) {
+    constexpr int W = decltype(w)::value, N = decltype(n)::value;
+    if (a.res == nullptr)
+      add_norm_kernel<W, N, 0><<<grid, kNormThreads, 0, stream>>>(a);
+    else if (a.res_f32 == 0)
+      add_norm_kernel<W, N, 1><<<grid, kNormThreads, 0, stream>>>(a);
+    else
+      add_norm_kernel<W, N, 2><<<grid, kNormThreads, 0, stream>>>(a);
     return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
-  };
-  if (wpr == 1) return nc == 1 ? run(add_norm_kernel<1, 1>) : nc <= 3 ? run(add_norm_kernel<1, 3>) : run(add_norm_kernel<1, 4>);
-  if (wpr == 4) return nc <= 2 ? run(add_norm_kernel<4, 2>) : run(add_norm_kernel<4, 4>);
-  return nc <= 2 ? run(add_norm_kernel<16, 2>) : run(add_norm_kernel<16, 4>);
+  });
 }
 
 int launch_add_norm_backward(const AddNormBackwardArgs& a, uint16_t* dw, cudaStream_t stream) {
@@ -350,20 +431,15 @@ int launch_add_norm_backward(const AddNormBackwardArgs& a, uint16_t* dw, cudaStr
     if (dw == nullptr) return SPX_OK;
     return cudaMemsetAsync(dw, 0, static_cast<size_t>(a.d) * 2, stream) == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
   }
-  const int wpr = norm_wpr(a.d);
   const int grid = add_norm_backward_parts(a.rows, a.d);
-  const int nc = (a.d / 8 + 32 * wpr - 1) / (32 * wpr);
-  auto run = [&](auto kernel) {
-    kernel<<<grid, kNormThreads, 0, stream>>>(a);
+  const int rc = with_shape(a.d, [&](auto w, auto n) {
+    constexpr int W = decltype(w)::value, N = decltype(n)::value;
+    if (a.res_f32 == 0)
+      add_norm_backward_kernel<W, N, false><<<grid, kNormThreads, 0, stream>>>(a);
+    else
+      add_norm_backward_kernel<W, N, true><<<grid, kNormThreads, 0, stream>>>(a);
     return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
-  };
-  int rc;
-  if (wpr == 1)
-    rc = nc == 1 ? run(add_norm_backward_kernel<1, 1>) : nc <= 3 ? run(add_norm_backward_kernel<1, 3>) : run(add_norm_backward_kernel<1, 4>);
-  else if (wpr == 4)
-    rc = nc <= 2 ? run(add_norm_backward_kernel<4, 2>) : run(add_norm_backward_kernel<4, 4>);
-  else
-    rc = nc <= 2 ? run(add_norm_backward_kernel<16, 2>) : run(add_norm_backward_kernel<16, 4>);
+  });
   if (rc != SPX_OK || dw == nullptr) return rc;
   return launch_pdl(norm_dw_kernel, dim3((a.d + 31) / 32), dim3(256), 0, stream, a.dw_part, grid, a.d, dw);
 }
