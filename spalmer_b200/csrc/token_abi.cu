@@ -33,12 +33,27 @@ int check_dims(const spx_linattn_dims* d) {
 
 int64_t total_tokens(const spx_linattn_dims& d) { return d.packed != 0 ? d.seq_len : d.batch * d.seq_len; }
 
-int check_heads(const spx_heads* t) {
+// Pointer, alignment and strides; the stride of a dimension of one element is not used.
+int check_heads(const spx_heads* t, int64_t batch, int64_t tokens, int64_t heads) {
   if (t == nullptr || t->ptr == nullptr) return SPX_ERR_INVALID_ARG;
-  if (!aligned(t->ptr) || t->batch_stride % 8 != 0 || t->token_stride % 8 != 0 || t->head_stride % 8 != 0)
-    return SPX_ERR_ALIGNMENT;
-  if (t->batch_stride < 0 || t->token_stride < 0 || t->head_stride < 0) return SPX_ERR_INVALID_ARG;
-  return SPX_OK;
+  const int64_t extent[3] = {batch, tokens, heads}, stride[3] = {t->batch_stride, t->token_stride, t->head_stride};
+  bool misaligned = !aligned(t->ptr);
+  for (int i = 0; i < 3; ++i) {
+    if (extent[i] <= 1) continue;
+    if (stride[i] < 0) return SPX_ERR_INVALID_ARG;
+    if (stride[i] % 8 != 0) misaligned = true;
+  }
+  return misaligned ? SPX_ERR_ALIGNMENT : SPX_OK;
+}
+
+// Of q, k, v (and the output's gradient) of a call over sequences.
+int check_sequences(const spx_linattn_dims& d, const spx_heads* q, const spx_heads* k, const spx_heads* v,
+                    const spx_heads* d_out) {
+  const int64_t rows = d.packed != 0 ? 1 : d.batch;
+  if (int rc = check_heads(q, rows, d.seq_len, d.heads); rc != SPX_OK) return rc;
+  if (int rc = check_heads(k, rows, d.seq_len, d.kv_heads); rc != SPX_OK) return rc;
+  if (int rc = check_heads(v, rows, d.seq_len, d.kv_heads); rc != SPX_OK) return rc;
+  return d_out == nullptr ? SPX_OK : check_heads(d_out, rows, d.seq_len, d.heads);
 }
 
 LaOperand operand(const spx_heads* t, int group) {
@@ -244,8 +259,7 @@ int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const
   if (d.batch == 0) return SPX_OK;
   if (d.packed != 0 && cu_seqlens == nullptr) return SPX_ERR_INVALID_ARG;
   if (total_tokens(d) > 0) {
-    for (const spx_heads* t : {q, k, v})
-      if (int rc = check_heads(t); rc != SPX_OK) return rc;
+    if (int rc = check_sequences(d, q, k, v, nullptr); rc != SPX_OK) return rc;
     if (decays == nullptr || decays->ptr == nullptr || out == nullptr) return SPX_ERR_INVALID_ARG;
   } else if (q == nullptr || k == nullptr || v == nullptr || decays == nullptr) {
     return SPX_ERR_INVALID_ARG;
@@ -288,8 +302,8 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   if (d.packed != 0 && cu_seqlens == nullptr) return SPX_ERR_INVALID_ARG;
   const int64_t total = total_tokens(d);
   if (total > 0) {
-    for (const spx_heads* t : {q, k, v, d_out})
-      if (int rc = check_heads(t); rc != SPX_OK) return rc;
+    if (d_out == nullptr) return SPX_ERR_INVALID_ARG;
+    if (int rc = check_sequences(d, q, k, v, d_out); rc != SPX_OK) return rc;
     if (decays == nullptr || decays->ptr == nullptr || d_q == nullptr || d_k == nullptr || d_v == nullptr ||
         d_decay == nullptr)
       return SPX_ERR_INVALID_ARG;
@@ -403,8 +417,9 @@ int spx_linear_attention_step(const spx_heads* q, const spx_heads* k, const spx_
   if (key_dim % 8 != 0 || value_dim % 8 != 0 || key_dim > kLaMaxD || value_dim > kLaMaxD) return SPX_ERR_UNSUPPORTED;
   if (batch == 0) return SPX_OK;
   if (slot_index == nullptr && batch > slots) return SPX_ERR_INVALID_ARG;
-  for (const spx_heads* t : {q, k, v})
-    if (int rc = check_heads(t); rc != SPX_OK) return rc;
+  if (int rc = check_heads(q, batch, 1, heads); rc != SPX_OK) return rc;
+  if (int rc = check_heads(k, batch, 1, kv_heads); rc != SPX_OK) return rc;
+  if (int rc = check_heads(v, batch, 1, kv_heads); rc != SPX_OK) return rc;
   if (decays == nullptr || decays->ptr == nullptr || (state == nullptr && slots > 0) || out == nullptr)
     return SPX_ERR_INVALID_ARG;
   if (!aligned(state) || !aligned(out)) return SPX_ERR_ALIGNMENT;

@@ -26,8 +26,24 @@ from spalmer_b200 import _lib
 _MAX_HEAD_DIM = 128
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_BF16, _F32 = torch.bfloat16, torch.float32
+_FLOATS = (_F32, _BF16)
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(i).cuda_stream without the Stream object
+_current_device = torch.cuda.current_device
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """Call a libspx entry point on the current stream of ``device`` (which it gets as its last argument)."""
+
+    index = device.index
+    fn = getattr(_lib.load(), name)
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def _require(tensor: Tensor, name: str, dtype: torch.dtype | tuple, device: torch.device | None = None) -> None:
@@ -39,11 +55,20 @@ def _require(tensor: Tensor, name: str, dtype: torch.dtype | tuple, device: torc
         raise ValueError(f"{name} is on {tensor.device}, not on {device}")
 
 
+def _ptr(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 # ---------------------------------------------------------------- residual + RMSNorm
 def _rows(t: Tensor, d: int, item: int) -> Tensor:
     """``t`` as [rows, d] whose rows start on 16 bytes (a copy only if it must be)."""
 
-    r = t.reshape(-1, d)
+    if t.is_contiguous():
+        r = t.view(-1, d)
+        if not r.data_ptr() % 16 and not d * item % 16:
+            return r
+    else:
+        r = t.reshape(-1, d)
     if r.shape[0] and (r.stride(1) != 1 or (r.stride(0) * item) % 16 or r.data_ptr() % 16):
         r = r.contiguous()
         if r.data_ptr() % 16:
@@ -75,22 +100,21 @@ def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: 
     d = hidden.shape[-1]
     x = _rows(hidden, d, 2)
     n, dev = x.shape[0], x.device
-    f32 = residual is not None and residual.dtype == torch.float32
-    r = None if residual is None else _rows(residual, d, 4 if f32 else 2)
+    r, f32, total, scales = None, False, hidden, None
+    if residual is not None:
+        f32 = residual.dtype == _F32
+        r = _rows(residual, d, 4 if f32 else 2)
+        total = torch.empty_like(residual, memory_format=torch.contiguous_format)
     w = weight.contiguous()
-    total = hidden if r is None else torch.empty(hidden.shape, dtype=residual.dtype, device=dev)
-    scales = None
     if mxfp8:
-        out = torch.empty(hidden.shape, dtype=torch.uint8, device=dev)
-        scales = torch.empty(*hidden.shape[:-1], d // 32, dtype=torch.uint8, device=dev)
+        out = hidden.new_empty(hidden.shape, dtype=torch.uint8)
+        scales = hidden.new_empty((*hidden.shape[:-1], d // 32), dtype=torch.uint8)
     else:
-        out = torch.empty(hidden.shape, dtype=torch.bfloat16, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.spx_add_rmsnorm_rows(
-            x.data_ptr(), x.stride(0), _lib.ptr(r), 0 if r is None else r.stride(0), int(f32), w.data_ptr(), float(eps),
-            n, d, None if r is None else total.data_ptr(), None if mxfp8 else out.data_ptr(),
-            out.data_ptr() if mxfp8 else None, _lib.ptr(scales), _stream(dev)), "spx_add_rmsnorm_rows")
+        out = torch.empty_like(hidden, memory_format=torch.contiguous_format)
+    ptr = out.data_ptr()
+    _call("spx_add_rmsnorm_rows", dev, x.data_ptr(), x.stride(0), _ptr(r), 0 if r is None else r.stride(0), f32,
+          w.data_ptr(), eps, n, d, None if r is None else total.data_ptr(), None if mxfp8 else ptr,
+          ptr if mxfp8 else None, _ptr(scales))
     return out, scales, total
 
 
@@ -109,30 +133,29 @@ class _AddRMSNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_out, d_total):
         total, weight = ctx.saved_tensors
-        d = total.shape[-1]
+        d = weight.shape[0]
         dev = total.device
         if d_out is None:
-            d_out = torch.zeros(total.shape, dtype=torch.bfloat16, device=dev)
-        f32 = total.dtype == torch.float32
+            d_out = torch.zeros(total.shape, dtype=_BF16, device=dev)
+        f32 = total.dtype == _F32
         item = 4 if f32 else 2
-        h, dy = _rows(total, d, item), _rows(d_out.to(torch.bfloat16), d, 2)
-        ds = None if d_total is None else _rows(d_total.to(total.dtype), d, item)
+        h, dy = _rows(total, d, item), _rows(d_out, d, 2)
+        ds = None if d_total is None else _rows(d_total, d, item)
         n = h.shape[0]
-        d_hidden = torch.empty(total.shape, dtype=torch.bfloat16, device=dev)
-        d_residual = torch.empty(total.shape, dtype=torch.float32, device=dev) if f32 else None
-        d_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
-        lib = _lib.load()
-        nbytes = lib.spx_add_rmsnorm_backward_workspace(n, d) if d_weight is not None else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with torch.cuda.device(dev):
-            _lib.check(lib.spx_add_rmsnorm_backward(
-                h.data_ptr(), h.stride(0), int(f32), weight.contiguous().data_ptr(), ctx.eps, dy.data_ptr(),
-                dy.stride(0), _lib.ptr(ds), 0 if ds is None else ds.stride(0), n, d, d_hidden.data_ptr(),
-                _lib.ptr(d_residual), _lib.ptr(d_weight), _lib.ptr(ws), nbytes, _stream(dev)),
-                "spx_add_rmsnorm_backward")
+        d_hidden = torch.empty_like(d_out, memory_format=torch.contiguous_format)
+        d_residual = torch.empty_like(total, memory_format=torch.contiguous_format) if f32 else None
+        d_weight = ws = None
+        nbytes = 0
+        if ctx.needs_input_grad[2]:
+            d_weight = torch.empty_like(weight, memory_format=torch.contiguous_format)
+            nbytes = _lib.load().spx_add_rmsnorm_backward_workspace(n, d)
+            ws = weight.new_empty(nbytes, dtype=torch.uint8)
+        _call("spx_add_rmsnorm_backward", dev, h.data_ptr(), h.stride(0), f32, weight.contiguous().data_ptr(), ctx.eps,
+              dy.data_ptr(), dy.stride(0), _ptr(ds), 0 if ds is None else ds.stride(0), n, d, d_hidden.data_ptr(),
+              _ptr(d_residual), _ptr(d_weight), _ptr(ws), nbytes)
         d_res = None
         if ctx.has_residual:
-            d_res = d_residual if f32 else d_hidden
+            d_res = d_residual if f32 else d_hidden  # a BF16 residual's gradient is the same tensor
         return d_hidden, d_res, d_weight, None
 
 
@@ -152,7 +175,7 @@ def add_rms_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: f
                                     or (residual is not None and residual.requires_grad)):
         normed, summed = _AddRMSNorm.apply(hidden, residual, weight, float(eps))
         return normed, hidden if summed is None else summed
-    normed, _, summed = _norm_forward(hidden, residual, weight, eps, False)
+    normed, _, summed = _norm_forward(hidden, residual, weight, float(eps), False)
     return normed, summed
 
 
@@ -169,7 +192,7 @@ def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor,
         raise ValueError("the row length must be a multiple of the block size 32")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, residual, weight)):
         raise NotImplementedError("add_rms_norm_mxfp8 implements the forward pass only")
-    return _norm_forward(hidden, residual, weight, eps, True)
+    return _norm_forward(hidden, residual, weight, float(eps), True)
 
 
 # ---------------------------------------------------------------- rotary positions
@@ -213,34 +236,32 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
     return freq.to(device) if device is not None else freq, mult
 
 
-def _token_heads(t: Tensor, name: str) -> tuple[Tensor, Tensor]:
-    """``t`` [..., heads, d] as (the tensor kept alive, a [tokens, heads, d] view with unit inner stride)."""
+def _token_heads(t: Tensor) -> Tensor:
+    """``t`` [..., heads, d] as [tokens, heads, d] with unit inner stride: a view wherever the leading dimensions merge."""
 
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         t = t.contiguous()
-    return t.reshape(-1, t.shape[-2], t.shape[-1])  # a view wherever the leading dimensions merge
+    return t if t.ndim == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
 
 
 def _rotate(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Tensor, interleaved: bool, factor: float,
             inverse: bool) -> tuple[Tensor, Tensor | None]:
     dev = q.device
-    qt = _token_heads(q, "q")
-    kt = None if k is None else _token_heads(k, "k")
-    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    k_out = None if k is None else torch.empty(k.shape, dtype=torch.bfloat16, device=dev)
-    n = qt.shape[0]
-    if n == 0:
-        return q_out, k_out
-    hq = _lib.Heads(qt.data_ptr(), 0, qt.stride(0), qt.stride(1))
-    hk = None if kt is None else _lib.Heads(kt.data_ptr(), 0, kt.stride(0), kt.stride(1))
-    pos = positions.contiguous()
-    freq = frequencies.contiguous()
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.spx_rotary(
-            hq, qt.shape[1], hk, 0 if kt is None else kt.shape[1], n, q.shape[-1], freq.shape[0], pos.data_ptr(),
-            int(pos.dtype == torch.int64), pos.numel(), freq.data_ptr(), factor, int(interleaved), int(inverse),
-            q_out.data_ptr(), _lib.ptr(k_out), _stream(dev)), "spx_rotary")
+    qt = _token_heads(q)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    n, h, d = qt.shape
+    st, sh, _ = qt.stride()
+    hq, hk, kt, k_out, kv = _lib.Heads(qt.data_ptr(), 0, st, sh), None, None, None, 0
+    if k is not None:
+        kt = _token_heads(k)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        kv = kt.shape[1]
+        st, sh, _ = kt.stride()
+        hk = _lib.Heads(kt.data_ptr(), 0, st, sh)
+    if n:
+        pos, freq = positions.contiguous(), frequencies.contiguous()
+        _call("spx_rotary", dev, hq, h, hk, kv, n, d, freq.shape[0], pos.data_ptr(), pos.dtype == torch.int64, pos.numel(),
+              freq.data_ptr(), factor, interleaved, inverse, q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
@@ -318,11 +339,13 @@ def linear_attention_status(device: torch.device | str | int | None = None, clea
 
 
 def _aligned_heads(t: Tensor) -> Tensor:
-    """``t`` [B, T, H, d] with unit inner stride and heads on 16 bytes (a copy only if it must be)."""
+    """``t`` [..., d] (d % 8 == 0) with unit inner stride and rows on 16 bytes (a copy only if it must be)."""
 
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return t
     sizes, strides = t.shape, t.stride()
-    if (t.data_ptr() % 16 or (strides[-1] != 1 and sizes[-1] > 1)
-            or any(st % 8 and n > 1 for st, n in zip(strides[:-1], sizes[:-1]))):
+    if (t.data_ptr() % 16 or strides[-1] != 1
+            or any(n > 1 and (st % 8 or st <= 0) for st, n in zip(strides[:-1], sizes[:-1]))):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -330,9 +353,13 @@ def _aligned_heads(t: Tensor) -> Tensor:
 
 
 def _heads(t: Tensor) -> _lib.Heads:
-    # the stride of a dimension of one element is never used; views may carry any value there
-    b, n, h = (st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape[:3]))
+    b, n, h, _ = t.stride()
     return _lib.Heads(t.data_ptr(), b, n, h)
+
+
+def _step_heads(t: Tensor) -> _lib.Heads:
+    b, h, _ = t.stride()
+    return _lib.Heads(t.data_ptr(), b, 0, h)
 
 
 def _decays(g: Tensor) -> _lib.Decays:
@@ -352,13 +379,10 @@ def _attend(q: Tensor, k: Tensor, v: Tensor, g: Tensor, cu: Tensor | None, state
     last = None
     if want_state:
         last = torch.empty(dims.batch, q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=dev)
-    lib = _lib.load()
-    nbytes = lib.spx_linear_attention_workspace(dims)
+    nbytes = _lib.load().spx_linear_attention_workspace(dims)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        _lib.check(lib.spx_linear_attention(dims, _heads(q), _heads(k), _heads(v), _decays(g), _lib.ptr(cu),
-                                            _lib.ptr(state), out.data_ptr(), _lib.ptr(last), _lib.ptr(ws), nbytes,
-                                            _status_word(dev).data_ptr(), _stream(dev)), "spx_linear_attention")
+    _call("spx_linear_attention", dev, dims, _heads(q), _heads(k), _heads(v), _decays(g), _ptr(cu), _ptr(state),
+          out.data_ptr(), _ptr(last), _ptr(ws), nbytes, _status_word(dev).data_ptr())
     return out, last
 
 
@@ -382,34 +406,32 @@ class _LinearAttention(torch.autograd.Function):
         dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
         dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
         d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
-        lib = _lib.load()
-        nbytes = lib.spx_linear_attention_backward_workspace(dims)
+        nbytes = _lib.load().spx_linear_attention_backward_workspace(dims)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with torch.cuda.device(dev):
-            _lib.check(lib.spx_linear_attention_backward(
-                dims, _heads(q), _heads(k), _heads(v), _decays(g), _lib.ptr(cu), _lib.ptr(state), _heads(d_out),
-                _lib.ptr(d_last), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), _lib.ptr(d_state),
-                _lib.ptr(ws), nbytes, _status_word(dev).data_ptr(), _stream(dev)), "spx_linear_attention_backward")
+        _call("spx_linear_attention_backward", dev, dims, _heads(q), _heads(k), _heads(v), _decays(g), _ptr(cu),
+              _ptr(state), _heads(d_out), _ptr(d_last), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+              _ptr(d_state), _ptr(ws), nbytes, _status_word(dev).data_ptr())
         return dq, dk, dv, dg, d_state, None, None, None
 
 
 def _check_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, scale: float, lead: int, layout: str) -> None:
-    _require(q, "q", torch.bfloat16)
+    _require(q, "q", _BF16)
     dev = q.device
-    for name, t in (("k", k), ("v", v)):
-        _require(t, name, torch.bfloat16, dev)
-    _require(g, "log_decay", (torch.float32, torch.bfloat16), dev)
-    if q.ndim != lead + 2 or k.ndim != lead + 2 or v.ndim != lead + 2 or g.ndim != lead + 1:
+    _require(k, "k", _BF16, dev)
+    _require(v, "v", _BF16, dev)
+    _require(g, "log_decay", _FLOATS, dev)
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != lead + 2 or len(ks) != lead + 2 or len(vs) != lead + 2 or g.ndim != lead + 1:
         raise ValueError(f"q, k, v must be [{layout}, heads, dim] and log_decay [{layout}, heads]")
-    if k.shape[:lead] != q.shape[:lead] or v.shape[:lead] != q.shape[:lead] or g.shape != q.shape[:lead + 1]:
+    if ks[:lead] != qs[:lead] or vs[:lead] != qs[:lead] or g.shape != qs[:-1]:
         raise ValueError("q, k, v and log_decay must share their leading dimensions, log_decay q's heads too")
-    if k.shape[-1] != q.shape[-1] or v.shape[lead] != k.shape[lead]:
+    if ks[-1] != qs[-1] or vs[lead] != ks[lead]:
         raise ValueError("k must have q's head dimension and v the heads of k")
-    if k.shape[lead] < 1 or q.shape[lead] % k.shape[lead] or q.shape[lead] < 1:
+    if ks[lead] < 1 or qs[lead] % ks[lead] or qs[lead] < 1:
         raise ValueError("the query heads must be a multiple of the key/value heads")
-    for name, n in (("key", q.shape[-1]), ("value", v.shape[-1])):
-        if n < 8 or n % 8 or n > _MAX_HEAD_DIM:
-            raise ValueError(f"the {name} dimension of a head must be a multiple of 8 up to {_MAX_HEAD_DIM}")
+    dk, dv = qs[-1], vs[-1]
+    if not (8 <= dk <= _MAX_HEAD_DIM and 8 <= dv <= _MAX_HEAD_DIM) or dk % 8 or dv % 8:
+        raise ValueError(f"the key and value dimensions of a head must be multiples of 8 up to {_MAX_HEAD_DIM}")
     if not (math.isfinite(scale) and scale != 0):
         raise ValueError("scale must be finite and not zero")
 
@@ -486,16 +508,14 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if slots.shape != (B,):
             raise ValueError(f"slots must be [{B}]")
         slots = slots.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad):
         raise NotImplementedError("linear_attention_step implements the forward pass only")
-    q, k, v = (_aligned_heads(t[:, None]) for t in (q, k, v))
-    out = torch.empty(B, H, dv, dtype=torch.bfloat16, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.spx_linear_attention_step(
-            _heads(q), _heads(k), _heads(v), _lib.Decays(log_decay.data_ptr(), log_decay.stride(0), 0, log_decay.stride(1)),
-            int(log_decay.dtype == torch.float32), B, H, k.shape[2], dk, dv, scale, state.data_ptr(), state.shape[0],
-            _lib.ptr(slots), out.data_ptr(), _stream(dev)), "spx_linear_attention_step")
+    q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
+    out = q.new_empty((B, H, dv))
+    _call("spx_linear_attention_step", dev, _step_heads(q), _step_heads(k), _step_heads(v),
+          _lib.Decays(log_decay.data_ptr(), log_decay.stride(0), 0, log_decay.stride(1)), log_decay.dtype == _F32, B, H,
+          k.shape[1], dk, dv, scale, state.data_ptr(), state.shape[0], _ptr(slots), out.data_ptr())
     return out
 
 
