@@ -224,6 +224,18 @@ size_t spx_mxfp8_mm_workspace(int64_t m, int64_t n, int64_t k);
 int spx_mxfp8_mm_nt(const uint16_t* left, const uint16_t* right_rows, int64_t m, int64_t n, int64_t k,
                     uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same product with both operands quantised beforehand, as a server keeps
+ * its weights: spx_mxfp8_pack_rows once for right_rows [n, k] (sizes in bytes
+ * from spx_mxfp8_packed_sizes), then spx_mxfp8_mm_rows for left rows in the
+ * layout of spx_mxfp8_quantize_rows or spx_add_rmsnorm_rows (E4M3 [m, k],
+ * E8M0 [m, k / 32]).  k % 128 == 0.  status: device int, zero before the
+ * first call (NULL = kernel errors are not recorded). */
+int spx_mxfp8_packed_sizes(int64_t n, int64_t k, size_t* value_bytes, size_t* scale_bytes);
+int spx_mxfp8_pack_rows(const uint16_t* rows, int64_t n, int64_t k, uint8_t* values, uint8_t* scales, void* stream);
+int spx_mxfp8_mm_rows(const uint8_t* left_values, const uint8_t* left_scales, const uint8_t* right_values,
+                      const uint8_t* right_scales, int64_t m, int64_t n, int64_t k, uint16_t* out, int* status,
+                      void* stream);
+
 /* Scores, top-k ids and routing weights from given BF16 router logits [T, E]. */
 int spx_route(const spx_layer_dims* dims, const uint16_t* logits, const uint16_t* softplus_table,
               const uint8_t* resident_mask, uint16_t* router_scores, int64_t* expert_ids,
@@ -540,9 +552,10 @@ int spx_layer_backward(const spx_layer_dims* dims, const spx_packed_weights* wei
  *
  * spx_add_rmsnorm_rows: h = hidden + residual, stored in the residual's type
  *   (residual_f32: FP32, else BF16), and RMSNorm of h as stored, rounded once:
- *   y = h * w / sqrt(mean(h^2) + eps).  Either `normed` (BF16 [rows, d]) or
- *   mx_values / mx_scales (E4M3 [rows, d] and E8M0 [rows, d / 32], the layout
- *   of spx_mxfp8_quantize_rows, quantised from the FP32 result; d % 32 == 0).
+ *   y = h * w / sqrt(mean(h^2) + eps).  `normed` (BF16 [rows, d]), mx_values
+ *   with mx_scales (E4M3 [rows, d] and E8M0 [rows, d / 32], the layout of
+ *   spx_mxfp8_quantize_rows, quantised from the FP32 result; d % 32 == 0), or
+ *   both.
  *   residual NULL: h = hidden, `sum` unused.  Row strides in elements; `sum`
  *   may be the residual itself when its rows are contiguous.  d % 8 == 0,
  *   d <= 16384; 16-byte aligned rows.

@@ -22,6 +22,7 @@ from spalmer_b200.experts import (
     rms_norm,
     route,
 )
+from spalmer_b200.token_mixer import B200DecoderLayer, LinearAttentionMixer
 from spalmer_b200.token_ops import (
     add_rms_norm,
     add_rms_norm_mxfp8,
@@ -34,10 +35,12 @@ from spalmer_b200.token_ops import (
 
 __all__ = [
     "B200ChannelBlock",
+    "B200DecoderLayer",
     "B200MicroExpertChannelMixer",
     "ChannelMixerOutput",
     "ExpertPotentiationController",
     "ExpertResidency",
+    "LinearAttentionMixer",
     "MicroExpertBank",
     "MicroExpertChannelMixer",
     "MicroExpertsConfig",

@@ -85,6 +85,9 @@ EXPORTED = (
     "spx_linear_attention_backward_workspace",
     "spx_linear_attention_backward",
     "spx_linear_attention_step",
+    "spx_mxfp8_packed_sizes",
+    "spx_mxfp8_pack_rows",
+    "spx_mxfp8_mm_rows",
 )
 
 ABI_VERSION = 12
@@ -347,6 +350,15 @@ def load() -> ctypes.CDLL:
         "spx_nvfp4_mm_nt": (
             ctypes.c_int,
             [_vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp],
+        ),
+        "spx_mxfp8_packed_sizes": (
+            ctypes.c_int,
+            [ctypes.c_int64, ctypes.c_int64, P(ctypes.c_size_t), P(ctypes.c_size_t)],
+        ),
+        "spx_mxfp8_pack_rows": (ctypes.c_int, [_vp, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp]),
+        "spx_mxfp8_mm_rows": (
+            ctypes.c_int,
+            [_vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp],
         ),
         "spx_add_rmsnorm_rows": (
             ctypes.c_int,

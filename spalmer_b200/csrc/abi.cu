@@ -1026,6 +1026,56 @@ int spx_mxfp8_mm_nt(const uint16_t* left, const uint16_t* right_rows, int64_t m,
   return launch_gemm(kEpiStore, g, ceil_div(m, kTileRows), ceil_div(n, L.bn), st, true);
 }
 
+// The packed form of `right_rows` that spx_mxfp8_mm_nt makes for itself at
+// every call, and the product of it with rows that are quantised already.
+int spx_mxfp8_packed_sizes(int64_t n, int64_t k, size_t* value_bytes, size_t* scale_bytes) {
+  if (n <= 0 || k <= 0 || value_bytes == nullptr || scale_bytes == nullptr) return SPX_ERR_INVALID_ARG;
+  if (k % 128 != 0 || n > (int64_t(1) << 31) - 1 || k > (int64_t(1) << 30)) return SPX_ERR_UNSUPPORTED;
+  const MmLayout L = mm_layout(1, n, k);
+  *value_bytes = static_cast<size_t>(n) * k;
+  *scale_bytes = mx_atoms_bytes(1, static_cast<int>(n), static_cast<int>(k), L.bn);
+  return SPX_OK;
+}
+
+int spx_mxfp8_pack_rows(const uint16_t* rows, int64_t n, int64_t k, uint8_t* values, uint8_t* scales, void* stream) {
+  size_t vb = 0, sb = 0;
+  if (int rc = spx_mxfp8_packed_sizes(n, k, &vb, &sb); rc != SPX_OK) return rc;
+  if (rows == nullptr || values == nullptr || scales == nullptr) return SPX_ERR_INVALID_ARG;
+  if (!aligned16(rows) || !aligned16(values) || !aligned16(scales)) return SPX_ERR_ALIGNMENT;
+  return launch_mx_quantize_b(kMxSrcRows, rows, nullptr, 1, static_cast<int>(n), static_cast<int>(n),
+                              static_cast<int>(k), static_cast<int>(k), mm_layout(1, n, k).bn, 0, 0, 0, k, values,
+                              scales, static_cast<cudaStream_t>(stream));
+}
+
+int spx_mxfp8_mm_rows(const uint8_t* left_values, const uint8_t* left_scales, const uint8_t* right_values,
+                      const uint8_t* right_scales, int64_t m, int64_t n, int64_t k, uint16_t* out, int* status,
+                      void* stream) {
+  size_t vb = 0, sb = 0;
+  if (int rc = spx_mxfp8_packed_sizes(n, k, &vb, &sb); rc != SPX_OK) return rc;
+  if (m < 0) return SPX_ERR_INVALID_ARG;
+  if (m > (int64_t(1) << 31) - 1) return SPX_ERR_UNSUPPORTED;
+  if (m == 0) return SPX_OK;
+  if (left_values == nullptr || left_scales == nullptr || right_values == nullptr || right_scales == nullptr ||
+      out == nullptr)
+    return SPX_ERR_INVALID_ARG;
+  if (!aligned16(left_values) || !aligned16(right_values) || !aligned16(right_scales) || !aligned16(out) ||
+      (reinterpret_cast<uintptr_t>(left_scales) & 3u) != 0)
+    return SPX_ERR_ALIGNMENT;
+  const int bn = mm_layout(1, n, k).bn, kp = static_cast<int>(k);
+  GemmArgs g = base_args(kEpiStore, bn, kp / 128, status, true);
+  int rc = SPX_OK;
+  if ((rc = encode_2d(&g.tma_a, left_values, m, kp, kp, kTileRows, 1)) != SPX_OK) return rc;
+  if ((rc = encode_3d(&g.tma_b, right_values, 1, n, kp, bn, 1)) != SPX_OK) return rc;
+  g.m_rows = static_cast<int>(m);
+  g.n_valid = static_cast<int>(n);
+  g.out = out;
+  g.ldo = n;
+  g.sfa = left_scales;
+  g.ld_sfa = kp / kMxBlock;
+  g.sfb = right_scales;
+  return launch_gemm(kEpiStore, g, ceil_div(m, kTileRows), ceil_div(n, bn), static_cast<cudaStream_t>(stream), true);
+}
+
 namespace {
 struct NvMmLayout {
   int64_t kp;

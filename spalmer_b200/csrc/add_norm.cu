@@ -199,9 +199,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
       unpack8(wv[i], wf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = h[i][j] * r * wf[j];
-      if (a.mx_values == nullptr) {
-        if (in) store8(a.y, row * a.d + c * 8, false, y);
-      } else {
+      if (a.y != nullptr && in) store8(a.y, row * a.d + c * 8, false, y);
+      if (a.mx_values != nullptr) {
         // blocks of 32 = four lanes; all lanes take part in the shuffles (d % 32 == 0, so a block is wholly in or out)
         float amax = 0.0f;
 #pragma unroll

@@ -481,9 +481,9 @@ struct AddNormArgs {
   const void* res;        // [rows, d] BF16 / FP32, row stride ld_res | null
   const uint16_t* w;      // [d]
   void* sum;              // [rows, d] in res's type (null without res)
-  uint16_t* y;            // [rows, d] BF16, or
-  uint8_t* mx_values;     // [rows, d] E4M3 and
-  uint8_t* mx_scales;     // [rows, d / 32] E8M0
+  uint16_t* y;            // [rows, d] BF16 | null
+  uint8_t* mx_values;     // [rows, d] E4M3 | null
+  uint8_t* mx_scales;     // [rows, d / 32] E8M0 (with mx_values)
   int64_t rows, ld_x, ld_res;
   int d;
   int res_f32;

@@ -143,7 +143,7 @@ int spx_add_rmsnorm_rows(const uint16_t* hidden, int64_t ld_hidden, const void* 
   if (rows < 0 || d <= 0 || !(eps > 0.0f)) return SPX_ERR_INVALID_ARG;
   if (d % 8 != 0 || d > kNormMaxD) return SPX_ERR_UNSUPPORTED;
   const bool mx = mx_values != nullptr || mx_scales != nullptr;
-  if (mx && (normed != nullptr || mx_values == nullptr || mx_scales == nullptr)) return SPX_ERR_INVALID_ARG;
+  if (mx && (mx_values == nullptr || mx_scales == nullptr)) return SPX_ERR_INVALID_ARG;
   if (mx && d % kMxBlock != 0) return SPX_ERR_UNSUPPORTED;
   if (rows == 0) return SPX_OK;
   if (hidden == nullptr || norm_weight == nullptr || (!mx && normed == nullptr)) return SPX_ERR_INVALID_ARG;

@@ -5,6 +5,8 @@
   (precision.py:68-107).  Claims are verified by running one small layer on the
   device.  The BF16 pair trains (``spx_layer_backward``); the MXFP8 and NVFP4
   pairs are forward-only, so their ``backward_available`` is False.
+* ``mxfp8_pack_rows`` / ``mxfp8_mm_rows``: the MXFP8 GEMM on operands that are
+  quantised already (a weight packed once, rows from ``add_rms_norm_mxfp8``).
 * ``mx_quantize_rows`` / ``mxfp8_mm_nt`` / ``native_mxfp8_linear``,
   ``nvfp4_quantize_rows`` / ``nvfp4_mm_nt`` / ``native_nvfp4_linear`` and
   ``native_expert_matmul``: forward-only equivalents of ``_mx_quantize_rows``,
@@ -84,6 +86,51 @@ def mxfp8_mm_nt(left: Tensor, right_rows: Tensor) -> Tensor:
     stream = torch.cuda.current_stream(left.device).cuda_stream
     _lib.check(lib.spx_mxfp8_mm_nt(a.data_ptr(), b.data_ptr(), m, n, k, out.data_ptr(), ws.data_ptr(), nbytes,
                                    stream), "spx_mxfp8_mm_nt")
+    return out
+
+
+def mxfp8_pack_rows(rows: Tensor) -> tuple[Tensor, Tensor, tuple[int, int]]:
+    """A weight ``[n, k]`` packed once as the right operand of ``mxfp8_mm_rows``
+    (k a multiple of 128): E4M3 values, scale atoms and the shape."""
+
+    if rows.ndim != 2 or rows.dtype != torch.bfloat16 or not rows.is_cuda:
+        raise ValueError("mxfp8_pack_rows expects a [n, k] bfloat16 CUDA tensor")
+    n, k = rows.shape
+    if n < 1 or k < 1 or k % 128:
+        raise ValueError("mxfp8_pack_rows needs n >= 1 and k a multiple of 128")
+    lib = _lib.load()
+    sizes = _lib.ctypes.c_size_t(), _lib.ctypes.c_size_t()
+    _lib.check(lib.spx_mxfp8_packed_sizes(n, k, *sizes), "spx_mxfp8_packed_sizes")
+    values, scales = (torch.empty(v.value, dtype=torch.uint8, device=rows.device) for v in sizes)
+    src = rows.detach().contiguous()
+    with torch.cuda.device(rows.device):
+        stream = torch.cuda.current_stream(rows.device).cuda_stream
+        _lib.check(lib.spx_mxfp8_pack_rows(src.data_ptr(), n, k, values.data_ptr(), scales.data_ptr(), stream),
+                   "spx_mxfp8_pack_rows")
+    return values, scales, (n, k)
+
+
+def mxfp8_mm_rows(values: Tensor, scales: Tensor, packed: tuple[Tensor, Tensor, tuple[int, int]]) -> Tensor:
+    """``deq(values, scales) @ weight.T`` in BF16 for rows that are MXFP8 already
+    (``mx_quantize_rows``, ``add_rms_norm_mxfp8``: E4M3 bytes [..., k] and E8M0
+    bytes [..., k / 32]) and a weight from ``mxfp8_pack_rows``.  The same product,
+    bit for bit, as ``mxfp8_mm_nt`` of the rows the values were quantised from."""
+
+    weight, atoms, (n, k) = packed
+    if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or not values.is_cuda or values.ndim < 1:
+        raise ValueError("mxfp8_mm_rows expects uint8 CUDA values and scales")
+    if values.shape[-1] != k or scales.shape != (*values.shape[:-1], k // 32):
+        raise ValueError(f"values must be [..., {k}] and scales [..., {k // 32}]")
+    if scales.device != values.device or weight.device != values.device:
+        raise NativeExpertPrecisionError("native MXFP8 GEMM operands must share one device")
+    v, s = values.contiguous(), scales.contiguous()
+    m = v.numel() // k
+    out = torch.empty(*values.shape[:-1], n, dtype=torch.bfloat16, device=values.device)
+    lib = _lib.load()
+    with torch.cuda.device(values.device):
+        stream = torch.cuda.current_stream(values.device).cuda_stream
+        _lib.check(lib.spx_mxfp8_mm_rows(v.data_ptr(), s.data_ptr(), weight.data_ptr(), atoms.data_ptr(), m, n, k,
+                                         out.data_ptr(), None, stream), "spx_mxfp8_mm_rows")
     return out
 
 

@@ -93,35 +93,33 @@ def _check_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: fl
     return d
 
 
-def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float,
-                  mxfp8: bool) -> tuple[Tensor, Tensor | None, Tensor]:
-    """(normed, None, sum) or (values, scales, sum); sum is hidden itself without a residual."""
+def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float, rows: bool,
+                  mxfp8: bool) -> tuple[Tensor | None, Tensor | None, Tensor | None, Tensor]:
+    """(BF16 rows, MXFP8 values, their scales, sum); sum is hidden itself without a residual."""
 
     d = hidden.shape[-1]
     x = _rows(hidden, d, 2)
     n, dev = x.shape[0], x.device
-    r, f32, total, scales = None, False, hidden, None
+    r, f32, total, out, values, scales = None, False, hidden, None, None, None
     if residual is not None:
         f32 = residual.dtype == _F32
         r = _rows(residual, d, 4 if f32 else 2)
         total = torch.empty_like(residual, memory_format=torch.contiguous_format)
     w = weight.contiguous()
-    if mxfp8:
-        out = hidden.new_empty(hidden.shape, dtype=torch.uint8)
-        scales = hidden.new_empty((*hidden.shape[:-1], d // 32), dtype=torch.uint8)
-    else:
+    if rows:
         out = torch.empty_like(hidden, memory_format=torch.contiguous_format)
-    ptr = out.data_ptr()
+    if mxfp8:
+        values = hidden.new_empty(hidden.shape, dtype=torch.uint8)
+        scales = hidden.new_empty((*hidden.shape[:-1], d // 32), dtype=torch.uint8)
     _call("spx_add_rmsnorm_rows", dev, x.data_ptr(), x.stride(0), _ptr(r), 0 if r is None else r.stride(0), f32,
-          w.data_ptr(), eps, n, d, None if r is None else total.data_ptr(), None if mxfp8 else ptr,
-          ptr if mxfp8 else None, _ptr(scales))
-    return out, scales, total
+          w.data_ptr(), eps, n, d, None if r is None else total.data_ptr(), _ptr(out), _ptr(values), _ptr(scales))
+    return out, values, scales, total
 
 
 class _AddRMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, residual, weight, eps):
-        out, _, total = _norm_forward(hidden, residual, weight, eps, False)
+        out, _, _, total = _norm_forward(hidden, residual, weight, eps, True, False)
         ctx.set_materialize_grads(False)
         ctx.eps = eps
         ctx.has_residual = residual is not None
@@ -175,13 +173,13 @@ def add_rms_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: f
                                     or (residual is not None and residual.requires_grad)):
         normed, summed = _AddRMSNorm.apply(hidden, residual, weight, float(eps))
         return normed, hidden if summed is None else summed
-    normed, _, summed = _norm_forward(hidden, residual, weight, float(eps), False)
+    normed, _, _, summed = _norm_forward(hidden, residual, weight, float(eps), True, False)
     return normed, summed
 
 
-def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor,
-                       eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor]:
-    """``(values, scales, summed)``: ``add_rms_norm`` with MXFP8 rows out, quantised
+def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: float = 1e-6, *,
+                       rows: bool = False) -> tuple[Tensor, ...]:
+    """``(values, scales, summed)`` (with ``rows`` the BF16 rows as a fourth): ``add_rms_norm`` with MXFP8 rows out, quantised
     from the FP32 result: E4M3 bytes [..., d] and one E8M0 byte per 32 elements
     [..., d / 32] (uint8), the layout of ``native.mx_quantize_rows`` and the left
     operand of ``native.mxfp8_mm_rows``.  d a multiple of 32.  Forward only.
@@ -192,7 +190,8 @@ def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor,
         raise ValueError("the row length must be a multiple of the block size 32")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, residual, weight)):
         raise NotImplementedError("add_rms_norm_mxfp8 implements the forward pass only")
-    return _norm_forward(hidden, residual, weight, float(eps), True)
+    normed, values, scales, summed = _norm_forward(hidden, residual, weight, float(eps), rows, True)
+    return (values, scales, summed, normed) if rows else (values, scales, summed)
 
 
 # ---------------------------------------------------------------- rotary positions
