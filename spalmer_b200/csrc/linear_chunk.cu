@@ -24,11 +24,12 @@
 //     pass, whose output is rounded to BF16 as coarsely, two in the gradients,
 //     because d decay is a long sum of q . dq - k . dk that cancels.
 //
-// Decay factors are exponentials of differences <= 0, never quotients, so no
-// decay overflows: inside a 32-token block e^{G_i - G_j} directly, across
-// blocks e^{G_i - G_end} * e^{G_end - G_j} with the end of j's block between
-// them.  Sums run from the block's start, so a token that forgets everything
-// (clamped to 2^-150, which is zero in FP32) costs its neighbours no digits.
+// Decay factors are exponentials of sums <= 0, never quotients, so no decay
+// overflows: inside a 32-token block the sum between two tokens, across blocks a
+// factor up to the block's edge and one from there.  A token's log2 decay is
+// clamped to -150, which is zero in FP32; sums start at block edges, and those that
+// stay small are not differences of large ones, so that a token that forgets
+// everything costs its neighbours no digits.
 //
 // When (job, sequence, head, slice) fill too few SMs, the sequence is cut into
 // segments: a pass over b and c alone gives each segment's state from zero, a
@@ -74,9 +75,13 @@ struct alignas(64) LaChunkArgs {
   float* seg_decay;      // [lane][nseg]
 };
 
+// Decays of a chunk, each sum taken directly (a small one as the difference of
+// large ones would lose its digits): log2 decays from the token's 32-token block's
+// start up to it (reverse: from it to the block's end), the factor over the rest of
+// the block, and the blocks' totals.
 struct DecayTable {
-  float lg[kC];  // log2 decay from the start of the token's 32-token block, inclusive
-  float cf[kC];  // from the token to its block's end (forward) / from the block's start to it (reverse)
+  float a[kC];
+  float cf[kC];
   float total[4];
 };
 
@@ -86,14 +91,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Decay from the chunk's start to a token (inclusive), and from it to the chunk's end.
-__device__ __forceinline__ float from_start(const DecayTable& t, int quad, int row) {
-  const float x = quad == 0 ? 0.0f : quad == 1 ? t.total[0] : quad == 2 ? t.total[0] + t.total[1] : t.total[0] + t.total[1] + t.total[2];
-  return ex2(x + t.lg[row]);
+// The other blocks of the chunk on the token's far side: those before its own (reverse: after it), or the others.
+__device__ __forceinline__ float blocks(const DecayTable& t, int quad, bool before) {
+  float x = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x += (before ? q < quad : q > quad) ? t.total[q] : 0.0f;
+  return x;
 }
-__device__ __forceinline__ float to_end(const DecayTable& t, int quad, int row) {
-  const float x = quad == 3 ? 0.0f : quad == 2 ? t.total[3] : quad == 1 ? t.total[3] + t.total[2] : t.total[3] + t.total[2] + t.total[1];
-  return ex2((t.total[quad] - t.lg[row]) + x);
+// Between the state at the chunk's near end and the token (on a . S), and between the token and the far end (on c).
+__device__ __forceinline__ float into_token(const DecayTable& t, int quad, int row, bool rev) {
+  return ex2(t.a[row] + blocks(t, quad, !rev));
+}
+__device__ __forceinline__ float out_of_token(const DecayTable& t, int quad, int row, bool rev) {
+  return t.cf[row] * ex2(blocks(t, quad, rev));
 }
 
 template <int DKB, bool PRECISE, int PARTS>
@@ -407,7 +417,6 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       Item w;
       item_of(args, idx, &w);
       const bool rev = args.la.job[w.job].reverse != 0;
-      const float sign = rev ? 1.0f : -1.0f;
       // of this row's words in the diagonal block: a masked entry is zero whatever it holds
       uint32_t mask[8];
 #pragma unroll
@@ -419,7 +428,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const uint32_t b = it & 1u, ph = (it >> 1) & 1u;
         const DecayTable& t = tables[b];
         if (!(ok = warp_wait(&bar.gfull[b], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const float lg = t.lg[row];
+        const float a = t.a[row];
         if (!(ok = warp_wait(&bar.pacc[b], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         // The operand takes the accumulator's place: 16 FP32 columns become 8 of BF16
@@ -429,7 +438,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const float own = t.total[quad];
         // inside the diagonal block the two factors are on either side of 1; a block
         // that decays by more than 2^100 takes the exponential of each difference
-        float run = rev ? -lg : lg - own;
+        float run = a - own;
         const bool steep = !(own >= -100.0f);
 #pragma unroll 1
         for (int n = 0; n < 4; ++n) {
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             }
             if (n == 0 && steep) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) f[q] = pair(ex2((t.lg[c0 + 2 * q] - lg) * sign), ex2((t.lg[c0 + 2 * q + 1] - lg) * sign));
+              for (int q = 0; q < 8; ++q) f[q] = pair(ex2(a - t.a[c0 + 2 * q]), ex2(a - t.a[c0 + 2 * q + 1]));
             }
             tmem_wait_ld();
 #pragma unroll
@@ -514,7 +523,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           if (full_pass) warp_arrive(&bar.tail[tails++ & 1u], lane);  // else the product alone reads them, after vp
         }
         if (!(ok = warp_wait(&bar.gfull[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const float wgt = rev ? from_start(tables[b], quad, row) : to_end(tables[b], quad, row);
+        const float wgt = out_of_token(tables[b], quad, row, rev);
         warp_arrive(&bar.gfree[b], lane);
         const uint64_t wgt2 = pair(wgt, wgt);
         // the parts' last reader: the state product of the chunk before (or the one before that)
@@ -664,7 +673,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       auto read_factor = [&](uint32_t n) {
         const uint32_t b = n & 1u;
         if (!warp_wait(&bar.gfull[b], (n >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE)) return false;
-        factor = rev ? to_end(tables[b], quad, row) : from_start(tables[b], quad, row);
+        factor = into_token(tables[b], quad, row, rev);
         warp_arrive(&bar.gfree[b], lane);
         return true;
       };
@@ -994,29 +1003,31 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       if (w.n > 0) fetch(0);
       for (int p = 0; p < w.n; ++p, ++it) {
         const uint32_t b = it & 1u;
-        float lg[4];
+        float up[4], down[4];  // sums up to the lane's token, and after it
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float x = __uint_as_float(f32 ? next[q] : next[q] << 16) * 1.44269504088896340736f;  // log2 e
-          lg[q] = x < -150.0f ? -150.0f : x;                  // a NaN stays
+          up[q] = x < -150.0f ? -150.0f : x;                                                         // a NaN stays
+          const float after = __shfl_down_sync(0xFFFFFFFFu, up[q], 1);
+          down[q] = lane == 31 ? 0.0f : after;
         }
         if (p + 1 < w.n) fetch(p + 1);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float u = __shfl_up_sync(0xFFFFFFFFu, lg[q], off);
-            if (lane >= off) lg[q] += u;
+            const float u = __shfl_up_sync(0xFFFFFFFFu, up[q], off), v = __shfl_down_sync(0xFFFFFFFFu, down[q], off);
+            if (lane >= off) up[q] += u;
+            if (lane < 32 - off) down[q] += v;
           }
         }
         if (!(ok = warp_wait(&bar.gfree[b], ((it >> 1) & 1u) ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
         DecayTable& t = tables[b];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float total = __shfl_sync(0xFFFFFFFFu, lg[q], 31);
-          t.lg[32 * q + lane] = lg[q];
-          t.cf[32 * q + lane] = ex2(rev ? lg[q] : total - lg[q]);
-          if (lane == q) t.total[q] = total;
+          t.a[32 * q + lane] = rev ? down[q] : up[q];
+          t.cf[32 * q + lane] = ex2(rev ? up[q] : down[q]);
+          if (lane == 31) t.total[q] = up[q];
         }
         warp_arrive(&bar.gfull[b], lane);
       }
