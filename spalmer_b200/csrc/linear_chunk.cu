@@ -62,7 +62,8 @@ constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
 // Registers of the warpgroups' threads: the launch gives each 64 (1024 x 64 = 65,536).
 constexpr int kRegsAB = 64, kRegsC = 48, kRegsState = 120, kRegsOut = 64, kRegsRest = 40;
 static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + 2 * kRegsOut + kRegsRest <= 8 * 64, "registers of a CTA");
-constexpr uint32_t kBarBytes = 336;
+constexpr int kOrderMax = 4096;  // more sequences are taken as they come
+constexpr uint32_t kBarBytes = 416;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
 
 struct alignas(64) LaChunkArgs {
@@ -71,6 +72,8 @@ struct alignas(64) LaChunkArgs {
   int lanes[4];          // first lane of each job; lanes[njobs] = all of them
   int slices[3];
   int nseg, state_only, run_segs;
+  const int* order;      // packed: the sequences, longest first | null
+  int* queue;            // with order: the next item to take
   float* seg_state;      // [lane][nseg][128][64]
   float* seg_decay;      // [lane][nseg]
 };
@@ -126,8 +129,9 @@ static_assert(Cfg<2, false, 3>::kBytes <= 232448 && Cfg<2, true, 2>::kBytes <= 2
 
 struct Item {
   int job, seq, h, slice, seg, lane;
-  int64_t start, len;  // tokens of the sequence in the flattened order
-  int nch, p0, n;      // chunks of the sequence; this item's: p0 .. p0 + n in processing order
+  int start, len;   // tokens of the sequence in the flattened order
+  int n;            // this item's chunks
+  int first, step;  // first token of the first of them in the sequence, and to the next one's
 };
 
 __device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
@@ -142,20 +146,24 @@ __device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it)
   r /= a.slices[j];
   it->h = r % a.la.H;
   it->seq = r / a.la.H;
+  if (a.order != nullptr) it->seq = __ldg(a.order + it->seq);
   bool ok = true;
   if (a.la.cu == nullptr) {
-    it->start = it->seq * a.la.T;
-    it->len = a.la.T;
+    it->start = static_cast<int>(it->seq * a.la.T);
+    it->len = static_cast<int>(a.la.T);
   } else {
-    const int64_t lo = __ldg(a.la.cu + it->seq), hi = __ldg(a.la.cu + it->seq + 1);
+    const int lo = __ldg(a.la.cu + it->seq), hi = __ldg(a.la.cu + it->seq + 1);
     ok = lo >= 0 && hi >= lo && hi <= a.la.total;
     it->start = ok ? lo : 0;
     it->len = ok ? hi - lo : 0;
   }
-  it->nch = static_cast<int>((it->len + kC - 1) / kC);
-  const int per = (it->nch + a.nseg - 1) / a.nseg;
-  it->p0 = min(it->seg * per, it->nch);
-  it->n = min(per, it->nch - it->p0);
+  const int nch = (it->len + kC - 1) / kC;
+  const int per = (nch + a.nseg - 1) / a.nseg;
+  const int p0 = min(it->seg * per, nch);
+  it->n = min(per, nch - p0);
+  const bool rev = a.la.job[j].reverse != 0;
+  it->first = (rev ? nch - 1 - p0 : p0) * kC;
+  it->step = rev ? -kC : kC;
   return ok;
 }
 
@@ -335,6 +343,8 @@ struct Bars {
   uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
   uint64_t vp[2], kv[2], kvfree[2];  // by the chunk's parity
   uint64_t sop, qs, o, ofree, drained;
+  uint64_t qfull[4], qfree[4];  // of the items taken from the queue
+  int taken[4];
   uint32_t tmem;
   int failed;
 };
@@ -387,6 +397,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       mbar_init(&bar.kv[s], 1);
       mbar_init(&bar.kvfree[s], 4);
     }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&bar.qfull[s], 1);
+      mbar_init(&bar.qfree[s], full_pass ? 31 : 15);  // every warp that takes items but the one that fetches them
+    }
     mbar_init(&bar.sop, 4);
     mbar_init(&bar.qs, 1);
     mbar_init(&bar.o, 1);
@@ -408,15 +422,35 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   const int row = quad * 32 + lane;  // this thread's TMEM lane / tile row
   bool ok = true;
   uint32_t it = 0;  // chunks so far, the same count in every role
+  uint32_t st = 0, ph = 0;  // it % kStages, and the parity of it / kStages
+  auto advance = [&]() {
+    ++it;
+    if (++st == K::kStages) {
+      st = 0;
+      ph ^= 1u;
+    }
+  };
+  // Items: a fixed stride, or for packed sequences (longest first) a queue that all
+  // CTAs take from; the warp of c's TMA fetches one ahead and hands it to the others.
+  uint32_t nitem = 0;  // taken so far, the CTA's first item (its index) apart
+  auto next_item = [&](int idx) {
+    if (args.order == nullptr) return idx + static_cast<int>(gridDim.x);
+    const uint32_t slot = nitem & 3u;
+    if (!(ok = warp_wait(&bar.qfull[slot], (nitem >> 2) & 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) return items;
+    const int got = *const_cast<volatile int*>(&bar.taken[slot]);
+    warp_arrive(&bar.qfree[slot], lane);
+    ++nitem;
+    return got;
+  };
 
   if (warp < 8) {
     static_assert(kRegsAB == 64, "the launch's own");
     // ---------------- the decayed a . b matrix: 16 columns of each 32-token block
     const int half = warp >> 2;
-    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
+    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
       Item w;
       item_of(args, idx, &w);
-      const bool rev = args.la.job[w.job].reverse != 0;
+      const bool rev = w.step < 0;
       // of this row's words in the diagonal block: a masked entry is zero whatever it holds
       uint32_t mask[8];
 #pragma unroll
@@ -498,21 +532,20 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- scaled c
     uint32_t tails = 0;
-    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
       Item w;
       item_of(args, idx, &w);
-      const bool rev = args.la.job[w.job].reverse != 0;
-      for (int p = 0; p < w.n; ++p, ++it) {
+      const bool rev = w.step < 0;
+      int left = w.len - w.first;  // tokens from the chunk's first one on
+      for (int p = 0; p < w.n; ++p, advance(), left -= w.step) {
         const uint32_t b = it & 1u;
-        const int st = static_cast<int>(it % K::kStages);
-        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-        const int len = static_cast<int>(w.len - static_cast<int64_t>(chunk) * kC);
-        if (!(ok = warp_wait(&bar.full_c[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+        const int len = left;
+        if (!(ok = warp_wait(&bar.full_c[st], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
         const uint32_t stage = base + st * K::kStage;
         const uint32_t sc_row = stage + 2 * DKB * kTile + swz(row, 0);  // ^ (c << 4): the row's chunk c
         if (len < kC && args.la.cu != nullptr) {
           // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
-          if (!(ok = warp_wait(&bar.full_ab[st], (it / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
+          if (!(ok = warp_wait(&bar.full_ab[st], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
           if (row >= len) {
 #pragma unroll
             for (int x = 0; x < DKB + 1; ++x)
@@ -550,7 +583,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     regs_up<kRegsState>();
     // ---------------- the state: one row of da, 64 columns, in registers
     const bool rows_in = quad < 2 * DKB;
-    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
       Item w;
       const bool sound = item_of(args, idx, &w);
       const LaJob& j = args.la.job[w.job];
@@ -652,11 +685,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     static_assert(kRegsOut == 64, "the launch's own");
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- epilogue: 32 columns of one token a thread
-    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx += gridDim.x) {
+    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
       Item w;
       item_of(args, idx, &w);
       const LaJob& j = args.la.job[w.job];
-      const bool rev = j.reverse != 0, f32 = PRECISE && j.out_f32 != 0;
+      const bool rev = w.step < 0, f32 = PRECISE && j.out_f32 != 0;
       const int col0 = w.slice * 64;
       const int valid = min(64, j.dc - col0);  // a multiple of 8
       const bool packed = args.la.cu != nullptr;
@@ -678,13 +711,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         return true;
       };
       if (w.n > 0) ok = read_factor(it);
-      for (int p = 0; ok && p < w.n; ++p, ++it) {
-        const int64_t first = static_cast<int64_t>(rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p) * kC;  // in the sequence
-        const int left = static_cast<int>(min(w.len - first, static_cast<int64_t>(kC)));            // tokens of the chunk
+      int first = w.first;  // the chunk's first token
+      int64_t at = (static_cast<int64_t>(w.start) + first + r0) * stride + w.h * j.dc + col0;
+      for (int p = 0; ok && p < w.n; ++p, advance(), first += w.step, at += w.step * stride) {
+        const int left = w.len - first;  // tokens from there on
         // Rows go through shared memory on their way to and from global memory (four
         // lanes this warp's 64 bytes of a row): a thread's own row would touch 32 lines an
         // instruction and hold up every barrier and shared-memory access of the CTA.
-        const int st = static_cast<int>(it % K::kStages);
         const uint32_t tile = base + (K::kOwnOut ? K::kOffOut : st * K::kStage + 2 * DKB * kTile);
         auto fetch_e = [&]() {  // rows past the sequence and columns past the width read as zero
           const uint16_t* src = pe + (first + r0) * j.e.st + 8 * c4;
@@ -709,7 +742,6 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             __syncwarp();
           }
         }
-        const int64_t at = (w.start + first + r0) * stride + w.h * j.dc + col0;
         uint64_t dot[2] = {0, 0};  // four FP32 sums
         uint32_t x[16], y[16];
         const uint32_t tm = tmem + tm_lane + 32u * half;
@@ -797,49 +829,64 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     regs_down<kRegsRest>();
     if (warp == 28 || warp == 31) {
     // ---------------- TMA: a and b, and in a warp of its own c, whose tile is free later
-    if (lane == 0) {
-      const bool ab = warp == 28;
-      uint64_t* const full = ab ? bar.full_ab : bar.full_c;
-      for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
-        Item w;
-        item_of(args, idx, &w);
+    const bool ab = warp == 28;
+    uint64_t* const full = ab ? bar.full_ab : bar.full_c;
+    auto fetch_item = [&]() {  // the next item: from the queue into its slot
+      const uint32_t slot = nitem & 3u;
+      if (lane == 0 && wait_for(&bar.qfree[slot], ((nitem >> 2) & 1u) ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER)) {
+        const int got = atomicAdd(args.queue, 1);
+        bar.taken[slot] = got < items ? got : items;
+        mbar_arrive(&bar.qfull[slot]);
+      }
+      __syncwarp();
+    };
+    const bool queue = args.order != nullptr && !ab;
+    int idx = blockIdx.x;
+    while (ok && idx < items) {
+      Item w;
+      item_of(args, idx, &w);
+      if (queue) fetch_item();
+      if (lane == 0) {
         const LaJob& j = args.la.job[w.job];
         const bool packed = args.la.cu != nullptr;
         const int batch = packed ? 0 : w.seq;
-        const int t0 = packed ? static_cast<int>(w.start) : 0;
-        for (int p = 0; p < w.n; ++p, ++it) {
-          const int st = static_cast<int>(it % K::kStages);
-          const uint32_t ph = ((it / K::kStages) & 1u) ^ 1u;
-          const int chunk = j.reverse != 0 ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
+        int t = (packed ? w.start : 0) + w.first;
+        for (int p = 0; p < w.n; ++p, advance(), t += w.step) {
           const uint32_t stage = base + st * K::kStage;
-          const int t = t0 + chunk * kC;
           if (!ab) {
-            if (!(ok = wait_for(&bar.empty_c[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
+            if (!(ok = wait_for(&bar.empty_c[st], ph ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
             mbar_arrive_expect_tx(&full[st], kTile);
             tma_load_4d(stage + 2 * DKB * kTile, &args.map[w.job][2], &full[st], 64 * w.slice, w.h / j.c.group, t, batch);
             continue;
           }
-          if (!(ok = wait_for(&bar.empty_b[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
+          if (!(ok = wait_for(&bar.empty_b[st], ph ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) break;
           mbar_arrive_expect_tx(&full[st], (full_pass ? 2 * DKB : DKB) * kTile);
           for (int x = 0; x < DKB; ++x)
             tma_load_4d(stage + (DKB + x) * kTile, &args.map[w.job][1], &full[st], 64 * x, w.h / j.b.group, t, batch);
           if (full_pass) {
             // with b's copies on their way the count has to come to its end: a's follow even after a failed wait
-            ok = wait_for(&bar.empty_a[st], ph, failed, SPX_DEV_TIMEOUT_PRODUCER);
+            ok = wait_for(&bar.empty_a[st], ph ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER);
             for (int x = 0; x < DKB; ++x)
               tma_load_4d(stage + x * kTile, &args.map[w.job][0], &full[st], 64 * x, w.h / j.a.group, t, batch);
             if (!ok) {
-              ++it;
+              advance();
               break;
             }
           }
         }
       }
-      if (!ok) {  // leave no copy in flight behind an abandoned pipeline
-        for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
-          const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
-          wait_for(&full[s], (last / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_PRODUCER);
-        }
+      ok = __all_sync(0xFFFFFFFFu, ok) != 0;
+      if (!queue) {
+        idx = next_item(idx);
+      } else {
+        idx = *const_cast<volatile int*>(&bar.taken[nitem & 3u]);
+        ++nitem;
+      }
+    }
+    if (lane == 0 && !ok) {  // leave no copy in flight behind an abandoned pipeline
+      for (int s = 0; s < K::kStages && static_cast<uint32_t>(s) < it; ++s) {
+        const uint32_t last = it - 1 - ((it - 1 - s) % K::kStages);  // the newest chunk loaded into stage s
+        wait_for(&full[s], (last / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_PRODUCER);
       }
     }
     } else if (warp == 29) {
@@ -849,15 +896,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       const uint32_t id_o = idesc_bf16_f32(128, 64) | (1u << 16);               // B MN-major
       const uint32_t id_kv = idesc_bf16_f32(128, K::kParts == 3 ? 64 : 128) | (1u << 15) | (1u << 16);  // A and B MN-major
       uint32_t tails = 0;
-      auto fixed = [&](const Item& w, int p) {  // whether the chunk's tail rows are zeroed first
-        const bool rev = args.la.job[w.job].reverse != 0;
-        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-        return args.la.cu != nullptr && w.len - static_cast<int64_t>(chunk) * kC < kC;
-      };
-      auto ready = [&](const Item& w, int p, uint32_t n) {  // chunk n's tiles are in shared memory
-        const int st = static_cast<int>(n % K::kStages);
-        if (!warp_wait(&bar.full_ab[st], (n / K::kStages) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
-        if (full_pass && fixed(w, p)) {
+      uint32_t ast = 0, aph = 0;  // stage and parity of the chunk to start
+      auto ready = [&](const Item& w, int p) {  // its tiles are in shared memory
+        if (!warp_wait(&bar.full_ab[ast], aph, failed, SPX_DEV_TIMEOUT_MMA)) return false;
+        // the tail of a packed sequence: its rows are zeroed first
+        if (full_pass && args.la.cu != nullptr && w.len - (w.first + p * w.step) < kC) {
           if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
           ++tails;
         }
@@ -865,7 +908,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         return true;
       };
       auto product_ab = [&](uint32_t n) {  // a . b of chunk n
-        const uint32_t sa = base + (n % K::kStages) * K::kStage;
+        const uint32_t sa = base + ast * K::kStage;
         const uint64_t da = desc_kmajor_sw128(sa), db = desc_kmajor_sw128(sa + DKB * kTile);
         const uint32_t acc = tmem + kTmP + (n & 1u) * 128u;
         if (elect_one()) {
@@ -885,7 +928,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       if (more) item_of(args, nidx, &nw);
       auto settle = [&]() {
         while (more && np >= nw.n) {
-          nidx += gridDim.x;
+          nidx = next_item(nidx);
           np = 0;
           if ((more = nidx < items)) item_of(args, nidx, &nw);
         }
@@ -894,7 +937,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       uint32_t ahead = 0;  // chunks whose tiles are known to be ready
       auto start_next = [&]() {
         if (!more) return true;
-        if (!ready(nw, np, ahead)) return false;
+        if (!ready(nw, np)) return false;
         if (full_pass) {
           // the buffer's last reader: the product with c two chunks before
           if (ahead >= 2 && !warp_wait(&bar.o, (ahead - 2) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
@@ -902,12 +945,15 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
         ++ahead;
         ++np;
+        if (++ast == K::kStages) {
+          ast = 0;
+          aph ^= 1u;
+        }
         settle();
-        return true;
+        return ok;
       };
       ok = start_next();
       while (ok && it < ahead) {
-        const int st = static_cast<int>(it % K::kStages);
         const uint32_t stage = base + st * K::kStage;
         // state product b^T (scaled c)
         if (!(ok = warp_wait(&bar.vp[it & 1u], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
@@ -969,38 +1015,37 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           }
           __syncwarp();
         }
-        ++it;
+        advance();
       }
       if (elect_one()) mma_commit(&bar.drained);  // arrives once everything issued above has completed
       __syncwarp();
     }
     } else if (warp == 30) {
     // ---------------- decay tables: lane l of block b is token 32 b + l
-    for (int idx = blockIdx.x; ok && idx < items; idx += gridDim.x) {
+    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
       Item w;
       item_of(args, idx, &w);
-      const bool rev = args.la.job[w.job].reverse != 0;
+      const bool rev = w.step < 0;
       const bool packed = args.la.cu != nullptr;
       const int64_t g0 = (packed ? 0 : w.seq) * args.la.g_sb + (packed ? w.start : 0) * args.la.g_st + w.h * args.la.g_sh;
       uint32_t next[4];  // raw: nothing of a load is used before the next chunk
       const bool f32 = args.la.g_f32 != 0;
-      auto fetch = [&](int p) {
-        const int chunk = rev ? w.nch - 1 - (w.p0 + p) : w.p0 + p;
-        const int64_t t0 = static_cast<int64_t>(chunk) * kC + lane;
+      int t = w.first + lane;
+      auto fetch = [&]() {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int64_t t = t0 + 32 * q;
           next[q] = 0u;  // past the sequence: no decay
-          if (t < w.len) {
-            const int64_t at = g0 + t * args.la.g_st;
+          if (t + 32 * q < w.len) {
+            const int64_t at = g0 + (t + 32 * q) * args.la.g_st;
             if (f32)
               next[q] = __ldg(reinterpret_cast<const uint32_t*>(args.la.g) + at);
             else
               next[q] = __ldg(reinterpret_cast<const uint16_t*>(args.la.g) + at);
           }
         }
+        t += w.step;
       };
-      if (w.n > 0) fetch(0);
+      if (w.n > 0) fetch();
       for (int p = 0; p < w.n; ++p, ++it) {
         const uint32_t b = it & 1u;
         float up[4], down[4];  // sums up to the lane's token, and after it
@@ -1011,7 +1056,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           const float after = __shfl_down_sync(0xFFFFFFFFu, up[q], 1);
           down[q] = lane == 31 ? 0.0f : after;
         }
-        if (p + 1 < w.n) fetch(p + 1);
+        if (p + 1 < w.n) fetch();
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
 #pragma unroll
@@ -1044,6 +1089,29 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     tc_fence_after();
     if (lane == 0 && *failed != 0) record_error(status, *failed);
     tmem_dealloc(tmem, kTmCols);
+  }
+}
+
+// The sequences by their number of chunks, longest first (ties by index), and
+// the queue's start: a rank is the count of those that come before.
+__global__ void __launch_bounds__(1024) la_order_kernel(const int32_t* __restrict__ cu, int n, int64_t total,
+                                                        int* __restrict__ order, int* __restrict__ queue, int first_state,
+                                                        int first_full) {
+  __shared__ int chunks[kOrderMax];
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int lo = cu[i], hi = cu[i + 1];
+    chunks[i] = lo >= 0 && hi >= lo && hi <= total ? (hi - lo + kC - 1) / kC : 0;
+  }
+  if (threadIdx.x == 0) {  // each pass has its own, behind the items that its CTAs start with
+    queue[0] = first_state;
+    queue[1] = first_full;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int mine = chunks[i];
+    int rank = 0;
+    for (int k = 0; k < n; ++k) rank += chunks[k] > mine || (chunks[k] == mine && k < i) ? 1 : 0;
+    order[rank] = i;
   }
 }
 
@@ -1113,12 +1181,17 @@ int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total +
 
 }  // namespace
 
+namespace {
+bool ordered(const LaArgs& a) { return a.cu != nullptr && a.nseq > 1 && a.nseq <= kOrderMax; }
+size_t order_bytes(const LaArgs& a) { return ordered(a) ? (static_cast<size_t>(a.nseq) + 2 + 3) / 4 * 16 : 0; }
+}  // namespace
+
 size_t la_chunk_workspace(const LaArgs& a) {
   int slices[3];
   int64_t first[4];
   const int64_t lanes = lanes_of(a, slices, first);
   const int nseg = segments_for(lanes, mean_tokens(a), device_sm_count());
-  return nseg == 1 ? 0 : static_cast<size_t>(lanes) * nseg * (8192 + 1) * sizeof(float);
+  return order_bytes(a) + (nseg == 1 ? 0 : static_cast<size_t>(lanes) * nseg * (8192 + 1) * sizeof(float));
 }
 
 int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream) {
@@ -1145,9 +1218,19 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
     }
   }
   for (int i = 0; i <= a.njobs; ++i) c.lanes[i] = static_cast<int>(first[i]);
+  if (workspace == nullptr && (c.nseg > 1 || ordered(a))) return SPX_ERR_WORKSPACE;
+  if (ordered(a)) {
+    int* const order = static_cast<int*>(workspace) + 2;
+    c.order = order;
+    c.queue = order - 2;
+    const int state_ctas = static_cast<int>(std::min<int64_t>(lanes * (c.nseg - 1), sms));
+    const int full_ctas = static_cast<int>(std::min<int64_t>(lanes * c.nseg, sms));
+    la_order_kernel<<<1, a.nseq < 1024 ? (a.nseq + 31) / 32 * 32 : 1024, 0, stream>>>(a.cu, a.nseq, a.total, order, c.queue,
+                                                                                     state_ctas, full_ctas);
+    if (cudaGetLastError() != cudaSuccess) return SPX_ERR_CUDA;
+  }
   if (c.nseg > 1) {
-    if (workspace == nullptr) return SPX_ERR_WORKSPACE;
-    c.seg_state = static_cast<float*>(workspace);
+    c.seg_state = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + order_bytes(a));
     c.seg_decay = c.seg_state + lanes * c.nseg * 8192;
   }
   auto run = [&](auto kernel, size_t smem) {
@@ -1177,6 +1260,7 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
   }
   c.state_only = 0;
   c.run_segs = c.nseg;
+  if (c.queue != nullptr) ++c.queue;
   return pass();
 }
 
