@@ -196,6 +196,25 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// Whether a phase is over, at once (a try_wait may sleep first).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0u;
+}
+
+// A wait whose first poll was made earlier, so that its latency has passed.
+__device__ __forceinline__ bool wait_after(bool polled, uint64_t* bar, uint32_t parity, int* failed, int code) {
+  if (__all_sync(0xFFFFFFFFu, polled) != 0) return true;
+  return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, failed, code)) != 0;
+}
+
 // Every lane polls; the warp goes on together, or gives up together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* failed, int code) {
   return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, failed, code)) != 0;
@@ -341,8 +360,9 @@ struct Bars {
   uint64_t gfull[2], gfree[2];
   uint64_t pacc[2], pop[2];
   uint64_t tail[2];  // at most one tail is fixed ahead of the one being waited for
-  uint64_t vp[2], kv[2], kvfree[2];  // by the chunk's parity
-  uint64_t sop, qs, o, ofree, drained;
+  uint64_t kvgo[2], kv[2];  // by the chunk's parity: scaled c is there and the accumulator free; the product done
+  uint64_t qsgo, qs;        // the state's operand is there and the output's accumulators free; a . S done
+  uint64_t o, drained;
   uint64_t qfull[4], qfree[4];  // of the items taken from the queue
   int taken[4];
   uint32_t tmem;
@@ -393,18 +413,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       mbar_init(&bar.pacc[s], 1);
       mbar_init(&bar.pop[s], 8);
       mbar_init(&bar.tail[s], 8);
-      mbar_init(&bar.vp[s], 8);
+      mbar_init(&bar.kvgo[s], 12);
       mbar_init(&bar.kv[s], 1);
-      mbar_init(&bar.kvfree[s], 4);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&bar.qfull[s], 1);
       mbar_init(&bar.qfree[s], full_pass ? 31 : 15);  // every warp that takes items but the one that fetches them
     }
-    mbar_init(&bar.sop, 4);
+    mbar_init(&bar.qsgo, 12);
     mbar_init(&bar.qs, 1);
     mbar_init(&bar.o, 1);
-    mbar_init(&bar.ofree, 8);
     mbar_init(&bar.drained, 1);
     bar.failed = 0;
     fence_mbar_init();
@@ -474,16 +492,17 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         // that decays by more than 2^100 takes the exponential of each difference
         float run = a - own;
         const bool steep = !(own >= -100.0f);
+        uint32_t x[16];  // a block's columns; once they are multiplied, the next block's are on their way
+        tmem_ld16(acc + 32u * quad + 16u * half, x);
 #pragma unroll 1
         for (int n = 0; n < 4; ++n) {
           const int j = (rev ? quad + n : quad - n) & 3;
           const int c0 = 32 * j + 16 * half;
-          uint32_t x[16];  // columns in, words out
+          uint32_t words[16];
           if (rev ? j < quad : j > quad) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) x[q] = 0u;
+            for (int q = 0; q < 16; ++q) words[q] = 0u;
           } else {
-            tmem_ld16(acc + c0, x);
             const float rf = ex2(run);
             const uint64_t rf2 = pair(rf, rf);
             run += t.total[j];
@@ -501,25 +520,24 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             }
             tmem_wait_ld();
 #pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = mul2(pair(x[2 * q], x[2 * q + 1]), f[q]);
+            if (rev ? j < 3 : j > 0) tmem_ld16(acc + (rev ? c0 + 32 : c0 - 32), x);
+#pragma unroll
             for (int q = 0; q < 8; ++q) {
               uint32_t part[PRECISE ? 2 : 1];
-              split2<PRECISE ? 2 : 1>(mul2(pair(x[2 * q], x[2 * q + 1]), f[q]), part);
-              x[q] = part[0];  // its column has been taken: 2 q >= q
-              if constexpr (PRECISE) f[q] = part[1];
-            }
-            if constexpr (PRECISE) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) x[8 + q] = static_cast<uint32_t>(f[q]);
+              split2<PRECISE ? 2 : 1>(f[q], part);
+              words[q] = part[0];
+              if constexpr (PRECISE) words[8 + q] = part[1];
             }
             if (n == 0) {
 #pragma unroll
-              for (int q = 0; q < (PRECISE ? 16 : 8); ++q) x[q] &= mask[q & 7];
+              for (int q = 0; q < (PRECISE ? 16 : 8); ++q) words[q] &= mask[q & 7];
             }
           }
           if constexpr (PRECISE)
-            tmem_st16(acc + c0, x);
+            tmem_st16(acc + c0, words);
           else
-            tmem_st8(acc + c0, x);
+            tmem_st8(acc + c0, words);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -576,13 +594,14 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             sts16(dst[part] ^ (c << 4), q[0][part], q[1][part], q[2][part], q[3][part]);
         }
         fence_proxy_async_smem();
-        warp_arrive(&bar.vp[b], lane);
+        warp_arrive(&bar.kvgo[b], lane);
       }
     }
   } else if (warp < 20) {
     regs_up<kRegsState>();
     // ---------------- the state: one row of da, 64 columns, in registers
     const bool rows_in = quad < 2 * DKB;
+    for (uint32_t n = 0; n < depth; ++n) warp_arrive(&bar.kvgo[n], lane);  // the accumulators are free at first
     for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
       Item w;
       const bool sound = item_of(args, idx, &w);
@@ -622,7 +641,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           }
         }
         fence_proxy_async_smem();
-        warp_arrive(&bar.sop, lane);
+        warp_arrive(&bar.qsgo, lane);
       };
       for (int p = 0; p < w.n; ++p, ++it) {
         const uint32_t b = it & 1u;
@@ -656,7 +675,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           }
         }
         tc_fence_before();
-        warp_arrive(&bar.kvfree[b], lane);
+        warp_arrive(&bar.kvgo[(it + depth) & 1u], lane);  // for the chunk `depth` on
       }
       if (!ok) break;
       if (!full_pass) {
@@ -685,6 +704,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     static_assert(kRegsOut == 64, "the launch's own");
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- epilogue: 32 columns of one token a thread
+    if (full_pass) warp_arrive(&bar.qsgo, lane);  // the accumulators are free at first
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
       Item w;
       item_of(args, idx, &w);
@@ -753,7 +773,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           if (part == 1) {
             // the accumulators are free before the stores: the next chunk's products wait for them
             tc_fence_before();
-            warp_arrive(&bar.ofree, lane);
+            warp_arrive(&bar.qsgo, lane);  // for the next chunk
           }
           uint64_t v[8];
 #pragma unroll
@@ -897,16 +917,6 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       const uint32_t id_kv = idesc_bf16_f32(128, K::kParts == 3 ? 64 : 128) | (1u << 15) | (1u << 16);  // A and B MN-major
       uint32_t tails = 0;
       uint32_t ast = 0, aph = 0;  // stage and parity of the chunk to start
-      auto ready = [&](const Item& w, int p) {  // its tiles are in shared memory
-        if (!warp_wait(&bar.full_ab[ast], aph, failed, SPX_DEV_TIMEOUT_MMA)) return false;
-        // the tail of a packed sequence: its rows are zeroed first
-        if (full_pass && args.la.cu != nullptr && w.len - (w.first + p * w.step) < kC) {
-          if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
-          ++tails;
-        }
-        tc_fence_after();
-        return true;
-      };
       auto product_ab = [&](uint32_t n) {  // a . b of chunk n
         const uint32_t sa = base + ast * K::kStage;
         const uint64_t da = desc_kmajor_sw128(sa), db = desc_kmajor_sw128(sa + DKB * kTile);
@@ -934,15 +944,19 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         }
       };
       settle();
-      uint32_t ahead = 0;  // chunks whose tiles are known to be ready
-      auto start_next = [&]() {
+      uint32_t ahead = 0;  // chunks whose a . b has been issued (state-only: whose tiles are there)
+      auto start_next = [&](bool polled) {
         if (!more) return true;
-        if (!ready(nw, np)) return false;
-        if (full_pass) {
-          // the buffer's last reader: the product with c two chunks before
-          if (ahead >= 2 && !warp_wait(&bar.o, (ahead - 2) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
-          product_ab(ahead);
+        if (!wait_after(polled, &bar.full_ab[ast], aph, failed, SPX_DEV_TIMEOUT_MMA)) return false;
+        // the tail of a packed sequence: its rows are zeroed first
+        if (full_pass && args.la.cu != nullptr && nw.len - (nw.first + np * nw.step) < kC) {
+          if (!warp_wait(&bar.tail[tails & 1u], (tails >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA)) return false;
+          ++tails;
         }
+        tc_fence_after();
+        // its accumulator's last reader is the product with c two chunks before: done, as the
+        // epilogue of that chunk has freed the output for the a . S issued before this
+        if (full_pass) product_ab(ahead);
         ++ahead;
         ++np;
         if (++ast == K::kStages) {
@@ -952,13 +966,17 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         settle();
         return ok;
       };
-      ok = start_next();
+      ok = start_next(false);
+      bool kv_ready = false;
       while (ok && it < ahead) {
+        const uint32_t b = it & 1u, ph2 = (it >> 1) & 1u;
         const uint32_t stage = base + st * K::kStage;
+        // A satisfied wait still takes a few hundred cycles of a busy CTA: each is polled one product ahead.
         // state product b^T (scaled c)
-        if (!(ok = warp_wait(&bar.vp[it & 1u], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
-        if (it >= depth && !(ok = warp_wait(&bar.kvfree[(it - depth) & 1u], ((it - depth) >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = wait_after(kv_ready, &bar.kvgo[b], ph2, failed, SPX_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
+        const bool qs_ready = full_pass && mbar_test(&bar.qsgo, it & 1u);
+        const bool ab_ready = mbar_test(&bar.full_ab[ast], aph);
         const uint64_t db = desc_mn(stage + DKB * kTile, kTile);
         uint64_t dv[K::kParts];  // (two parts: the first, with the distance to the second)
 #pragma unroll
@@ -973,17 +991,17 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             for (uint32_t part = 0; part < (K::kParts == 3 ? 3u : 1u); ++part)
               mma_bf16_ss(acc, db + q * 128u, dv[part] + q * 128u, id_kv, (part | q) != 0u ? 1u : 0u);
           }
-          mma_commit(&bar.kv[it & 1u]);
+          mma_commit(&bar.kv[b]);
           mma_commit(&bar.empty_b[st]);  // a . b of this chunk was issued before
           if (!full_pass) mma_commit(&bar.empty_c[st]);
         }
         __syncwarp();
-        if (!(ok = start_next())) break;
+        bool pop_ready = false;
         if (full_pass) {
           // a . S
-          if (!(ok = warp_wait(&bar.sop, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
-          if (it > 0 && !(ok = warp_wait(&bar.ofree, (it - 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = wait_after(qs_ready, &bar.qsgo, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
+          pop_ready = mbar_test(&bar.pop[b], ph2);
           const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
           if (elect_one()) {
 #pragma unroll
@@ -997,11 +1015,14 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             mma_commit(&bar.empty_a[st]);
           }
           __syncwarp();
+        }
+        if (!(ok = start_next(ab_ready))) break;
+        kv_ready = mbar_test(&bar.kvgo[b ^ 1u], ((it + 1) >> 1) & 1u);
+        if (full_pass) {
           // (decayed a . b) c
-          const uint32_t b = it & 1u;
-          const uint64_t dc = desc_mn(stage + 2 * DKB * kTile, kTile);
-          if (!(ok = warp_wait(&bar.pop[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = wait_after(pop_ready, &bar.pop[b], ph2, failed, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
+          const uint64_t dc = desc_mn(stage + 2 * DKB * kTile, kTile);
           if (elect_one()) {
 #pragma unroll
             for (uint32_t q = 0; q < 8; ++q) {
