@@ -60,8 +60,7 @@ constexpr int kTile = kC * 128;      // bytes of a [128 tokens][64] BF16 tile
 constexpr int kLaThreads = 32 * 32;  // eight warpgroups
 constexpr int64_t kWaitCycles = 4000000000;  // about two seconds
 // Registers of the warpgroups' threads: the launch gives each 64 (1024 x 64 = 65,536).
-constexpr int kRegsAB = 64, kRegsC = 48, kRegsState = 120, kRegsOut = 64, kRegsRest = 40;
-static_assert(2 * kRegsAB + 2 * kRegsC + kRegsState + 2 * kRegsOut + kRegsRest <= 8 * 64, "registers of a CTA");
+constexpr int kRegsC = 48, kRegsRest = 40;
 constexpr int kOrderMax = 4096;  // more sequences are taken as they come
 constexpr uint32_t kBarBytes = 416;
 constexpr uint32_t kTmP = 0, kTmOI = 256, kTmOX = 320, kTmKV = 384, kTmCols = 512;
@@ -114,6 +113,12 @@ struct Cfg {
   static constexpr int kStages = DKB == 1 ? 3 : 2;
   static constexpr int kParts = PARTS;            // of scaled c
   static constexpr int kSParts = PRECISE ? 2 : 1; // of the state
+  // 64 rows of state in the 128 lanes of an accumulator: computed twice, so that each of the four warps
+  // keeps half of the columns of 32 rows and not two of them all (training backward 459 -> 412 us for 65,536
+  // tokens, 12 heads; packed prompts 79 -> 72).
+  static constexpr int kStateCols = DKB == 1 ? 32 : 64;
+  static constexpr int kRegsState = DKB == 1 ? 88 : 120;
+  static_assert(4 * 64 + 2 * kRegsC + kRegsState + kRegsRest <= 8 * 64, "registers of a CTA");
   static constexpr uint32_t kStage = (2 * DKB + 1) * kTile;
   static constexpr uint32_t kSTile = DKB * 64 * 128;
   static constexpr uint32_t kOffS = kStages * kStage;
@@ -462,7 +467,6 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   };
 
   if (warp < 8) {
-    static_assert(kRegsAB == 64, "the launch's own");
     // ---------------- the decayed a . b matrix: 16 columns of each 32-token block
     const int half = warp >> 2;
     for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
@@ -598,24 +602,26 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       }
     }
   } else if (warp < 20) {
-    regs_up<kRegsState>();
-    // ---------------- the state: one row of da, 64 columns, in registers
-    const bool rows_in = quad < 2 * DKB;
+    regs_up<K::kRegsState>();
+    // ---------------- the state: 64 (or 32) columns of one row of da, in registers
+    constexpr int kN = K::kStateCols / 2;  // pairs of columns
+    const int row = (DKB == 1 ? quad & 1 : quad) * 32 + lane;
+    const int part_col = DKB == 1 ? (quad >> 1) * 32 : 0;
     for (uint32_t n = 0; n < depth; ++n) warp_arrive(&bar.kvgo[n], lane);  // the accumulators are free at first
     for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
       Item w;
       const bool sound = item_of(args, idx, &w);
       const LaJob& j = args.la.job[w.job];
       if (!sound && threadIdx.x == 512) *failed = SPX_DEV_BAD_TILE;
-      uint64_t s[32];  // pairs of columns
+      uint64_t s[kN];
       const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
-      const int col0 = w.slice * 64;
+      const int col0 = w.slice * 64 + part_col;
       const bool live = row < j.da;
+      float* const seg = args.seg_state == nullptr ? nullptr : args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64 + part_col;
       if (args.nseg > 1 && full_pass) {
-        const float4* f = reinterpret_cast<const float4*>(
-            args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64);
+        const float4* f = reinterpret_cast<const float4*>(seg);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
+        for (int q = 0; q < kN / 2; ++q) {
           const float4 v = live ? f[q] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           s[2 * q] = pair(v.x, v.y);
           s[2 * q + 1] = pair(v.z, v.w);
@@ -624,21 +630,19 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const float* f = j.init + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.init != nullptr && args.nseg == 1 && live ? j.dc - col0 : 0;
 #pragma unroll
-        for (int c = 0; c < 32; ++c, f += 2 * j.s_col)  // widths are even
+        for (int c = 0; c < kN; ++c, f += 2 * j.s_col)  // widths are even
           s[c] = 2 * c < n ? pair(j.init_scale * f[0], j.init_scale * f[j.s_col]) : 0;
       }
       float decay = 1.0f;
       auto write_operand = [&]() {  // BF16 parts of the state for the next chunk's a . S
-        if (rows_in) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t q[4][K::kSParts];
+        for (int c = 0; c < kN / 4; ++c) {
+          uint32_t q[4][K::kSParts];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split2<K::kSParts>(s[4 * c + e], q[e]);
+          for (int e = 0; e < 4; ++e) split2<K::kSParts>(s[4 * c + e], q[e]);
 #pragma unroll
-            for (int part = 0; part < K::kSParts; ++part)
-              sts16(base + K::kOffS + part * K::kSTile + swz(row, c), q[0][part], q[1][part], q[2][part], q[3][part]);
-          }
+          for (int part = 0; part < K::kSParts; ++part)
+            sts16(base + K::kOffS + part * K::kSTile + swz(row, part_col / 8 + c), q[0][part], q[1][part], q[2][part], q[3][part]);
         }
         fence_proxy_async_smem();
         warp_arrive(&bar.qsgo, lane);
@@ -657,21 +661,19 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const uint64_t gamma2 = pair(gamma, gamma);
         decay *= gamma;
         if (!(ok = warp_wait(&bar.kv[b], (it >> 1) & 1u, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
-        const uint32_t acc = tmem + acc_at(it) + tm_lane;
+        const uint32_t acc = tmem + acc_at(it) + tm_lane + part_col;
         tc_fence_after();
-        if (rows_in) {
 #pragma unroll
-          for (int part = 0; part < 4; ++part) {
-            uint32_t x[16], y[16];
-            tmem_ld16(acc + 16u * part, x);
-            if constexpr (K::kParts == 2) tmem_ld16(acc + 64u + 16u * part, y);
-            tmem_wait_ld();
+        for (int part = 0; part < kN / 8; ++part) {
+          uint32_t x[16], y[16];
+          tmem_ld16(acc + 16u * part, x);
+          if constexpr (K::kParts == 2) tmem_ld16(acc + 64u + 16u * part, y);
+          tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint64_t add = pair(x[2 * c], x[2 * c + 1]);
-              if constexpr (K::kParts == 2) add = add2(add, pair(y[2 * c], y[2 * c + 1]));
-              s[8 * part + c] = fma2(gamma2, s[8 * part + c], add);
-            }
+          for (int c = 0; c < 8; ++c) {
+            uint64_t add = pair(x[2 * c], x[2 * c + 1]);
+            if constexpr (K::kParts == 2) add = add2(add, pair(y[2 * c], y[2 * c + 1]));
+            s[8 * part + c] = fma2(gamma2, s[8 * part + c], add);
           }
         }
         tc_fence_before();
@@ -679,18 +681,17 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       }
       if (!ok) break;
       if (!full_pass) {
-        float4* f = reinterpret_cast<float4*>(
-            args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64);
+        float4* f = reinterpret_cast<float4*>(seg);
         if (live) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q) *reinterpret_cast<ulonglong2*>(f + q) = make_ulonglong2(s[2 * q], s[2 * q + 1]);
+          for (int q = 0; q < kN / 2; ++q) *reinterpret_cast<ulonglong2*>(f + q) = make_ulonglong2(s[2 * q], s[2 * q + 1]);
         }
         if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
 #pragma unroll
-        for (int c = 0; c < 32; ++c, f += 2 * j.s_col) {
+        for (int c = 0; c < kN; ++c, f += 2 * j.s_col) {
           float v0, v1;
           unpair(s[c], v0, v1);
           if (2 * c < n) {
@@ -701,7 +702,6 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       }
     }
   } else if (warp < 28) {
-    static_assert(kRegsOut == 64, "the launch's own");
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- epilogue: 32 columns of one token a thread
     if (full_pass) warp_arrive(&bar.qsgo, lane);  // the accumulators are free at first
@@ -766,20 +766,18 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         uint32_t x[16], y[16];
         const uint32_t tm = tmem + tm_lane + 32u * half;
 #pragma unroll 1
-        for (int part = 0; part < 2; ++part) {  // 16 columns
+        for (uint32_t part = 0; part < 2; ++part) {  // 16 columns
           tmem_ld16(tm + kTmOI + 16u * part, x);
           tmem_ld16(tm + kTmOX + 16u * part, y);
           tmem_wait_ld();
-          if (part == 1) {
+          if (part == 1u) {
             // the accumulators are free before the stores: the next chunk's products wait for them
             tc_fence_before();
-            warp_arrive(&bar.qsgo, lane);  // for the next chunk
+            warp_arrive(&bar.qsgo, lane);
           }
           uint64_t v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = fma2(sx2, pair(y[2 * i], y[2 * i + 1]), mul2(sc2, pair(x[2 * i], x[2 * i + 1])));
-          }
+          for (int i = 0; i < 8; ++i) v[i] = fma2(sx2, pair(y[2 * i], y[2 * i + 1]), mul2(sc2, pair(x[2 * i], x[2 * i + 1])));
           if constexpr (PRECISE) {
             if (f32) {  // (no dots then) 16 columns at a time fill this warp's half of the tile
 #pragma unroll
@@ -977,7 +975,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         tc_fence_after();
         const bool qs_ready = full_pass && mbar_test(&bar.qsgo, it & 1u);
         const bool ab_ready = mbar_test(&bar.full_ab[ast], aph);
-        const uint64_t db = desc_mn(stage + DKB * kTile, kTile);
+        const uint64_t db = desc_mn(stage + DKB * kTile, DKB == 1 ? 0u : kTile);  // 64 columns: the same rows twice
         uint64_t dv[K::kParts];  // (two parts: the first, with the distance to the second)
 #pragma unroll
         for (uint32_t part = 0; part < K::kParts; ++part) dv[part] = desc_mn(part_at(it, part), part_at(it, 1) - part_at(it, 0));
