@@ -581,6 +581,7 @@ struct LaDecayGradArgs {
   const int32_t* cu;
   int64_t T, total, state_elems;
   int nseq, H, g_f32;
+  int from_zero;  // no initial states
 };
 int launch_la_decay_grad(const LaDecayGradArgs& a, cudaStream_t stream);
 // out[t][kv][d] = bf16(sum over the group's query heads of in[t][h][d]); with

@@ -75,6 +75,10 @@ struct alignas(64) LaChunkArgs {
   int* queue;            // with order: the next item to take
   float* seg_state;      // [lane][nseg][128][64]
   float* seg_decay;      // [lane][nseg]
+  // Even shares (or null): every CTA takes as many chunks, and a lane that two of
+  // them share is handed on by its state, [CTA][128][64], and a flag per warp of it.
+  float* hand;
+  int* handed;
 };
 
 // Decays of a chunk, each sum taken directly (a small one as the difference of
@@ -137,12 +141,44 @@ struct Item {
   int start, len;   // tokens of the sequence in the flattened order
   int n;            // this item's chunks
   int first, step;  // first token of the first of them in the sequence, and to the next one's
+  bool resume, save;  // goes on from the CTA before; is gone on with by the next one
 };
 
-__device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it) {
+// A CTA's share of all lanes' chunks in a row.  It is at least one lane, so that
+// a lane is cut at most once: the share is the end of a lane, whole lanes, and
+// the start of another.
+struct Share {
+  int lane0, at0, lane1, at1;  // from chunk at0 of lane0 up to chunk at1 of lane1
+  __device__ __forceinline__ void set(int lanes, int chunks) {
+    const int64_t all = static_cast<int64_t>(lanes) * chunks, cta = blockIdx.x, ctas = gridDim.x;
+    const int64_t lo = cta * all / ctas, hi = (cta + 1) * all / ctas;
+    lane0 = static_cast<int>(lo / chunks);
+    at0 = static_cast<int>(lo - static_cast<int64_t>(lane0) * chunks);
+    lane1 = static_cast<int>(hi / chunks);
+    at1 = static_cast<int>(hi - static_cast<int64_t>(lane1) * chunks);
+  }
+  __device__ __forceinline__ int whole() const { return lane0 + (at0 > 0 ? 1 : 0); }  // the first one
+  __device__ __forceinline__ int items() const { return lane1 - whole() + 2; }
+};
+
+__device__ __forceinline__ bool item_of(const LaChunkArgs& a, const Share& s, int idx, Item* it) {
   const int all = a.lanes[a.la.njobs];
-  it->seg = idx / all;
-  it->lane = idx - it->seg * all;
+  int from = 0, till = 0;  // of its chunks, with even shares
+  if (a.hand != nullptr) {
+    // the start that another CTA goes on from comes first, and the end that needs another's state last
+    const int chunks = static_cast<int>((a.la.T + kC - 1) / kC);
+    const int last = s.items() - 1;
+    it->save = idx == 0;
+    it->resume = idx == last;
+    it->lane = idx == 0 ? min(s.lane1, all - 1) : idx == last ? s.lane0 : s.whole() + idx - 1;
+    from = idx == last ? s.at0 : 0;
+    till = idx == 0 ? s.at1 : idx == last && s.at0 == 0 ? 0 : chunks;
+    it->seg = 0;
+  } else {
+    it->save = it->resume = false;
+    it->seg = idx / all;
+    it->lane = idx - it->seg * all;
+  }
   int j = 0;
   while (j + 1 < a.la.njobs && it->lane >= a.lanes[j + 1]) ++j;
   it->job = j;
@@ -164,8 +200,8 @@ __device__ __forceinline__ bool item_of(const LaChunkArgs& a, int idx, Item* it)
   }
   const int nch = (it->len + kC - 1) / kC;
   const int per = (nch + a.nseg - 1) / a.nseg;
-  const int p0 = min(it->seg * per, nch);
-  it->n = min(per, nch - p0);
+  const int p0 = a.hand != nullptr ? from : min(it->seg * per, nch);
+  it->n = a.hand != nullptr ? till - from : min(per, nch - p0);
   const bool rev = a.la.job[j].reverse != 0;
   it->first = (rev ? nch - 1 - p0 : p0) * kC;
   it->step = rev ? -kC : kC;
@@ -218,6 +254,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool wait_after(bool polled, uint64_t* bar, uint32_t parity, int* failed, int code) {
   if (__all_sync(0xFFFFFFFFu, polled) != 0) return true;
   return __all_sync(0xFFFFFFFFu, wait_for(bar, parity, failed, code)) != 0;
+}
+
+// A flag in global memory that another CTA sets.
+__device__ __forceinline__ bool wait_flag(const int* flag, int* failed) {
+  const int64_t start = clock64();
+  int set;
+  do {
+    asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(set) : "l"(flag) : "memory");
+  } while (set == 0 && clock64() - start < kWaitCycles);
+  if (set == 0) *failed = SPX_DEV_TIMEOUT_PRODUCER;
+  return __all_sync(0xFFFFFFFFu, set != 0) != 0;
 }
 
 // Every lane polls; the warp goes on together, or gives up together.
@@ -370,6 +417,8 @@ struct Bars {
   uint64_t o, drained;
   uint64_t qfull[4], qfree[4];  // of the items taken from the queue
   int taken[4];
+  int items;
+  Share share;
   uint32_t tmem;
   int failed;
 };
@@ -392,7 +441,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   DecayTable* const tables = reinterpret_cast<DecayTable*>(la_smem + K::kOffT);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform to the compiler
   const bool full_pass = args.state_only == 0;
-  const int items = args.lanes[args.la.njobs] * args.run_segs;
+  const int item0 = args.hand != nullptr ? 0 : blockIdx.x, item_step = args.hand != nullptr ? 1 : gridDim.x;
   // The state-only pass has room for two chunks' parts of scaled c (the second in
   // the places of a and of the state's operand) and two accumulators, so that
   // scaling, product and update of neighbouring chunks overlap.
@@ -430,6 +479,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     mbar_init(&bar.o, 1);
     mbar_init(&bar.drained, 1);
     bar.failed = 0;
+    bar.items = args.lanes[args.la.njobs] * args.run_segs;
+    if (args.hand != nullptr) {
+      bar.share.set(bar.items, static_cast<int>((args.la.T + kC - 1) / kC));
+      bar.items = bar.share.items();
+    }
     fence_mbar_init();
   }
   if (warp == 29) {
@@ -440,6 +494,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar.tmem;
+  const int items = bar.items;
   const int quad = warp & 3;
   const uint32_t tm_lane = static_cast<uint32_t>(quad * 32) << 16;
   const int row = quad * 32 + lane;  // this thread's TMEM lane / tile row
@@ -457,7 +512,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   // CTAs take from; the warp of c's TMA fetches one ahead and hands it to the others.
   uint32_t nitem = 0;  // taken so far, the CTA's first item (its index) apart
   auto next_item = [&](int idx) {
-    if (args.order == nullptr) return idx + static_cast<int>(gridDim.x);
+    if (args.order == nullptr) return idx + item_step;
     const uint32_t slot = nitem & 3u;
     if (!(ok = warp_wait(&bar.qfull[slot], (nitem >> 2) & 1u, failed, SPX_DEV_TIMEOUT_PRODUCER))) return items;
     const int got = *const_cast<volatile int*>(&bar.taken[slot]);
@@ -469,9 +524,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   if (warp < 8) {
     // ---------------- the decayed a . b matrix: 16 columns of each 32-token block
     const int half = warp >> 2;
-    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
+    for (int idx = item0; full_pass && ok && idx < items; idx = next_item(idx)) {
       Item w;
-      item_of(args, idx, &w);
+      item_of(args, bar.share, idx, &w);
       const bool rev = w.step < 0;
       // of this row's words in the diagonal block: a masked entry is zero whatever it holds
       uint32_t mask[8];
@@ -554,9 +609,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- scaled c
     uint32_t tails = 0;
-    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
+    for (int idx = item0; ok && idx < items; idx = next_item(idx)) {
       Item w;
-      item_of(args, idx, &w);
+      item_of(args, bar.share, idx, &w);
       const bool rev = w.step < 0;
       int left = w.len - w.first;  // tokens from the chunk's first one on
       for (int p = 0; p < w.n; ++p, advance(), left -= w.step) {
@@ -608,9 +663,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     const int row = (DKB == 1 ? quad & 1 : quad) * 32 + lane;
     const int part_col = DKB == 1 ? (quad >> 1) * 32 : 0;
     for (uint32_t n = 0; n < depth; ++n) warp_arrive(&bar.kvgo[n], lane);  // the accumulators are free at first
-    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
+    for (int idx = item0; ok && idx < items; idx = next_item(idx)) {
       Item w;
-      const bool sound = item_of(args, idx, &w);
+      const bool sound = item_of(args, bar.share, idx, &w);
+      if (args.hand != nullptr && w.n == 0) continue;
       const LaJob& j = args.la.job[w.job];
       if (!sound && threadIdx.x == 512) *failed = SPX_DEV_BAD_TILE;
       uint64_t s[kN];
@@ -618,11 +674,16 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       const int col0 = w.slice * 64 + part_col;
       const bool live = row < j.da;
       float* const seg = args.seg_state == nullptr ? nullptr : args.seg_state + ((static_cast<int64_t>(w.lane) * args.nseg + w.seg) * 128 + row) * 64 + part_col;
-      if (args.nseg > 1 && full_pass) {
-        const float4* f = reinterpret_cast<const float4*>(seg);
+      if ((args.nseg > 1 && full_pass) || w.resume) {
+        const float* from = seg;
+        if (w.resume) {  // its start was its CTA's first item, so that it has long been done
+          from = args.hand + (static_cast<int64_t>(blockIdx.x - 1) * 128 + row) * 64 + part_col;
+          if (!(ok = wait_flag(args.handed + (blockIdx.x - 1) * 4 + quad, failed))) break;
+        }
+        const float4* f = reinterpret_cast<const float4*>(from);
 #pragma unroll
         for (int q = 0; q < kN / 2; ++q) {
-          const float4 v = live ? f[q] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const float4 v = live ? __ldcg(f + q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           s[2 * q] = pair(v.x, v.y);
           s[2 * q + 1] = pair(v.z, v.w);
         }
@@ -680,13 +741,18 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         warp_arrive(&bar.kvgo[(it + depth) & 1u], lane);  // for the chunk `depth` on
       }
       if (!ok) break;
-      if (!full_pass) {
-        float4* f = reinterpret_cast<float4*>(seg);
+      if (!full_pass || w.save) {
+        float4* f = reinterpret_cast<float4*>(
+            w.save ? args.hand + (static_cast<int64_t>(blockIdx.x) * 128 + row) * 64 + part_col : seg);
         if (live) {
 #pragma unroll
           for (int q = 0; q < kN / 2; ++q) *reinterpret_cast<ulonglong2*>(f + q) = make_ulonglong2(s[2 * q], s[2 * q + 1]);
         }
-        if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
+        if (w.save) {
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) atomicExch(args.handed + blockIdx.x * 4 + quad, 1);
+        } else if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
@@ -705,9 +771,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     const int half = warp >> 2 & 1;  // 32 of the 64 columns
     // ---------------- epilogue: 32 columns of one token a thread
     if (full_pass) warp_arrive(&bar.qsgo, lane);  // the accumulators are free at first
-    for (int idx = blockIdx.x; full_pass && ok && idx < items; idx = next_item(idx)) {
+    for (int idx = item0; full_pass && ok && idx < items; idx = next_item(idx)) {
       Item w;
-      item_of(args, idx, &w);
+      item_of(args, bar.share, idx, &w);
       const LaJob& j = args.la.job[w.job];
       const bool rev = w.step < 0, f32 = PRECISE && j.out_f32 != 0;
       const int col0 = w.slice * 64;
@@ -859,10 +925,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       __syncwarp();
     };
     const bool queue = args.order != nullptr && !ab;
-    int idx = blockIdx.x;
+    int idx = item0;
     while (ok && idx < items) {
       Item w;
-      item_of(args, idx, &w);
+      item_of(args, bar.share, idx, &w);
       if (queue) fetch_item();
       if (lane == 0) {
         const LaJob& j = args.la.job[w.job];
@@ -930,15 +996,15 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         __syncwarp();
       };
       // a . b runs one chunk ahead, over item borders
-      int nidx = blockIdx.x, np = 0;  // the next chunk to start
+      int nidx = item0, np = 0;  // the next chunk to start
       Item nw{};
       bool more = nidx < items;
-      if (more) item_of(args, nidx, &nw);
+      if (more) item_of(args, bar.share, nidx, &nw);
       auto settle = [&]() {
         while (more && np >= nw.n) {
           nidx = next_item(nidx);
           np = 0;
-          if ((more = nidx < items)) item_of(args, nidx, &nw);
+          if ((more = nidx < items)) item_of(args, bar.share, nidx, &nw);
         }
       };
       settle();
@@ -1041,9 +1107,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     }
     } else if (warp == 30) {
     // ---------------- decay tables: lane l of block b is token 32 b + l
-    for (int idx = blockIdx.x; ok && idx < items; idx = next_item(idx)) {
+    for (int idx = item0; ok && idx < items; idx = next_item(idx)) {
       Item w;
-      item_of(args, idx, &w);
+      item_of(args, bar.share, idx, &w);
       const bool rev = w.step < 0;
       const bool packed = args.la.cu != nullptr;
       const int64_t g0 = (packed ? 0 : w.seq) * args.la.g_sb + (packed ? w.start : 0) * args.la.g_st + w.h * args.la.g_sh;
@@ -1138,7 +1204,7 @@ __global__ void __launch_bounds__(1024) la_order_kernel(const int32_t* __restric
 __global__ void __launch_bounds__(256) la_chain_kernel(const __grid_constant__ LaChunkArgs args) {
   const int lane_id = blockIdx.x;
   Item w;
-  item_of(args, lane_id, &w);
+  item_of(args, Share{}, lane_id, &w);
   const LaJob& j = args.la.job[w.job];
   const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
   float* seg = args.seg_state + static_cast<int64_t>(lane_id) * args.nseg * 8192;
@@ -1177,14 +1243,24 @@ int64_t lanes_of(const LaArgs& a, int (&slices)[3], int64_t (&first)[4]) {
   return n;
 }
 
+int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total + a.nseq - 1) / (a.nseq > 0 ? a.nseq : 1); }
+
+// Even shares pay where whole lanes would leave many SMs idle: 192 lanes of 32 chunks on 148 SMs take 128 us, not
+// 146 (forward, 64 wide) and 213, not 244 (gradients, 128 wide).  They cost something themselves, as neighbouring
+// heads no longer read the same tokens at the same time: 576 lanes, which fill four rounds to 97%, 466, not 420.
+bool even_shares(const LaArgs& a, int64_t lanes, int sms) {
+  return a.cu == nullptr && a.T > kC && lanes > sms && (lanes + sms - 1) / sms * sms * 7 > lanes * 8;
+}
+
 // Segments per sequence that leave the shortest time, in units of one chunk
 // of the full pass (the state-only pass costs about 0.6 of it, the chaining and
 // the two extra launches about ten).
-int segments_for(int64_t lanes, int64_t tokens, int sms) {
-  const int64_t chunks = (tokens + kC - 1) / kC;
+int segments_for(const LaArgs& a, int64_t lanes, int sms) {
+  const int64_t chunks = (mean_tokens(a) + kC - 1) / kC;
   auto waves = [&](int64_t n) { return (n + sms - 1) / sms; };
   int best = 1;
-  double least = static_cast<double>(waves(lanes) * chunks);
+  double least = even_shares(a, lanes, sms) ? static_cast<double>(lanes * chunks) / sms + 1.0
+                                            : static_cast<double>(waves(lanes) * chunks);
   for (int s = 2; s <= 64 && s <= chunks; ++s) {
     const int64_t per = (chunks + s - 1) / s;
     const double t = static_cast<double>(waves(lanes * s) * per) + 0.6 * static_cast<double>(waves(lanes * (s - 1)) * per) + 10.0;
@@ -1196,8 +1272,6 @@ int segments_for(int64_t lanes, int64_t tokens, int sms) {
   return best;
 }
 
-int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total + a.nseq - 1) / (a.nseq > 0 ? a.nseq : 1); }
-
 }  // namespace
 
 namespace {
@@ -1205,12 +1279,17 @@ bool ordered(const LaArgs& a) { return a.cu != nullptr && a.nseq > 1 && a.nseq <
 size_t order_bytes(const LaArgs& a) { return ordered(a) ? (static_cast<size_t>(a.nseq) + 2 + 3) / 4 * 16 : 0; }
 }  // namespace
 
+namespace {
+size_t hand_bytes(int sms) { return static_cast<size_t>(sms) * (8192 * sizeof(float) + 4 * sizeof(int)); }
+}  // namespace
+
 size_t la_chunk_workspace(const LaArgs& a) {
   int slices[3];
   int64_t first[4];
   const int64_t lanes = lanes_of(a, slices, first);
-  const int nseg = segments_for(lanes, mean_tokens(a), device_sm_count());
-  return order_bytes(a) + (nseg == 1 ? 0 : static_cast<size_t>(lanes) * nseg * (8192 + 1) * sizeof(float));
+  const int nseg = segments_for(a, lanes, device_sm_count());
+  if (nseg == 1) return order_bytes(a) + (even_shares(a, lanes, device_sm_count()) ? hand_bytes(device_sm_count()) : 0);
+  return order_bytes(a) + static_cast<size_t>(lanes) * nseg * (8192 + 1) * sizeof(float);
 }
 
 int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t stream) {
@@ -1219,7 +1298,7 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
   const int64_t lanes = lanes_of(a, c.slices, first);
   if (lanes == 0) return SPX_OK;
   const int sms = device_sm_count();
-  c.nseg = segments_for(lanes, mean_tokens(a), sms);
+  c.nseg = segments_for(a, lanes, sms);
   if (lanes * c.nseg > 0x7FFFFFFF) return SPX_ERR_UNSUPPORTED;
   c.la = a;
   int dkb = 1;
@@ -1237,7 +1316,13 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
     }
   }
   for (int i = 0; i <= a.njobs; ++i) c.lanes[i] = static_cast<int>(first[i]);
-  if (workspace == nullptr && (c.nseg > 1 || ordered(a))) return SPX_ERR_WORKSPACE;
+  const bool even = c.nseg == 1 && even_shares(a, lanes, sms);
+  if (workspace == nullptr && (c.nseg > 1 || even || ordered(a))) return SPX_ERR_WORKSPACE;
+  if (even) {
+    c.hand = static_cast<float*>(workspace);
+    c.handed = reinterpret_cast<int*>(c.hand + static_cast<int64_t>(sms) * 8192);
+    if (cudaMemsetAsync(c.handed, 0, static_cast<size_t>(sms) * 4 * sizeof(int), stream) != cudaSuccess) return SPX_ERR_CUDA;
+  }
   if (ordered(a)) {
     int* const order = static_cast<int*>(workspace) + 2;
     c.order = order;

@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(kDgThreads) la_decay_grad_kernel(const LaDecay
 #pragma unroll
     for (int e = 0; e < kDgEach; ++e) {
       if (t0 - e < 0) continue;
-      const float r = static_cast<float>(before + v[e]);
+      // nothing decays into a first token that no state comes before: zero, not what rounding leaves of it
+      const float r = t0 - e == 0 && a.from_zero != 0 ? 0.0f : static_cast<float>(before + v[e]);
       const int64_t at = (start + t0 - e) * a.H + h;
       if (a.g_f32 != 0)
         reinterpret_cast<float*>(a.dg)[at] = r;

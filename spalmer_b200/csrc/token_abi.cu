@@ -404,6 +404,7 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   g.nseq = a.nseq;
   g.H = a.H;
   g.g_f32 = a.g_f32;
+  g.from_zero = initial_state == nullptr;
   if (int rc = launch_la_decay_grad(g, st); rc != SPX_OK) return rc;
   return SPX_OK;
 }

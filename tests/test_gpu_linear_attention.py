@@ -163,6 +163,28 @@ def test_packed_gradients(name, kv):
     _check_gradients(*_inputs(1, T, 4, kv, 64, 128, n=len(cu) - 1, init=True), cu=cu)
 
 
+# more sequences and heads than SMs, in numbers that whole ones do not fill: the kernel cuts some in two
+@pytest.mark.parametrize("B,T,H,kv,dk,dv", [(13, 300, 12, 6, 64, 64), (5, 700, 8, 8, 128, 128), (75, 129, 2, 2, 64, 32),
+                                            (41, 517, 4, 1, 40, 104)])
+def test_even_shares(B, T, H, kv, dk, dv):
+    q, k, v, a, state = _inputs(B, T, H, kv, dk, dv, init=True)
+    first = _check_forward(q, k, v, a, state)
+    again = _check_forward(q, k, v, a, state)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    _check_gradients(q, k, v, a, state)
+
+
+@pytest.mark.parametrize("T,cu", [(1, None), (5, None), (130, None), (9, [0, 1, 2, 6, 6, 9])])
+def test_first_token_has_no_decay_gradient(T, cu):
+    q, k, v, a, _ = _inputs(3 if cu is None else 1, T, 4, 2, 96, 128)
+    a = a.requires_grad_(True)
+    cut = None if cu is None else torch.tensor(cu, device=DEV, dtype=torch.int32)
+    out, last = linear_attention(q, k, v, a, cu_seqlens=cut, return_state=True)
+    (da,) = torch.autograd.grad([out, last], a, [torch.randn_like(out), torch.randn_like(last)])
+    first = [0] if cu is None else cu[:-1]
+    assert torch.all(da[:, first] == 0.0)
+
+
 def test_gradients_against_differences():
     """The last state is linear in k and v and smooth in the decays, and comes back in
     FP32; the output is linear in q: central differences of the operator itself."""
