@@ -19,7 +19,7 @@
 // so the statistics cost no second read; a CTA walks rows with a stride, which
 // keeps w in registers for all of them, and a row's loads are issued while the
 // row before is worked on (loads between the stores of one row went one after
-// another: 132 us instead of @FWD@ us for 65,536 rows of 768).  MXFP8: four
+// another: 132 us and not 66 for 65,536 rows of 768, 403 MB).  MXFP8: four
 // neighbouring lanes hold a block of 32, so its largest magnitude is two shuffles.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) add_norm_backward_kernel(cons
     }
   };
   int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
-  constexpr bool kAhead = NC <= 2;
+  constexpr bool kAhead = NC <= 3;
   if (kAhead) fetch(row);
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -372,21 +372,28 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ 
 
 namespace {
 
-// Threads of a row: up to two chunks a thread (registers for this row and the
+// Warps of a row: up to two chunks a thread (registers for this row and the
 // next), from one warp to sixteen; beyond that more chunks, loaded row by row.
-int norm_wpr(int d) {
+// (One chunk a thread and twice the warps: 51 and 64 us, not 44 and 49, forward and
+// backward over 2^25 elements in rows of 768.)  Where half of the warps hold the row
+// in three chunks, the backward of BF16 residuals takes those: 45 us, not 49,
+// as two chunks of two warps leave a quarter of the lanes idle.
+int norm_wpr(int d, bool three) {
   int wpr = 1;
   while (wpr < 16 && 32 * wpr * 2 < d / 8) wpr *= 2;
-  return wpr;
+  return three && wpr > 1 && 32 * (wpr / 2) * 3 >= d / 8 ? wpr / 2 : wpr;
 }
 
 // kernel(wpr, nc) as compile-time constants
-template <typename F>
+template <bool THREE, typename F>
 int with_shape(int d, F&& f) {
-  const int wpr = norm_wpr(d);
+  const int wpr = norm_wpr(d, THREE);
   const int nc = (d / 8 + 32 * wpr - 1) / (32 * wpr);
   using std::integral_constant;
   auto pick = [&](auto w) {
+    if constexpr (THREE && decltype(w)::value < 16) {
+      if (nc == 3) return f(w, integral_constant<int, 3>{});
+    }
     return nc <= 1 ? f(w, integral_constant<int, 1>{}) : f(w, integral_constant<int, 2>{});
   };
   switch (wpr) {
@@ -407,13 +414,13 @@ int norm_grid(int64_t rows, int wpr, int per_sm) {
 
 }  // namespace
 
-// Rows of partial dw sums that launch_add_norm_backward writes (d floats each).
-int add_norm_backward_parts(int64_t rows, int d) { return norm_grid(rows, norm_wpr(d), 1); }
+// Rows of partial dw sums that launch_add_norm_backward writes at most (d floats each).
+int add_norm_backward_parts(int64_t rows, int d) { return norm_grid(rows, norm_wpr(d, false), 1); }
 
 int launch_add_norm(const AddNormArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return SPX_OK;
-  const int grid = norm_grid(a.rows, norm_wpr(a.d), 2);
-  return with_shape(a.d, [&](auto w, auto n) {
+  const int grid = norm_grid(a.rows, norm_wpr(a.d, false), 2);
+  return with_shape<false>(a.d, [&](auto w, auto n) {
     constexpr int W = decltype(w)::value, N = decltype(n)::value;
     if (a.res == nullptr)
       add_norm_kernel<W, N, 0><<<grid, kNormThreads, 0, stream>>>(a);
@@ -430,13 +437,12 @@ int launch_add_norm_backward(const AddNormBackwardArgs& a, uint16_t* dw, cudaStr
     if (dw == nullptr) return SPX_OK;
     return cudaMemsetAsync(dw, 0, static_cast<size_t>(a.d) * 2, stream) == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
   }
-  const int grid = add_norm_backward_parts(a.rows, a.d);
-  const int rc = with_shape(a.d, [&](auto w, auto n) {
-    constexpr int W = decltype(w)::value, N = decltype(n)::value;
-    if (a.res_f32 == 0)
-      add_norm_backward_kernel<W, N, false><<<grid, kNormThreads, 0, stream>>>(a);
-    else
-      add_norm_backward_kernel<W, N, true><<<grid, kNormThreads, 0, stream>>>(a);
+  const int grid = norm_grid(a.rows, norm_wpr(a.d, a.res_f32 == 0), 1);
+  const int rc = a.res_f32 == 0 ? with_shape<true>(a.d, [&](auto w, auto n) {
+    add_norm_backward_kernel<decltype(w)::value, decltype(n)::value, false><<<grid, kNormThreads, 0, stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
+  }) : with_shape<false>(a.d, [&](auto w, auto n) {
+    add_norm_backward_kernel<decltype(w)::value, decltype(n)::value, true><<<grid, kNormThreads, 0, stream>>>(a);
     return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
   });
   if (rc != SPX_OK || dw == nullptr) return rc;
