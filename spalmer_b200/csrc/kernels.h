@@ -523,7 +523,7 @@ struct RotaryArgs {
 constexpr int kRotMaxD = 4096;
 int launch_rotary(RotaryArgs a, cudaStream_t stream);
 
-// Linear attention with a decay per head (linear_step.cu, linear_recurrent.cu).
+// Linear attention with a decay per head (linear_chunk.cu, linear_recurrent.cu, linear_step.cu).
 // One job computes, over each sequence and query head,
 //   out_i = scale * sum_j exp(decay between j and i) (a_i . b_j) c_j
 // over the j up to i (or, reverse, from i on), carrying a state [da][dc] =

@@ -10,16 +10,15 @@
 // one launch of three times the work and stores no states.
 //
 // A CTA walks its chunks in order for one (job, sequence, head, 64 columns of
-// C); the FP32 state stays in registers from chunk to chunk.  64 columns leave
-// room in shared memory to load the next chunk (two or three stages) and twice
-// as many CTAs at 128-wide heads; a . b is then computed once per 64 columns,
-// which the tensor cores have time for while HBM is the bound (at 128-wide
-// heads about 2,000 tensor cycles a chunk against 2,800 of memory time).
+// C), a "lane"; the FP32 state stays in registers from chunk to chunk.  64 columns
+// leave room in shared memory to load the next chunk (two or three stages) and give
+// twice as many CTAs at 128-wide heads; a . b is then computed once per 64 columns,
+// which the tensor cores have time for (they are busy for a quarter of it).
 //
 // Operand precision.  a, b, c are exact BF16.  What is not is split into BF16
 // parts that are multiplied one after another into the same FP32 accumulator:
-//   c scaled by its decay (into the state): three parts in the forward pass,
-//     whose state a caller keeps (2^-26), two in the gradients (2^-18);
+//   c scaled by its decay (into the state): three parts where a caller keeps the
+//     last state (exact), else two (2^-18);
 //   the decayed a . b matrix and the state (into out): one part in the forward
 //     pass, whose output is rounded to BF16 as coarsely, two in the gradients,
 //     because d decay is a long sum of q . dq - k . dk that cancels.
@@ -31,15 +30,28 @@
 // stay small are not differences of large ones, so that a token that forgets
 // everything costs its neighbours no digits.
 //
-// When (job, sequence, head, slice) fill too few SMs, the sequence is cut into
-// segments: a pass over b and c alone gives each segment's state from zero, a
-// small kernel chains them, and the full pass starts every segment from its
-// own first state.
+// How lanes meet SMs.  Too few lanes: the sequence is cut into segments; a pass
+// over b and c alone gives each segment's state from zero, a small kernel chains
+// them, and the full pass starts every segment from its own first state
+// (segments_for).  A few more lanes than SMs: even shares of chunks (even_shares).
+// Packed sequences: longest first from a queue (37 ragged prompts of 20,011 tokens
+// in all, 12 heads of 64: 83 us, in the order given and a fixed stride 115; with
+// the later steps 71).
+//
+// What bounds it: neither HBM nor the tensor cores, but instructions.  A chunk of
+// 64-wide heads takes about 3,600 cycles (gradients 4,300) in which four schedulers
+// issue 55% of the time and wait for instruction fetch in a quarter of the rest: a
+// dozen roles run at once, so that their code has to stay small, and unrolling or
+// prefetching more made every loop slower.  65,536 tokens of 12 heads of 64: forward
+// 121 us (403 MB, 3.3 TB/s), the three gradients 417 us.  8,190 tokens of 16 heads of
+// 128 over 4 shared ones: 85 and 203 us.
 //
 // Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
 // scaled c, 16-19 the state, 20-27 the epilogue, 28 and 31 TMA, 29 MMA, 30
 // decays.  One warp gets through an instruction every three or four cycles here,
-// so the longer roles have two warpgroups, and registers move between them.
+// so the longer roles have two warpgroups, and registers move between them.  (A
+// second MMA warp, a . b and its product apart from the state's, cost more
+// instructions than its shorter waits gave back: 173, not 154 us.)
 // Every wait is bounded (status word, then return).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -213,7 +225,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// mbar_wait that counts cycles instead of reading the timer: the kernel's 28
+// mbar_wait that counts cycles instead of reading the timer: the kernel's 32
 // warps run through a dozen loops at once, and what the instruction cache does
 // not hold is fetched again for every chunk, so its hot code has to stay small.
 // A wait that gives up leaves its code in shared memory; the CTA's end records it.
@@ -1254,7 +1266,8 @@ bool even_shares(const LaArgs& a, int64_t lanes, int sms) {
 
 // Segments per sequence that leave the shortest time, in units of one chunk
 // of the full pass (the state-only pass costs about 0.6 of it, the chaining and
-// the two extra launches about ten).
+// the two extra launches about ten).  One sequence of 65,536 tokens, 6 heads of 128:
+// 222 us in 12 segments, 1,363 in one piece.
 int segments_for(const LaArgs& a, int64_t lanes, int sms) {
   const int64_t chunks = (mean_tokens(a) + kC - 1) / kC;
   auto waves = [&](int64_t n) { return (n + sms - 1) / sms; };

