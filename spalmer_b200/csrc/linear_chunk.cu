@@ -702,9 +702,18 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       } else {
         const float* f = j.init + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.init != nullptr && args.nseg == 1 && live ? j.dc - col0 : 0;
+        if (j.s_col == 1) {  // a thread's columns side by side: widths are multiples of 8
 #pragma unroll
-        for (int c = 0; c < kN; ++c, f += 2 * j.s_col)  // widths are even
-          s[c] = 2 * c < n ? pair(j.init_scale * f[0], j.init_scale * f[j.s_col]) : 0;
+          for (int c = 0; c < kN; c += 2) {
+            const float4 v = 2 * c < n ? __ldg(reinterpret_cast<const float4*>(f + 2 * c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            s[c] = pair(j.init_scale * v.x, j.init_scale * v.y);
+            s[c + 1] = pair(j.init_scale * v.z, j.init_scale * v.w);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kN; ++c, f += 2 * j.s_col)
+            s[c] = 2 * c < n ? pair(j.init_scale * f[0], j.init_scale * f[j.s_col]) : 0;
+        }
       }
       float decay = 1.0f;
       auto write_operand = [&]() {  // BF16 parts of the state for the next chunk's a . S
@@ -768,13 +777,21 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
+        const bool wide = j.s_col == 1;
 #pragma unroll
-        for (int c = 0; c < kN; ++c, f += 2 * j.s_col) {
-          float v0, v1;
-          unpair(s[c], v0, v1);
-          if (2 * c < n) {
-            f[0] = j.fin_scale * v0;
-            f[j.s_col] = j.fin_scale * v1;
+        for (int c = 0; c < kN; c += 2, f += 4 * j.s_col) {
+          if (2 * c >= n) break;
+          float4 v;
+          unpair(s[c], v.x, v.y);
+          unpair(s[c + 1], v.z, v.w);
+          v = make_float4(j.fin_scale * v.x, j.fin_scale * v.y, j.fin_scale * v.z, j.fin_scale * v.w);
+          if (wide) {
+            *reinterpret_cast<float4*>(f) = v;
+          } else {
+            f[0] = v.x;
+            f[j.s_col] = v.y;
+            f[2 * j.s_col] = v.z;
+            f[3 * j.s_col] = v.w;
           }
         }
       }
@@ -927,22 +944,24 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
     // ---------------- TMA: a and b, and in a warp of its own c, whose tile is free later
     const bool ab = warp == 28;
     uint64_t* const full = ab ? bar.full_ab : bar.full_c;
-    auto fetch_item = [&]() {  // the next item: from the queue into its slot
-      const uint32_t slot = nitem & 3u;
-      if (lane == 0 && wait_for(&bar.qfree[slot], ((nitem >> 2) & 1u) ^ 1u, failed, SPX_DEV_TIMEOUT_PRODUCER)) {
-        const int got = atomicAdd(args.queue, 1);
-        bar.taken[slot] = got < items ? got : items;
-        mbar_arrive(&bar.qfull[slot]);
-      }
-      __syncwarp();
+    // The next item, from the queue into its place: at once if the place is free, and at the latest after this
+    // item's copies, which the roles that are to free it may be waiting for.
+    auto hand_out = [&](int got, bool wait) {
+      const uint32_t slot = nitem & 3u, parity = ((nitem >> 2) & 1u) ^ 1u;
+      if (!(wait ? wait_for(&bar.qfree[slot], parity, failed, SPX_DEV_TIMEOUT_PRODUCER) : mbar_test(&bar.qfree[slot], parity)))
+        return false;
+      bar.taken[slot] = got < items ? got : items;
+      mbar_arrive(&bar.qfull[slot]);
+      return true;
     };
     const bool queue = args.order != nullptr && !ab;
     int idx = item0;
     while (ok && idx < items) {
       Item w;
       item_of(args, bar.share, idx, &w);
-      if (queue) fetch_item();
       if (lane == 0) {
+        const int got = queue ? atomicAdd(args.queue, 1) : 0;
+        const bool handed = !queue || hand_out(got, false);
         const LaJob& j = args.la.job[w.job];
         const bool packed = args.la.cu != nullptr;
         const int batch = packed ? 0 : w.seq;
@@ -970,8 +989,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
             }
           }
         }
+        if (ok && !handed) ok = hand_out(got, true);
       }
       ok = __all_sync(0xFFFFFFFFu, ok) != 0;
+      __syncwarp();
       if (!queue) {
         idx = next_item(idx);
       } else {
@@ -1012,17 +1033,21 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       Item nw{};
       bool more = nidx < items;
       if (more) item_of(args, bar.share, nidx, &nw);
-      auto settle = [&]() {
+      // Looks for the item of the next chunk.  The queue frees a place only when every role is through with an older
+      // item, and they may wait for this warp's products: it waits for the queue only when it owes them none.
+      auto settle = [&](bool owing) {
         while (more && np >= nw.n) {
+          if (owing && args.order != nullptr &&
+              __all_sync(0xFFFFFFFFu, mbar_test(&bar.qfull[nitem & 3u], (nitem >> 2) & 1u)) == 0)
+            return;
           nidx = next_item(nidx);
           np = 0;
           if ((more = nidx < items)) item_of(args, bar.share, nidx, &nw);
         }
       };
-      settle();
       uint32_t ahead = 0;  // chunks whose a . b has been issued (state-only: whose tiles are there)
       auto start_next = [&](bool polled) {
-        if (!more) return true;
+        if (!more || np >= nw.n) return true;
         if (!wait_after(polled, &bar.full_ab[ast], aph, failed, SPX_DEV_TIMEOUT_MMA)) return false;
         // the tail of a packed sequence: its rows are zeroed first
         if (full_pass && args.la.cu != nullptr && nw.len - (nw.first + np * nw.step) < kC) {
@@ -1039,61 +1064,67 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           ast = 0;
           aph ^= 1u;
         }
-        settle();
-        return ok;
+        return true;
       };
-      ok = start_next(false);
-      bool kv_ready = false;
-      while (ok && it < ahead) {
+      bool kv_ready = false, qs_ready = false, ab_ready = false, pop_ready = false;
+      while (ok) {
+        const bool owing = it < ahead;
         const uint32_t b = it & 1u, ph2 = (it >> 1) & 1u;
         const uint32_t stage = base + st * K::kStage;
-        // A satisfied wait still takes a few hundred cycles of a busy CTA: each is polled one product ahead.
-        // state product b^T (scaled c)
-        if (!(ok = wait_after(kv_ready, &bar.kvgo[b], ph2, failed, SPX_DEV_TIMEOUT_MMA))) break;
-        tc_fence_after();
-        const bool qs_ready = full_pass && mbar_test(&bar.qsgo, it & 1u);
-        const bool ab_ready = mbar_test(&bar.full_ab[ast], aph);
-        const uint64_t db = desc_mn(stage + DKB * kTile, DKB == 1 ? 0u : kTile);  // 64 columns: the same rows twice
-        uint64_t dv[K::kParts];  // (two parts: the first, with the distance to the second)
-#pragma unroll
-        for (uint32_t part = 0; part < K::kParts; ++part) dv[part] = desc_mn(part_at(it, part), part_at(it, 1) - part_at(it, 0));
-        const uint32_t acc = tmem + acc_at(it);
-        if (elect_one()) {
-#pragma unroll
-          for (uint32_t q = 0; q < 8; ++q) {
-            // two parts side by side are one MMA of 128 columns, which reads b once; three go one after another
-            // into the same 64 (MMAs of different shapes on one accumulator have no order)
-#pragma unroll
-            for (uint32_t part = 0; part < (K::kParts == 3 ? 3u : 1u); ++part)
-              mma_bf16_ss(acc, db + q * 128u, dv[part] + q * 128u, id_kv, (part | q) != 0u ? 1u : 0u);
-          }
-          mma_commit(&bar.kv[b]);
-          mma_commit(&bar.empty_b[st]);  // a . b of this chunk was issued before
-          if (!full_pass) mma_commit(&bar.empty_c[st]);
-        }
-        __syncwarp();
-        bool pop_ready = false;
-        if (full_pass) {
-          // a . S
-          if (!(ok = wait_after(qs_ready, &bar.qsgo, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+        if (owing) {
+          // A satisfied wait still takes a few hundred cycles of a busy CTA: each is polled one product ahead.
+          // state product b^T (scaled c)
+          if (!(ok = wait_after(kv_ready, &bar.kvgo[b], ph2, failed, SPX_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
-          pop_ready = mbar_test(&bar.pop[b], ph2);
-          const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
+          qs_ready = full_pass && mbar_test(&bar.qsgo, it & 1u);
+          ab_ready = mbar_test(&bar.full_ab[ast], aph);
+          const uint64_t db = desc_mn(stage + DKB * kTile, DKB == 1 ? 0u : kTile);  // 64 columns: the same rows twice
+          uint64_t dv[K::kParts];  // (two parts: the first, with the distance to the second)
+#pragma unroll
+          for (uint32_t part = 0; part < K::kParts; ++part) dv[part] = desc_mn(part_at(it, part), part_at(it, 1) - part_at(it, 0));
+          const uint32_t acc = tmem + acc_at(it);
           if (elect_one()) {
 #pragma unroll
-            for (uint32_t n = 0; n < 4 * DKB; ++n) {
+            for (uint32_t q = 0; q < 8; ++q) {
+              // two parts side by side are one MMA of 128 columns, which reads b once; three go one after another
+              // into the same 64 (MMAs of different shapes on one accumulator have no order)
 #pragma unroll
-              for (uint32_t part = 0; part < K::kSParts; ++part)
-                mma_bf16_ss(tmem + kTmOX, da + (((n >> 2) * kTile + (n & 3u) * 32u) >> 4),
-                            ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
+              for (uint32_t part = 0; part < (K::kParts == 3 ? 3u : 1u); ++part)
+                mma_bf16_ss(acc, db + q * 128u, dv[part] + q * 128u, id_kv, (part | q) != 0u ? 1u : 0u);
             }
-            mma_commit(&bar.qs);
-            mma_commit(&bar.empty_a[st]);
+            mma_commit(&bar.kv[b]);
+            mma_commit(&bar.empty_b[st]);  // a . b of this chunk was issued before
+            if (!full_pass) mma_commit(&bar.empty_c[st]);
           }
           __syncwarp();
+          if (full_pass) {
+            // a . S
+            if (!(ok = wait_after(qs_ready, &bar.qsgo, it & 1u, failed, SPX_DEV_TIMEOUT_MMA))) break;
+            tc_fence_after();
+            pop_ready = mbar_test(&bar.pop[b], ph2);
+            const uint64_t da = desc_kmajor_sw128(stage), ds = desc_mn(base + K::kOffS, kTile);
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t n = 0; n < 4 * DKB; ++n) {
+#pragma unroll
+                for (uint32_t part = 0; part < K::kSParts; ++part)
+                  mma_bf16_ss(tmem + kTmOX, da + (((n >> 2) * kTile + (n & 3u) * 32u) >> 4),
+                              ds + (part * (K::kSTile >> 4) + n * 128u), id_o, (part | n) != 0u ? 1u : 0u);
+              }
+              mma_commit(&bar.qs);
+              mma_commit(&bar.empty_a[st]);
+            }
+            __syncwarp();
+          }
         }
-        if (!(ok = start_next(ab_ready))) break;
+        settle(owing);
+        if (!(ok = ok && start_next(ab_ready))) break;
         kv_ready = mbar_test(&bar.kvgo[b ^ 1u], ((it + 1) >> 1) & 1u);
+        if (!owing) {
+          if (it == ahead) break;  // there is no next one
+          kv_ready = false;
+          continue;
+        }
         if (full_pass) {
           // (decayed a . b) c
           if (!(ok = wait_after(pop_ready, &bar.pop[b], ph2, failed, SPX_DEV_TIMEOUT_MMA))) break;

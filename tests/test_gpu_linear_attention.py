@@ -174,6 +174,25 @@ def test_even_shares(B, T, H, kv, dk, dv):
     _check_gradients(q, k, v, a, state)
 
 
+# every CTA takes many short and empty sequences one after another
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 72)])
+@pytest.mark.parametrize("lengths", [(0, 0, 0, 1, 2, 5, 40, 129, 300), (0, 0, 0, 0, 0, 0, 0, 1), (0, 3), (1, 2)])
+def test_packed_short_and_empty(lengths, dk, dv):
+    g = torch.Generator().manual_seed(dk + len(lengths))
+    lens = [lengths[i] for i in torch.randint(len(lengths), (300,), generator=g).tolist()]
+    cu = [0] + torch.tensor(lens).cumsum(0).tolist()
+    q, k, v, a, state = _inputs(1, cu[-1], 4, 2, dk, dv, n=len(lens), init=True)
+    for _ in range(3):
+        _check_forward(q, k, v, a, state, cu=cu)
+    _check_gradients(q, k, v, a, state, cu=cu)
+
+
+@pytest.mark.parametrize("cu", [[0, 9000, 9000, 9000, 9000, 9003, 9003], [0, 0, 0, 0, 0, 7000]])
+def test_packed_long_among_empty(cu):
+    q, k, v, a, state = _inputs(1, cu[-1], 2, 2, 64, 64, n=len(cu) - 1, init=True)
+    _check_forward(q, k, v, a, state, cu=cu)
+
+
 @pytest.mark.parametrize("T,cu", [(1, None), (5, None), (130, None), (9, [0, 1, 2, 6, 6, 9])])
 def test_first_token_has_no_decay_gradient(T, cu):
     q, k, v, a, _ = _inputs(3 if cu is None else 1, T, 4, 2, 96, 128)
