@@ -1290,9 +1290,10 @@ int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total +
 
 // Even shares pay where whole lanes would leave many SMs idle: 192 lanes of 32 chunks on 148 SMs take 128 us, not
 // 146 (forward, 64 wide) and 213, not 244 (gradients, 128 wide).  They cost something themselves, as neighbouring
-// heads no longer read the same tokens at the same time: 576 lanes, which fill four rounds to 97%, 466, not 420.
+// heads no longer read the same tokens at the same time: 576 lanes, which fill four rounds to 97%, 466, not 420.  So a
+// sixth of the rounds has to be idle.
 bool even_shares(const LaArgs& a, int64_t lanes, int sms) {
-  return a.cu == nullptr && a.T > kC && lanes > sms && (lanes + sms - 1) / sms * sms * 7 > lanes * 8;
+  return a.cu == nullptr && a.T > kC && lanes > sms && (lanes + sms - 1) / sms * sms * 5 > lanes * 6;
 }
 
 // Segments per sequence that leave the shortest time, in units of one chunk
