@@ -16,7 +16,7 @@
 //
 // The pass is bound by HBM: each tensor is read or written once (65,536 rows of
 // 768, BF16: forward 65 us, 6.2 TB/s; backward 75 us, 5.4 TB/s; 16,387 rows of 2,048
-// to MXFP8 with an FP32 sum, 370 MB: 62 us, 6.0 TB/s).  A row is
+// to MXFP8 with an FP32 sum, 370 MB: 65 us, 5.7 TB/s).  A row is
 // held in the registers of 32 * WPR threads (NC chunks of eight elements each),
 // so the statistics cost no second read; a CTA walks rows with a stride, which
 // keeps w in registers for all of them, and a row's loads are issued while the
@@ -92,11 +92,11 @@ __device__ __forceinline__ void store8(void* base, int64_t at, bool f32, const f
   }
 }
 
-// Sum of `n` floats over the 32 * WPR threads of a row.  `part` holds
+// Sums over the 32 * WPR threads of a row.  `part` holds
 // [2][rows per CTA][WPR][n]; the two halves alternate from row to row, so one
 // barrier a row is enough.
-template <int WPR, int N>
-__device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, int wr, int lane, uint32_t turn) {
+template <int WPR, int N, typename T>
+__device__ __forceinline__ void row_sum(T (&s)[N], T* part, int group, int wr, int lane, uint32_t turn) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) {
 #pragma unroll
@@ -104,7 +104,7 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, i
   }
   if constexpr (WPR > 1) {
     constexpr int kGroups = kNormThreads / (32 * WPR);
-    float* p = part + ((turn & 1u) * kGroups + group) * WPR * N;
+    T* p = part + ((turn & 1u) * kGroups + group) * WPR * N;
     if (lane == 0) {
 #pragma unroll
       for (int j = 0; j < N; ++j) p[wr * N + j] = s[j];
@@ -113,7 +113,7 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, i
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * WPR) : "memory");
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      float t = 0.0f;
+      T t = 0;
 #pragma unroll
       for (int w = 0; w < WPR; ++w) t += p[w * N + j];
       s[j] = t;
@@ -123,8 +123,11 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* part, int group, i
 
 }  // namespace
 
-// RES: 0 no residual, 1 BF16, 2 FP32.
-template <int WPR, int NC, int RES>
+// RES: 0 no residual, 1 BF16, 2 FP32.  MX: MXFP8 rows out.  A value that is to become
+// E4M3 lies near a rounding border or not, and each bit of FP32 that y loses moves
+// twice as many across; so there 1 / sqrt and the two products keep their remainders
+// (16,387 rows of 2,048: 65 us, without 62).
+template <int WPR, int NC, int RES, bool MX>
 __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNormArgs a) {
   constexpr int kGroups = kNormThreads / (32 * WPR);
   __shared__ float part[2 * kGroups * WPR];
@@ -180,8 +183,10 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
       }
+      float sq = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] = fmaf(h[i][j], h[i][j], s[0]);
+      for (int j = 0; j < 8; ++j) sq = fmaf(h[i][j], h[i][j], sq);
+      s[0] += sq;
     }
     if (kAhead) fetch(row + step);
     if constexpr (RES != 0) {
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
       }
     }
     row_sum<WPR, 1>(s, part, group, wr, lane, turn);
-    const float r = 1.0f / sqrtf(s[0] * inv_d + a.eps);
+    const float ms = s[0] * inv_d + a.eps, r = 1.0f / sqrtf(ms);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = (i * WPR + wr) * 32 + lane;
@@ -202,7 +207,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = h[i][j] * r * wf[j];
       if (a.y != nullptr && in) store8(a.y, row * a.d + c * 8, false, y);
-      if (a.mx_values != nullptr) {
+      if constexpr (MX) {
+        // what r lacks: 1 / sqrt(ms) = r (1 + e / 2), e = 1 - ms r^2
+        const float mr = ms * r, r_rest = 0.5f * r * (fmaf(-mr, r, 1.0f) - fmaf(ms, r, -mr) * r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float p = h[i][j] * r;
+          y[j] += fmaf(fmaf(h[i][j], r_rest, fmaf(h[i][j], r, -p)), wf[j], fmaf(p, wf[j], -y[j]));
+        }
         // blocks of 32 = four lanes; all lanes take part in the shuffles (d % 32 == 0, so a block is wholly in or out)
         float amax = 0.0f;
 #pragma unroll
@@ -424,12 +436,19 @@ int launch_add_norm(const AddNormArgs& a, cudaStream_t stream) {
   const int grid = norm_grid(a.rows, norm_wpr(a.d, false), 2);
   return with_shape<false>(a.d, [&](auto w, auto n) {
     constexpr int W = decltype(w)::value, N = decltype(n)::value;
-    if (a.res == nullptr)
-      add_norm_kernel<W, N, 0><<<grid, kNormThreads, 0, stream>>>(a);
-    else if (a.res_f32 == 0)
-      add_norm_kernel<W, N, 1><<<grid, kNormThreads, 0, stream>>>(a);
+    auto run = [&](auto mx) {
+      constexpr bool MX = decltype(mx)::value;
+      if (a.res == nullptr)
+        add_norm_kernel<W, N, 0, MX><<<grid, kNormThreads, 0, stream>>>(a);
+      else if (a.res_f32 == 0)
+        add_norm_kernel<W, N, 1, MX><<<grid, kNormThreads, 0, stream>>>(a);
+      else
+        add_norm_kernel<W, N, 2, MX><<<grid, kNormThreads, 0, stream>>>(a);
+    };
+    if (a.mx_values != nullptr)
+      run(std::true_type{});
     else
-      add_norm_kernel<W, N, 2><<<grid, kNormThreads, 0, stream>>>(a);
+      run(std::false_type{});
     return cudaGetLastError() == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
   });
 }

@@ -36,15 +36,15 @@
 // (segments_for).  A few more lanes than SMs: even shares of chunks (even_shares).
 // Packed sequences: longest first from a queue (37 ragged prompts of 20,011 tokens
 // in all, 12 heads of 64: 83 us, in the order given and a fixed stride 115; with
-// the later steps 71).
+// the later steps 72).
 //
 // What bounds it: neither HBM nor the tensor cores, but instructions.  A chunk of
 // 64-wide heads takes about 3,600 cycles (gradients 4,300) in which four schedulers
 // issue 55% of the time and wait for instruction fetch in a quarter of the rest: a
 // dozen roles run at once, so that their code has to stay small, and unrolling or
 // prefetching more made every loop slower.  65,536 tokens of 12 heads of 64: forward
-// 121 us (403 MB, 3.3 TB/s), the three gradients 417 us.  8,190 tokens of 16 heads of
-// 128 over 4 shared ones: 85 and 203 us.
+// 140 us (403 MB, 2.9 TB/s), the three gradients 424 us.  8,190 tokens of 16 heads of
+// 128 over 4 shared ones: 87 and 211 us.
 //
 // Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
 // scaled c, 16-19 the state, 20-27 the epilogue, 28 and 31 TMA, 29 MMA, 30
@@ -1299,7 +1299,7 @@ bool even_shares(const LaArgs& a, int64_t lanes, int sms) {
 // Segments per sequence that leave the shortest time, in units of one chunk
 // of the full pass (the state-only pass costs about 0.6 of it, the chaining and
 // the two extra launches about ten).  One sequence of 65,536 tokens, 6 heads of 128:
-// 222 us in 12 segments, 1,363 in one piece.
+// 233 us in 12 segments, 1,363 in one piece.
 int segments_for(const LaArgs& a, int64_t lanes, int sms) {
   const int64_t chunks = (mean_tokens(a) + kC - 1) / kC;
   auto waves = [&](int64_t n) { return (n + sms - 1) / sms; };
