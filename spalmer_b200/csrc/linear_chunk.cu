@@ -1288,8 +1288,8 @@ int64_t lanes_of(const LaArgs& a, int (&slices)[3], int64_t (&first)[4]) {
 
 int64_t mean_tokens(const LaArgs& a) { return a.cu == nullptr ? a.T : (a.total + a.nseq - 1) / (a.nseq > 0 ? a.nseq : 1); }
 
-// Even shares pay where whole lanes would leave many SMs idle: 192 lanes of 32 chunks on 148 SMs take 128 us, not
-// 146 (forward, 64 wide) and 213, not 244 (gradients, 128 wide).  They cost something themselves, as neighbouring
+// Even shares pay where whole lanes would leave many SMs idle: 192 lanes of 32 chunks on 148 SMs take 143 us, not
+// 166 (forward, 64 wide), and 218, not 254 (gradients, 128 wide).  They cost something themselves, as neighbouring
 // heads no longer read the same tokens at the same time: 576 lanes, which fill four rounds to 97%, 466, not 420.  So a
 // sixth of the rounds has to be idle.
 bool even_shares(const LaArgs& a, int64_t lanes, int sms) {
