@@ -633,13 +633,14 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
         const uint32_t stage = base + st * K::kStage;
         const uint32_t sc_row = stage + 2 * DKB * kTile + swz(row, 0);  // ^ (c << 4): the row's chunk c
         if (len < kC && args.la.cu != nullptr) {
-          // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum
+          // packed: the rows past the sequence are another's (or nobody's); nothing of them may enter a sum.  A thread
+          // zeroes the chunks of c that it scales below: the row's other half is another warp's.
           if (!(ok = warp_wait(&bar.full_ab[st], ph, failed, SPX_DEV_TIMEOUT_EPILOGUE))) break;
           if (row >= len) {
 #pragma unroll
             for (int x = 0; x < DKB + 1; ++x)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) sts16(stage + (DKB + x) * kTile + row * 128 + (4 * half + c) * 16, 0u, 0u, 0u, 0u);
+              for (int c = 0; c < 4; ++c) sts16(stage + (DKB + x) * kTile + swz(row, 4 * half + c), 0u, 0u, 0u, 0u);
           }
           fence_proxy_async_smem();
           if (full_pass) warp_arrive(&bar.tail[tails++ & 1u], lane);  // else the product alone reads them, after vp
