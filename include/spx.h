@@ -601,9 +601,11 @@ int spx_rotary(const spx_heads* q, int32_t q_heads, const spx_heads* k, int32_t 
  * a factor below 2^-126 is zero.  Query head h uses key/value head
  * h / (heads / kv_heads).  packed = 0: `batch` sequences of seq_len tokens;
  * packed = 1: one batch row of seq_len tokens in all, cut into `batch`
- * sequences by cu_seqlens (int32 [batch + 1] on the device, from 0 to
+ * sequences by cu_seqlens (int32 [batch + 1] on the device, within 0 and
  * seq_len, not decreasing; an entry that is not is recorded in *status and
- * its sequence skipped).  States are FP32 [batch, heads, key_dim, value_dim].
+ * its sequence taken as empty, so that its last state is its first).  Tokens
+ * of no sequence, as those that pad a row, have zero outputs and gradients.
+ * States are FP32 [batch, heads, key_dim, value_dim].
  * key_dim and value_dim: multiples of 8 up to 128; heads 16-byte aligned.
  * status: device int, zero before the first call (NULL = not recorded);
  * workspace 16-byte aligned, not initialised, sized by the functions below. */

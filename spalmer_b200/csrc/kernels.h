@@ -552,6 +552,7 @@ struct LaArgs {
   int64_t g_sb, g_st, g_sh;
   const int32_t* cu;       // [nseq + 1] packed sequences | null
   int64_t T, total;        // tokens of a sequence (unpacked), tokens in all
+  void* dg;                // packed: [total][H] in g's type, whose rows outside every sequence are zeroed too | null
   int njobs, nseq, H, g_f32;
   float scale;
   int* status;

@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
       const bool sound = item_of(args, bar.share, idx, &w);
       if (args.hand != nullptr && w.n == 0) continue;
       const LaJob& j = args.la.job[w.job];
-      if (!sound && threadIdx.x == 512) *failed = SPX_DEV_BAD_TILE;
+      if (!sound && threadIdx.x == 512) *failed = SPX_DEV_BAD_TILE;  // and it counts as an empty sequence
       uint64_t s[kN];
       const int64_t st0 = (static_cast<int64_t>(w.seq) * args.la.H + w.h) * j.da * j.dc;
       const int col0 = w.slice * 64 + part_col;
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) atomicExch(args.handed + blockIdx.x * 4 + quad, 1);
         } else if (threadIdx.x == 512) args.seg_decay[static_cast<int64_t>(w.lane) * args.nseg + w.seg] = decay;
-      } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live && sound) {
+      } else if (j.fin != nullptr && w.seg == args.nseg - 1 && live) {
         float* f = j.fin + st0 + row * j.s_row + col0 * j.s_col;
         const int n = j.dc - col0;
         const bool wide = j.s_col == 1;
@@ -1221,15 +1221,38 @@ __global__ void __launch_bounds__(kLaThreads, 1) la_chunk_kernel(const __grid_co
   }
 }
 
-// The sequences by their number of chunks, longest first (ties by index), and
-// the queue's start: a rank is the count of those that come before.
-__global__ void __launch_bounds__(1024) la_order_kernel(const int32_t* __restrict__ cu, int n, int64_t total,
-                                                        int* __restrict__ order, int* __restrict__ queue, int first_state,
-                                                        int first_full) {
+// What packed sequences need first.  The last block sorts them by their number of
+// chunks, longest first (ties by index): a rank is the count of those that come
+// before; and sets the queue's start.  The others zero the rows of the outputs that no
+// sequence holds, which nobody else writes: with sound offsets those before the first
+// and after the last, else all of them, before the sound sequences write theirs.
+__global__ void __launch_bounds__(1024) la_prepare_kernel(const __grid_constant__ LaArgs a, int* __restrict__ order,
+                                                          int* __restrict__ queue, int first_state, int first_full) {
   __shared__ int chunks[kOrderMax];
+  const int n = a.nseq;
+  if (blockIdx.x + 1 < gridDim.x) {
+    bool sound = true;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int lo = a.cu[i], hi = a.cu[i + 1];
+      sound = sound && lo >= 0 && hi >= lo && hi <= a.total;
+    }
+    sound = __syncthreads_and(sound) != 0;
+    const int64_t lo = sound ? a.cu[0] : a.total, hi = sound ? a.cu[n] : a.total;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x - 1) * blockDim.x;
+    auto zero = [&](auto* p, int64_t row) {  // elements of a token's row
+      for (int64_t i = at; i < lo * row; i += step) p[i] = {};
+      for (int64_t i = hi * row + at; i < a.total * row; i += step) p[i] = {};
+    };
+    for (int j = 0; j < a.njobs; ++j)  // rows are multiples of 16 bytes
+      zero(static_cast<uint4*>(a.job[j].out), static_cast<int64_t>(a.H) * a.job[j].dc / (a.job[j].out_f32 != 0 ? 4 : 8));
+    if (a.dg != nullptr) zero(static_cast<uint16_t*>(a.dg), static_cast<int64_t>(a.H) * (a.g_f32 != 0 ? 2 : 1));
+    return;
+  }
+  if (order == nullptr) return;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int lo = cu[i], hi = cu[i + 1];
-    chunks[i] = lo >= 0 && hi >= lo && hi <= total ? (hi - lo + kC - 1) / kC : 0;
+    const int lo = a.cu[i], hi = a.cu[i + 1];
+    chunks[i] = lo >= 0 && hi >= lo && hi <= a.total ? (hi - lo + kC - 1) / kC : 0;
   }
   if (threadIdx.x == 0) {  // each pass has its own, behind the items that its CTAs start with
     queue[0] = first_state;
@@ -1369,14 +1392,13 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
     c.handed = reinterpret_cast<int*>(c.hand + static_cast<int64_t>(sms) * 8192);
     if (cudaMemsetAsync(c.handed, 0, static_cast<size_t>(sms) * 4 * sizeof(int), stream) != cudaSuccess) return SPX_ERR_CUDA;
   }
-  if (ordered(a)) {
-    int* const order = static_cast<int*>(workspace) + 2;
+  if (a.cu != nullptr) {
+    int* const order = ordered(a) ? static_cast<int*>(workspace) + 2 : nullptr;
     c.order = order;
-    c.queue = order - 2;
+    c.queue = order != nullptr ? order - 2 : nullptr;
     const int state_ctas = static_cast<int>(std::min<int64_t>(lanes * (c.nseg - 1), sms));
     const int full_ctas = static_cast<int>(std::min<int64_t>(lanes * c.nseg, sms));
-    la_order_kernel<<<1, a.nseq < 1024 ? (a.nseq + 31) / 32 * 32 : 1024, 0, stream>>>(a.cu, a.nseq, a.total, order, c.queue,
-                                                                                     state_ctas, full_ctas);
+    la_prepare_kernel<<<sms, 1024, 0, stream>>>(a, order, c.queue, state_ctas, full_ctas);
     if (cudaGetLastError() != cudaSuccess) return SPX_ERR_CUDA;
   }
   if (c.nseg > 1) {

@@ -33,6 +33,13 @@ int check_dims(const spx_linattn_dims* d) {
 
 int64_t total_tokens(const spx_linattn_dims& d) { return d.packed != 0 ? d.seq_len : d.batch * d.seq_len; }
 
+// An output of tokens that belong to no sequence.
+int zero_rows(void* p, size_t bytes, cudaStream_t stream) {
+  if (bytes == 0) return SPX_OK;
+  if (p == nullptr) return SPX_ERR_INVALID_ARG;
+  return cudaMemsetAsync(p, 0, bytes, stream) == cudaSuccess ? SPX_OK : SPX_ERR_CUDA;
+}
+
 // Pointer, alignment and strides; the stride of a dimension of one element is not used.
 int check_heads(const spx_heads* t, int64_t batch, int64_t tokens, int64_t heads) {
   if (t == nullptr || t->ptr == nullptr) return SPX_ERR_INVALID_ARG;
@@ -258,7 +265,10 @@ int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const
                          void* stream) {
   if (int rc = check_dims(dims); rc != SPX_OK) return rc;
   const spx_linattn_dims& d = *dims;
-  if (d.batch == 0) return SPX_OK;
+  if (d.batch == 0) {
+    const size_t n = static_cast<size_t>(total_tokens(d)) * d.heads;
+    return zero_rows(out, n * d.value_dim * 2, as_stream(stream));
+  }
   if (d.packed != 0 && cu_seqlens == nullptr) return SPX_ERR_INVALID_ARG;
   if (total_tokens(d) > 0) {
     if (int rc = check_sequences(d, q, k, v, nullptr); rc != SPX_OK) return rc;
@@ -300,9 +310,16 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
                                   void* workspace, size_t workspace_bytes, int* status, void* stream) {
   if (int rc = check_dims(dims); rc != SPX_OK) return rc;
   const spx_linattn_dims& d = *dims;
-  if (d.batch == 0) return SPX_OK;
-  if (d.packed != 0 && cu_seqlens == nullptr) return SPX_ERR_INVALID_ARG;
   const int64_t total = total_tokens(d);
+  if (d.batch == 0) {
+    const size_t n = static_cast<size_t>(total), h = d.heads, kv = d.kv_heads;
+    const cudaStream_t st = as_stream(stream);
+    if (int rc = zero_rows(d_q, n * h * d.key_dim * 2, st); rc != SPX_OK) return rc;
+    if (int rc = zero_rows(d_k, n * kv * d.key_dim * 2, st); rc != SPX_OK) return rc;
+    if (int rc = zero_rows(d_v, n * kv * d.value_dim * 2, st); rc != SPX_OK) return rc;
+    return zero_rows(d_decay, n * h * (d.decay_f32 != 0 ? 4 : 2), st);
+  }
+  if (d.packed != 0 && cu_seqlens == nullptr) return SPX_ERR_INVALID_ARG;
   if (total > 0) {
     if (d_out == nullptr) return SPX_ERR_INVALID_ARG;
     if (int rc = check_sequences(d, q, k, v, d_out); rc != SPX_OK) return rc;
@@ -322,6 +339,7 @@ int spx_linear_attention_backward(const spx_linattn_dims* dims, const spx_heads*
   const cudaStream_t st = as_stream(stream);
   LaArgs a = base_args(d, decays, cu_seqlens, status);
   a.njobs = 3;
+  a.dg = d_decay;
   // d q_i = scale sum_{j <= i} w_ij (d out_i . v_j) k_j: the forward's sum on (d out, v, k), state transposed
   LaJob& jq = a.job[0];
   jq.a = operand(d_out, 1);

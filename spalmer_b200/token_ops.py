@@ -448,9 +448,10 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scal
     h reads head ``h // (heads // kv_heads)``), ``log_decay`` [B, T, heads]
     FP32 or BF16, natural logarithms meant to be <= 0.  Head dimensions are
     multiples of 8 up to 128; ``scale`` defaults to ``key_dim ** -0.5``.
-    ``cu_seqlens`` (int32 [n + 1], from 0 to T, B = 1) packs n sequences into
-    one row; an entry that is out of order skips its sequence and shows in
-    ``linear_attention_status``.  ``initial_state`` and the returned last state
+    ``cu_seqlens`` (int32 [n + 1], within 0 and T, B = 1) packs n sequences into
+    one row; tokens before the first offset or after the last (a row padded to a
+    fixed length, say) have zero outputs and gradients.  An entry that is out of
+    order makes its sequence an empty one and shows in ``linear_attention_status``.  ``initial_state`` and the returned last state
     are FP32 [B or n, heads, key_dim, value_dim].  Nothing passes from one
     sequence to another, non-finite values included.
 

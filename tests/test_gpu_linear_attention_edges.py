@@ -63,3 +63,74 @@ def test_non_finite_neighbours_at_every_tail(kind, H, kv, dk, dv, bad):
         assert torch.isfinite(x[:, here].float()).all() and torch.equal(x[:, here], y[:, here])
     for x, y in zip(states, states2):
         assert torch.isfinite(x[::2]).all() and torch.equal(x[::2], y[::2])
+
+
+@pytest.fixture
+def dirty(monkeypatch):
+    """torch.empty and empty_like hand out memory that somebody else has left NaN in."""
+
+    def spoilt(make):
+        def made(*args, **kw):
+            t = make(*args, **kw)
+            return t.fill_(255 if t.dtype == torch.uint8 else math.nan) if t.is_cuda else t
+        return made
+
+    for name in ("empty", "empty_like"):
+        monkeypatch.setattr(torch, name, spoilt(getattr(torch, name)))
+
+
+def _train(q, k, v, a, state, cu, do, ds):
+    ins = [t.detach().clone().requires_grad_(True) for t in (q, k, v, a, state)]
+    out, last = linear_attention(*ins[:4], initial_state=ins[4], return_state=True,
+                                 cu_seqlens=torch.tensor(cu, device=DEV, dtype=torch.int32))
+    dq, dk, dv, da, d_state = torch.autograd.grad((out, last), ins, (do, ds), allow_unused=True)
+    return (out.detach(), dq, dk, dv, da), (last.detach(), d_state)
+
+
+@pytest.mark.parametrize("decay", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,kv,dk,dv", [(3, 3, 64, 64), (4, 2, 128, 72)])
+@pytest.mark.parametrize("T,cu", [(400, [5, 70, 70, 300]), (300, [10, 200]), (300, [0, 300]), (64, [64, 64]), (40, [7]),
+                                  (5003, list(range(1, 5001)))])
+def test_tokens_of_no_sequence(dirty, T, cu, H, kv, dk, dv, decay):
+    """Rows that a packed call does not cover are zero, gradients too; the others are those of the row cut to them."""
+
+    n = len(cu) - 1
+    q, k, v, a, state = _inputs(1, T, H, kv, dk, dv, n=n or 1, init=True, decay=decay)
+    state = state[:n]
+    g = torch.Generator(device=DEV).manual_seed(3)
+    do = torch.randn(1, T, H, dv, generator=g, device=DEV).to(torch.bfloat16)
+    ds = torch.randn(n, H, dk, dv, generator=g, device=DEV)
+    rows, states = _train(q, k, v, a, state, cu, do, ds)
+    assert linear_attention_status() == 0
+    lo, hi = cu[0], cu[-1]
+    for x in rows:
+        assert not x[:, :lo].any() and not x[:, hi:].any()
+    if hi > lo:
+        cut = [t[:, lo:hi] for t in (q, k, v, a)]
+        want_rows, want_states = _train(*cut, state, [c - lo for c in cu], do[:, lo:hi], ds)
+        for x, y in zip((*(x[:, lo:hi] for x in rows), *states), (*want_rows, *want_states)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("with_state", [True, False])
+@pytest.mark.parametrize("H,kv", [(2, 2), (4, 1)])
+def test_unsound_sequences_are_empty_ones(dirty, H, kv, with_state):
+    """Sequence 1 runs backwards, sequence 3 past the end: their states pass through, their rows are zero."""
+
+    cu = [0, 100, 50, 200, 400]
+    q, k, v, a, state = _inputs(1, 300, H, kv, 64, 64, n=4, init=True)
+    cut = torch.tensor(cu, device=DEV, dtype=torch.int32)
+    ins = [t.requires_grad_(True) for t in (q, k, v, a)] + ([state.requires_grad_(True)] if with_state else [])
+    out, last = linear_attention(*ins[:4], initial_state=state if with_state else None, cu_seqlens=cut, return_state=True)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    do = torch.randn(out.shape, generator=g, device=DEV).to(torch.bfloat16)
+    ds = torch.randn(last.shape, generator=g, device=DEV)
+    grads = torch.autograd.grad((out, last), ins, (do, ds))
+    assert linear_attention_status() != 0
+    for x in (out, *grads[:4]):
+        assert torch.isfinite(x.float()).all() and not x[:, 200:].any()
+    assert torch.isfinite(last).all()
+    for i in (1, 3):
+        assert torch.equal(last[i], state[i] if with_state else torch.zeros_like(last[i]))
+        if with_state:  # through 1 / scale and scale
+            assert torch.allclose(grads[4][i], ds[i], rtol=2.0 ** -22, atol=0)
