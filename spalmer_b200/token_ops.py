@@ -228,7 +228,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
         def pair_of(turns: float) -> float:  # the pair that turns `turns` times over the trained length
             return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim // 2 - 1)
+        # the ramp may end past the last pair, which after a long trained length still turns more than beta_slow times
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
         ramp = ((p / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq / factor * ramp + freq * (1 - ramp)
         mult = 0.1 * math.log(factor) + 1.0
