@@ -554,8 +554,8 @@ int spx_layer_backward(const spx_layer_dims* dims, const spx_packed_weights* wei
  *   (residual_f32: FP32, else BF16), and RMSNorm of h as stored, rounded once:
  *   y = h * w / sqrt(mean(h^2) + eps).  `normed` (BF16 [rows, d]), mx_values
  *   with mx_scales (E4M3 [rows, d] and E8M0 [rows, d / 32], the layout of
- *   spx_mxfp8_quantize_rows, quantised from the FP32 result; d % 32 == 0), or
- *   both.
+ *   spx_mxfp8_quantize_rows, quantised from the FP32 result, where a NaN stays
+ *   a NaN and has no part in its block's scale; d % 32 == 0), or both.
  *   residual NULL: h = hidden, `sum` unused.  Row strides in elements; `sum`
  *   may be the residual itself when its rows are contiguous.  d % 8 == 0,
  *   d <= 16384; 16-byte aligned rows.

@@ -92,6 +92,11 @@ __device__ __forceinline__ void store8(void* base, int64_t at, bool f32, const f
   }
 }
 
+// Two floats -> two E4M3 bytes, to nearest even and at most 448; a NaN stays one (mx_e4m3x2's clamp would make it -448).
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
+}
+
 // Sums over the 32 * WPR threads of a row.  `part` holds
 // [2][rows per CTA][WPR][n]; the two halves alternate from row to row, so one
 // barrier a row is enough.
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
           y[j] += fmaf(fmaf(h[i][j], r_rest, fmaf(h[i][j], r, -p)), wf[j], fmaf(p, wf[j], -y[j]));
         }
         // blocks of 32 = four lanes; all lanes take part in the shuffles (d % 32 == 0, so a block is wholly in or out)
-        float amax = 0.0f;
+        float amax = 0.0f;  // of the numbers: fmaxf passes over a NaN
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
         amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
@@ -224,8 +229,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
         const uint32_t sb = mx_scale_byte(amax);
         const float m = mx_multiplier(sb);
         if (in) {
-          const uint32_t q0 = mx_e4m3x2(y[0] * m, y[1] * m) | (mx_e4m3x2(y[2] * m, y[3] * m) << 16);
-          const uint32_t q1 = mx_e4m3x2(y[4] * m, y[5] * m) | (mx_e4m3x2(y[6] * m, y[7] * m) << 16);
+          const uint32_t q0 = e4m3x2(y[0] * m, y[1] * m) | (e4m3x2(y[2] * m, y[3] * m) << 16);
+          const uint32_t q1 = e4m3x2(y[4] * m, y[5] * m) | (e4m3x2(y[6] * m, y[7] * m) << 16);
           *reinterpret_cast<uint2*>(a.mx_values + row * a.d + c * 8) = make_uint2(q0, q1);
           if ((c & 3) == 0) a.mx_scales[row * (a.d / kMxBlock) + c / 4] = static_cast<uint8_t>(sb);
         }

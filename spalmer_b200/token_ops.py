@@ -182,7 +182,8 @@ def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor, 
     """``(values, scales, summed)`` (with ``rows`` the BF16 rows as a fourth): ``add_rms_norm`` with MXFP8 rows out, quantised
     from the FP32 result: E4M3 bytes [..., d] and one E8M0 byte per 32 elements
     [..., d / 32] (uint8), the layout of ``native.mx_quantize_rows`` and the left
-    operand of ``native.mxfp8_mm_rows``.  d a multiple of 32.  Forward only.
+    operand of ``native.mxfp8_mm_rows``.  A NaN stays one and has no part in its
+    block's scale.  d a multiple of 32.  Forward only.
     """
 
     d = _check_norm(hidden, residual, weight, eps)

@@ -1,0 +1,49 @@
+"""Residual + RMSNorm at its borders: non-finite values in MXFP8 rows, strides and alignment, autograd."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from spalmer_b200 import add_rms_norm_mxfp8
+from spalmer_b200.native import mxfp8_mm_rows, mxfp8_pack_rows
+from tests.test_gpu_token_norm import DEV, EPS, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def _dequantised(values, scales):
+    return values.view(torch.float8_e4m3fn).double() * torch.exp2(scales.double() - 127).repeat_interleave(32, -1)
+
+
+@pytest.mark.parametrize("res", ["none", "bf16", "fp32"])
+@pytest.mark.parametrize("d", [32, 768, 4128])
+def test_mxfp8_rows_keep_nan(d, res):
+    """A row with a NaN, and a column whose weight is one, are NaN in MXFP8 wherever they are in the BF16 rows; the
+    others of a block keep their scale."""
+
+    x, r, w = _inputs(9, d, res)
+    plain = w.clone()
+    x[2, 5] = math.nan
+    x[4] = math.nan
+    w[d - 3] = math.nan
+    values, scales, _, normed = add_rms_norm_mxfp8(x, r, w, EPS, rows=True)
+    got = _dequantised(values, scales)
+    assert torch.isnan(normed[[2, 4]]).all() and torch.isnan(normed[:, d - 3]).all()
+    assert torch.equal(torch.isnan(got), torch.isnan(normed))
+    plain[d - 3] = 0.0  # as small as a block's element can be
+    want = _dequantised(*add_rms_norm_mxfp8(x, r, plain, EPS)[:2])
+    keep = ~torch.isnan(got)
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_mm_rows_keep_nan():
+    """A NaN row of MXFP8 values gives a NaN row of the product, and no other."""
+
+    x, _, w = _inputs(5, 256, "none")
+    x[3, 7] = math.nan
+    weight = torch.randn(48, 256, device=DEV).to(torch.bfloat16)
+    got = mxfp8_mm_rows(*add_rms_norm_mxfp8(x, None, w, EPS)[:2], mxfp8_pack_rows(weight))
+    assert torch.isnan(got[3]).all() and torch.isfinite(got[[0, 1, 2, 4]].float()).all()
