@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) add_norm_kernel(const AddNorm
       if (a.y != nullptr && in) store8(a.y, row * a.d + c * 8, false, y);
       if constexpr (MX) {
         // what r lacks: 1 / sqrt(ms) = r (1 + e / 2), e = 1 - ms r^2
-        const float mr = ms * r, r_rest = 0.5f * r * (fmaf(-mr, r, 1.0f) - fmaf(ms, r, -mr) * r);
+        const float mr = ms * r;
+        const float r_rest = r > 0.0f ? 0.5f * r * (fmaf(-mr, r, 1.0f) - fmaf(ms, r, -mr) * r) : 0.0f;  // r = 0: ms overflowed
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float p = h[i][j] * r;

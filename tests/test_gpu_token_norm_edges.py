@@ -47,3 +47,25 @@ def test_mm_rows_keep_nan():
     weight = torch.randn(48, 256, device=DEV).to(torch.bfloat16)
     got = mxfp8_mm_rows(*add_rms_norm_mxfp8(x, None, w, EPS)[:2], mxfp8_pack_rows(weight))
     assert torch.isnan(got[3]).all() and torch.isfinite(got[[0, 1, 2, 4]].float()).all()
+
+
+@pytest.mark.parametrize("res", ["none", "fp32"])
+def test_mxfp8_rows_past_the_range(res):
+    """A row whose mean square overflows FP32 is zero, as its BF16 row is; a value that is infinite there is a NaN here."""
+
+    x, r, w = _inputs(6, 256, res)
+    x[1] = 1e25
+    if r is not None:
+        r[4] = -1e30
+    x[2, 9] = math.inf  # its own row: NaN there, zero elsewhere
+    w[77] = math.inf
+    values, scales, _, normed = add_rms_norm_mxfp8(x, r, w, EPS, rows=True)
+    got = _dequantised(values, scales)
+    assert torch.equal(torch.isnan(got), ~torch.isfinite(normed))
+    zero = normed == 0
+    assert zero[1].sum() == 255 and zero[2].sum() == 254 and (r is None or zero[4].sum() == 255)
+    assert not got[zero].any()
+    keep = torch.isfinite(normed)
+    # half a step of E4M3 is 2^-4 of a value, or 2^-10 of the scale below its normal range; BF16 adds 2^-8 of a value
+    step = torch.exp2(scales.double() - 127 - 10).repeat_interleave(32, -1)
+    assert torch.all((got - normed.double()).abs()[keep] <= ((2.0 ** -4 + 2.0 ** -7) * normed.double().abs() + step)[keep])
