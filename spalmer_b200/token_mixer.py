@@ -142,11 +142,23 @@ class B200DecoderLayer(nn.Module):
         object.__setattr__(self, "_mxfp8", None)
 
     def pack_mxfp8(self, on: bool = True) -> None:
-        """Serve the first projection in MXFP8 (d_model a multiple of 128): its weight is
-        packed now, and while gradients are off the first norm writes MXFP8 rows for it."""
+        """Serve the first projection in MXFP8 (d_model a multiple of 128): its weight is packed
+        now, and again when it has changed, and while gradients are off the first norm writes
+        MXFP8 rows for it."""
+
+        object.__setattr__(self, "_mxfp8", None)
+        if on:
+            self._packed_projection()
+
+    def _packed_projection(self) -> tuple[Tensor, Tensor, tuple[int, int]]:
+        """The first projection's weight in MXFP8, packed anew where the weight is not the one packed before."""
 
         weight = self.token_mixer.qkv_proj.weight.detach()
-        object.__setattr__(self, "_mxfp8", mxfp8_pack_rows(weight.to(torch.bfloat16)) if on else None)
+        key = (weight.device, weight.dtype, weight.data_ptr(), weight._version)
+        if self._mxfp8 is None or self._mxfp8[0] != key:
+            # the weight is kept with it, so that no other one can come to lie at its address
+            object.__setattr__(self, "_mxfp8", (key, weight, mxfp8_pack_rows(weight.to(torch.bfloat16))))
+        return self._mxfp8[2]
 
     def _enter(self, update: Tensor | None, h: Tensor) -> tuple[Tensor, Tensor | None, Tensor]:
         """(normalised rows, the projection in MXFP8 or None, the stream)."""
@@ -158,7 +170,7 @@ class B200DecoderLayer(nn.Module):
             x, total = add_rms_norm(first, residual, norm.weight, norm.eps)
             return x, None, h if update is None else total
         values, scales, total, x = add_rms_norm_mxfp8(first, residual, norm.weight, norm.eps, rows=True)
-        return x, mxfp8_mm_rows(values, scales, self._mxfp8), h if update is None else total
+        return x, mxfp8_mm_rows(values, scales, self._packed_projection()), h if update is None else total
 
     def _leave(self, t: Tensor, h: Tensor) -> tuple[Tensor, Tensor, ChannelMixerOutput]:
         y, h = add_rms_norm(t, h, self.channel_norm.weight, self.channel_norm.eps)
