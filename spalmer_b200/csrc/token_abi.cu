@@ -16,6 +16,9 @@ size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
+// Elements of 16 bytes, FP32 or BF16: a row stride is a multiple of them.
+int64_t row_unit(int32_t f32) { return f32 != 0 ? 4 : 8; }
+
 // ---------------------------------------------------------------- linear attention
 int check_dims(const spx_linattn_dims* d) {
   if (d == nullptr) return SPX_ERR_INVALID_ARG;
@@ -159,7 +162,7 @@ int spx_add_rmsnorm_rows(const uint16_t* hidden, int64_t ld_hidden, const void* 
   if ((residual == nullptr) != (sum == nullptr)) return SPX_ERR_INVALID_ARG;
   if (ld_hidden < 0 || (residual != nullptr && ld_residual < 0)) return SPX_ERR_INVALID_ARG;
   if (!aligned(hidden) || !aligned(norm_weight) || !aligned(residual) || !aligned(sum) || !aligned(normed) ||
-      !aligned(mx_values) || ld_hidden % 8 != 0 || (residual != nullptr && ld_residual % 8 != 0))
+      !aligned(mx_values) || ld_hidden % 8 != 0 || (residual != nullptr && ld_residual % row_unit(residual_f32) != 0))
     return SPX_ERR_ALIGNMENT;
   AddNormArgs a{};
   a.x = hidden;
@@ -195,7 +198,8 @@ int spx_add_rmsnorm_backward(const void* sum, int64_t ld_sum, int32_t residual_f
     if (d_residual != nullptr && residual_f32 == 0) return SPX_ERR_INVALID_ARG;
     if (ld_sum < 0 || ld_d_normed < 0 || (d_sum != nullptr && ld_d_sum < 0)) return SPX_ERR_INVALID_ARG;
     if (!aligned(sum) || !aligned(norm_weight) || !aligned(d_normed) || !aligned(d_sum) || !aligned(d_hidden) ||
-        !aligned(d_residual) || ld_sum % 8 != 0 || ld_d_normed % 8 != 0 || (d_sum != nullptr && ld_d_sum % 8 != 0))
+        !aligned(d_residual) || ld_sum % row_unit(residual_f32) != 0 || ld_d_normed % 8 != 0 ||
+        (d_sum != nullptr && ld_d_sum % row_unit(residual_f32) != 0))
       return SPX_ERR_ALIGNMENT;
     if (d_weight != nullptr) {
       if (workspace == nullptr || workspace_bytes < spx_add_rmsnorm_backward_workspace(rows, d)) return SPX_ERR_WORKSPACE;

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from spalmer_b200 import add_rms_norm_mxfp8
+from spalmer_b200 import add_rms_norm, add_rms_norm_mxfp8
 from spalmer_b200.native import mxfp8_mm_rows, mxfp8_pack_rows
 from tests.test_gpu_token_norm import DEV, EPS, _inputs
 
@@ -69,3 +69,29 @@ def test_mxfp8_rows_past_the_range(res):
     # half a step of E4M3 is 2^-4 of a value, or 2^-10 of the scale below its normal range; BF16 adds 2^-8 of a value
     step = torch.exp2(scales.double() - 127 - 10).repeat_interleave(32, -1)
     assert torch.all((got - normed.double()).abs()[keep] <= ((2.0 ** -4 + 2.0 ** -7) * normed.double().abs() + step)[keep])
+
+
+@pytest.mark.parametrize("rows,d", [(7, 96), (300, 768)])
+def test_fp32_rows_four_elements_apart(rows, d):
+    """FP32 rows start on 16 bytes where their stride is a multiple of four elements: residual and the sum's gradient."""
+
+    x, r, w = _inputs(rows, d, "fp32")
+    g = torch.Generator(device=DEV).manual_seed(4)
+    dy = torch.randn(rows, d, generator=g, device=DEV).to(torch.bfloat16)
+    ds = torch.randn(rows, d, generator=g, device=DEV)
+
+    def apart(t):
+        wide = torch.full((rows, d + 4), math.nan, device=DEV)
+        wide[:, :d] = t
+        return wide[:, :d]
+
+    def call(r, ds):
+        ins = [t.detach().requires_grad_(True) for t in (x, r, w)]
+        y, total = add_rms_norm(*ins, EPS)
+        return y, total, *torch.autograd.grad((y, total), ins, (dy, ds))
+
+    for got, want in zip(call(apart(r), apart(ds)), call(r, ds)):
+        assert torch.equal(got, want)
+    for got, want in zip(add_rms_norm_mxfp8(x, apart(r), w, EPS),
+                         add_rms_norm_mxfp8(x, r, w, EPS)):
+        assert torch.equal(got, want)
