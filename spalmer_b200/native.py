@@ -89,6 +89,13 @@ def mxfp8_mm_nt(left: Tensor, right_rows: Tensor) -> Tensor:
     return out
 
 
+def _dense(t: Tensor) -> Tensor:
+    """``t`` contiguous and on 16 bytes (a copy only if it must be)."""
+
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def mxfp8_pack_rows(rows: Tensor) -> tuple[Tensor, Tensor, tuple[int, int]]:
     """A weight ``[n, k]`` packed once as the right operand of ``mxfp8_mm_rows``
     (k a multiple of 128): E4M3 values, scale atoms and the shape."""
@@ -102,7 +109,7 @@ def mxfp8_pack_rows(rows: Tensor) -> tuple[Tensor, Tensor, tuple[int, int]]:
     sizes = _lib.ctypes.c_size_t(), _lib.ctypes.c_size_t()
     _lib.check(lib.spx_mxfp8_packed_sizes(n, k, *sizes), "spx_mxfp8_packed_sizes")
     values, scales = (torch.empty(v.value, dtype=torch.uint8, device=rows.device) for v in sizes)
-    src = rows.detach().contiguous()
+    src = _dense(rows.detach())
     with torch.cuda.device(rows.device):
         stream = torch.cuda.current_stream(rows.device).cuda_stream
         _lib.check(lib.spx_mxfp8_pack_rows(src.data_ptr(), n, k, values.data_ptr(), scales.data_ptr(), stream),
@@ -123,7 +130,7 @@ def mxfp8_mm_rows(values: Tensor, scales: Tensor, packed: tuple[Tensor, Tensor, 
         raise ValueError(f"values must be [..., {k}] and scales [..., {k // 32}]")
     if scales.device != values.device or weight.device != values.device:
         raise NativeExpertPrecisionError("native MXFP8 GEMM operands must share one device")
-    v, s = values.contiguous(), scales.contiguous()
+    v, s = _dense(values), _dense(scales)
     m = v.numel() // k
     out = torch.empty(*values.shape[:-1], n, dtype=torch.bfloat16, device=values.device)
     lib = _lib.load()

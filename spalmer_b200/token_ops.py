@@ -22,6 +22,7 @@ import torch
 from torch import Tensor
 
 from spalmer_b200 import _lib
+from spalmer_b200.native import _dense
 
 _MAX_HEAD_DIM = 128
 
@@ -70,9 +71,7 @@ def _rows(t: Tensor, d: int, item: int) -> Tensor:
     else:
         r = t.reshape(-1, d)
     if r.shape[0] and (r.stride(1) != 1 or (r.stride(0) * item) % 16 or r.data_ptr() % 16):
-        r = r.contiguous()
-        if r.data_ptr() % 16:
-            r = r.clone()
+        r = _dense(r)
     return r
 
 
@@ -105,7 +104,7 @@ def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: 
         f32 = residual.dtype == _F32
         r = _rows(residual, d, 4 if f32 else 2)
         total = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    w = weight.contiguous()
+    w = _dense(weight)
     if rows:
         out = torch.empty_like(hidden, memory_format=torch.contiguous_format)
     if mxfp8:
@@ -137,7 +136,7 @@ class _AddRMSNorm(torch.autograd.Function):
             d_out = torch.zeros(total.shape, dtype=_BF16, device=dev)
         f32 = total.dtype == _F32
         item = 4 if f32 else 2
-        h, dy = _rows(total, d, item), _rows(d_out, d, 2)
+        h, dy, w = _rows(total, d, item), _rows(d_out, d, 2), _dense(weight)
         ds = None if d_total is None else _rows(d_total, d, item)
         n = h.shape[0]
         d_hidden = torch.empty_like(d_out, memory_format=torch.contiguous_format)
@@ -148,7 +147,7 @@ class _AddRMSNorm(torch.autograd.Function):
             d_weight = torch.empty_like(weight, memory_format=torch.contiguous_format)
             nbytes = _lib.load().spx_add_rmsnorm_backward_workspace(n, d)
             ws = weight.new_empty(nbytes, dtype=torch.uint8)
-        _call("spx_add_rmsnorm_backward", dev, h.data_ptr(), h.stride(0), f32, weight.contiguous().data_ptr(), ctx.eps,
+        _call("spx_add_rmsnorm_backward", dev, h.data_ptr(), h.stride(0), f32, w.data_ptr(), ctx.eps,
               dy.data_ptr(), dy.stride(0), _ptr(ds), 0 if ds is None else ds.stride(0), n, d, d_hidden.data_ptr(),
               _ptr(d_residual), _ptr(d_weight), _ptr(ws), nbytes)
         d_res = None
@@ -347,9 +346,7 @@ def _aligned_heads(t: Tensor) -> Tensor:
     sizes, strides = t.shape, t.stride()
     if (t.data_ptr() % 16 or strides[-1] != 1
             or any(n > 1 and (st % 8 or st <= 0) for st, n in zip(strides[:-1], sizes[:-1]))):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+        t = _dense(t)
     return t
 
 
@@ -403,7 +400,7 @@ class _LinearAttention(torch.autograd.Function):
         if d_out is None:
             d_out = torch.zeros(*q.shape[:3], v.shape[3], dtype=torch.bfloat16, device=dev)
         d_out = _aligned_heads(d_out.to(torch.bfloat16))
-        d_last = None if d_last is None else d_last.float().contiguous()
+        d_last = None if d_last is None else _dense(d_last.float())
         dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
         dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
         d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
@@ -476,7 +473,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scal
         want = (n, q.shape[2], q.shape[3], v.shape[3])
         if tuple(initial_state.shape) != want:
             raise ValueError(f"initial_state must be {list(want)}")
-        initial_state = initial_state.contiguous()
+        initial_state = _dense(initial_state)
     q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         return _LinearAttention.apply(q, k, v, log_decay, initial_state, cu_seqlens, scale, return_state)

@@ -134,3 +134,25 @@ def test_unsound_sequences_are_empty_ones(dirty, H, kv, with_state):
         assert torch.equal(last[i], state[i] if with_state else torch.zeros_like(last[i]))
         if with_state:  # through 1 / scale and scale
             assert torch.allclose(grads[4][i], ds[i], rtol=2.0 ** -22, atol=0)
+
+
+def test_states_off_sixteen_bytes():
+    """An initial state, and a last state's gradient, one element behind a 16-byte boundary."""
+
+    q, k, v, a, state = _inputs(2, 150, 2, 1, 64, 72, init=True)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    ds = torch.randn(state.shape, generator=g, device=DEV)
+
+    def off(t):
+        moved = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        moved.copy_(t)
+        assert moved.data_ptr() % 16
+        return moved
+
+    def call(move):
+        ins = [t.detach().requires_grad_(True) for t in (q, k, v, a, move(state))]
+        out, last = linear_attention(*ins[:4], initial_state=ins[4], return_state=True)
+        return out, last, *torch.autograd.grad((out, last), ins, (torch.ones_like(out), move(ds)))
+
+    for got, want in zip(call(off), call(lambda t: t)):
+        assert torch.equal(got, want)

@@ -95,3 +95,38 @@ def test_fp32_rows_four_elements_apart(rows, d):
     for got, want in zip(add_rms_norm_mxfp8(x, apart(r), w, EPS),
                          add_rms_norm_mxfp8(x, r, w, EPS)):
         assert torch.equal(got, want)
+
+
+def _off(t):
+    """The same values one element behind a 16-byte boundary."""
+
+    moved = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    moved.copy_(t)
+    assert moved.data_ptr() % 16
+    return moved
+
+
+@pytest.mark.parametrize("res", ["none", "bf16", "fp32"])
+def test_operands_off_sixteen_bytes(res):
+    x, r, w = _inputs(33, 256, res)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    dy = torch.randn(33, 256, generator=g, device=DEV).to(torch.bfloat16)
+
+    def call(move):
+        ins = [move(t).detach().requires_grad_(True) for t in (x, r, w) if t is not None]
+        y, total = add_rms_norm(ins[0], ins[1] if r is not None else None, ins[-1], EPS)
+        return y, total, *torch.autograd.grad(y, ins, move(dy))
+
+    for got, want in zip(call(_off), call(lambda t: t)):
+        assert torch.equal(got, want)
+    rows = None if r is None else _off(r)
+    for got, want in zip(add_rms_norm_mxfp8(_off(x), rows, _off(w), EPS), add_rms_norm_mxfp8(x, r, w, EPS)):
+        assert torch.equal(got, want)
+
+
+def test_quantised_operands_off_sixteen_bytes():
+    x, _, w = _inputs(33, 256, "none")
+    weight = torch.randn(48, 256, device=DEV).to(torch.bfloat16)
+    values, scales, _ = add_rms_norm_mxfp8(x, None, w, EPS)
+    want = mxfp8_mm_rows(values, scales, mxfp8_pack_rows(weight))
+    assert torch.equal(mxfp8_mm_rows(_off(values), _off(scales), mxfp8_pack_rows(_off(weight))), want)
