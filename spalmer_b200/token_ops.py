@@ -16,6 +16,7 @@ tensors' device, without host synchronisation.  The reference's block
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -58,6 +59,38 @@ def _require(tensor: Tensor, name: str, dtype: torch.dtype | tuple, device: torc
 
 def _ptr(t: Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """The first ``n`` tensors, gradients that depend on the others; a derivative of them raises instead of
+    leaving their terms out."""
+
+    @staticmethod
+    def forward(ctx, name, n, *tensors):
+        ctx.name = name
+        return tuple(g.view_as(g) for g in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError(f"{ctx.name} implements first derivatives only")
+
+
+def _first_order(name: str):
+    """Of an autograd function's backward: it records nothing, and where a graph of it is wanted, that graph raises."""
+
+    def wrap(backward):
+        @functools.wraps(backward)
+        def wrapped(ctx, *d_outs):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *d_outs)
+            with torch.no_grad():
+                out = backward(ctx, *d_outs)
+            there = [g for g in out if g is not None]
+            needs = [t for t in (*d_outs, *ctx.saved_tensors) if t is not None and t.requires_grad]
+            marked = iter(_NoSecondDerivative.apply(name, len(there), *there, *needs) if needs else there)
+            return tuple(None if g is None else next(marked) for g in out)
+        return wrapped
+    return wrap
 
 
 # ---------------------------------------------------------------- residual + RMSNorm
@@ -128,6 +161,7 @@ class _AddRMSNorm(torch.autograd.Function):
         return out, total
 
     @staticmethod
+    @_first_order("add_rms_norm")
     def backward(ctx, d_out, d_total):
         total, weight = ctx.saved_tensors
         d = weight.shape[0]
@@ -274,6 +308,7 @@ class _Rotary(torch.autograd.Function):
         return _rotate(q, k, positions, frequencies, interleaved, factor, False)
 
     @staticmethod
+    @_first_order("rotary_embed")
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
         interleaved, factor = ctx.args
@@ -393,6 +428,7 @@ class _LinearAttention(torch.autograd.Function):
         return _attend(q, k, v, g, cu, state, scale, want_state)
 
     @staticmethod
+    @_first_order("linear_attention")
     def backward(ctx, d_out, d_last):
         q, k, v, g, state, cu = ctx.saved_tensors
         dev = q.device
