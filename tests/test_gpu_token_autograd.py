@@ -4,8 +4,16 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from spalmer_b200 import add_rms_norm, linear_attention, rotary_embed, rotary_frequencies
+from spalmer_b200 import (
+    add_rms_norm,
+    add_rms_norm_mxfp8,
+    linear_attention,
+    linear_attention_step,
+    rotary_embed,
+    rotary_frequencies,
+)
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -57,3 +65,26 @@ def test_second_derivatives_raise(name):
     else:
         with pytest.raises(NotImplementedError, match="first derivatives"):
             (got[0].float().square().sum() + ins[0].float().square().sum()).backward()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name", [*NAMES, "add_rms_norm_mxfp8", "linear_attention_step"])
+def test_tangents_are_refused(name, requires_grad):
+    """Whichever input has one; a call without one works beside them."""
+
+    calls = _calls() | {
+        "add_rms_norm_mxfp8": (add_rms_norm_mxfp8, (_bf16(6, 64), _bf16(6, 64, seed=1), _bf16(64))),
+        "linear_attention_step": (linear_attention_step, (_bf16(2, 2, 64), _bf16(2, 1, 64), _bf16(2, 1, 64),
+                                                          -torch.rand(2, 2, device=DEV),
+                                                          torch.zeros(2, 2, 64, 64, device=DEV))),
+    }
+    fn, inputs = calls[name]
+    if requires_grad and name not in NAMES:
+        pytest.skip("forward only")
+    for i in range(len(inputs)):
+        with forward_ad.dual_level():
+            fn(*inputs)
+            ins = [t.clone().requires_grad_(requires_grad) for t in inputs]
+            ins[i] = forward_ad.make_dual(ins[i], torch.ones_like(ins[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(*ins)
