@@ -565,6 +565,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     _call("spx_linear_attention_step", dev, _step_heads(q), _step_heads(k), _step_heads(v),
           _lib.Decays(log_decay.data_ptr(), log_decay.stride(0), 0, log_decay.stride(1)), log_decay.dtype == _F32, B, H,
           k.shape[1], dk, dv, scale, state.data_ptr(), state.shape[0], _ptr(slots), out.data_ptr())
+    torch.autograd.graph.increment_version(state)  # written in place: a backward pass that kept it has to notice
     return out
 
 

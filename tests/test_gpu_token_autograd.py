@@ -88,3 +88,21 @@ def test_tangents_are_refused(name, requires_grad):
             ins[i] = forward_ad.make_dual(ins[i], torch.ones_like(ins[i]))
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 fn(*ins)
+
+
+def test_a_step_is_a_change_of_its_state():
+    """A state kept for a backward pass and then stepped is noticed; one that only inference has seen may be stepped."""
+
+    _, (q, k, v, a, state) = _calls()["linear_attention"]
+    q = q.clone().requires_grad_(True)
+    out, _ = linear_attention(q, k, v, a, initial_state=state)
+    before = state._version
+    with torch.no_grad():
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], a[:, 0], state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+    with torch.inference_mode():
+        cache = torch.zeros_like(state)
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], a[:, 0], cache)
+        assert cache.any()
