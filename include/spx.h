@@ -620,6 +620,11 @@ typedef struct spx_decays {
   int64_t batch_stride, token_stride, head_stride;
 } spx_decays;
 
+/* A status word that libspx has on the current device, zero at first, for
+ * callers that keep none of their own; spx_workspace_status reads and clears
+ * it.  May be called, the first time too, while a stream is being captured. */
+int spx_token_status_word(int** word);
+
 size_t spx_linear_attention_workspace(const spx_linattn_dims* dims);
 /* out: BF16 [batch, seq_len, heads, value_dim] contiguous; final_state may be NULL. */
 int spx_linear_attention(const spx_linattn_dims* dims, const spx_heads* q, const spx_heads* k, const spx_heads* v,

@@ -80,6 +80,7 @@ EXPORTED = (
     "spx_add_rmsnorm_backward_workspace",
     "spx_add_rmsnorm_backward",
     "spx_rotary",
+    "spx_token_status_word",
     "spx_linear_attention_workspace",
     "spx_linear_attention",
     "spx_linear_attention_backward_workspace",
@@ -376,6 +377,7 @@ def load() -> ctypes.CDLL:
             [P(Heads), ctypes.c_int32, P(Heads), ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _vp,
              ctypes.c_int32, ctypes.c_int64, _vp, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp],
         ),
+        "spx_token_status_word": (ctypes.c_int, [P(_vp)]),
         "spx_linear_attention_workspace": (ctypes.c_size_t, [P(LinAttnDims)]),
         "spx_linear_attention": (
             ctypes.c_int,

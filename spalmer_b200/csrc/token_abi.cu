@@ -10,6 +10,8 @@ using namespace spx;
 
 namespace {
 
+__device__ int g_token_status;  // of callers without a word of their own
+
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
@@ -256,6 +258,19 @@ int spx_rotary(const spx_heads* q, int32_t q_heads, const spx_heads* k, int32_t 
   a.inverse = inverse != 0 ? 1 : 0;
   a.factor = factor;
   return launch_rotary(a, as_stream(stream));
+}
+
+int spx_token_status_word(int** word) {
+  if (word == nullptr) return SPX_ERR_INVALID_ARG;
+  // the first use on a device loads the variable, which a capture under way would not allow in its own mode
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return SPX_ERR_CUDA;
+  void* p = nullptr;
+  const cudaError_t got = cudaGetSymbolAddress(&p, g_token_status);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (got != cudaSuccess || p == nullptr) return SPX_ERR_CUDA;
+  *word = static_cast<int*>(p);
+  return SPX_OK;
 }
 
 size_t spx_linear_attention_workspace(const spx_linattn_dims* dims) {

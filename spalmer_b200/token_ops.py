@@ -362,13 +362,18 @@ def rotary_embed(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Te
 
 
 # ---------------------------------------------------------------- linear attention
-_status: dict[torch.device, Tensor] = {}
+_status: dict[torch.device, int] = {}
 
 
-def _status_word(device: torch.device) -> Tensor:
+def _status_word(device: torch.device) -> int:
+    """The address of libspx's status word on ``device``: not memory of PyTorch's, which a graph capture would make its own."""
+
     word = _status.get(device)
     if word is None:
-        word = _status[device] = torch.zeros(4, dtype=torch.int32, device=device)
+        at = _lib.ctypes.c_void_p()
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().spx_token_status_word(at), "spx_token_status_word")
+        word = _status[device] = at.value
     return word
 
 
@@ -379,10 +384,11 @@ def linear_attention_status(device: torch.device | str | int | None = None, clea
     word = _status.get(dev)
     if word is None:
         return 0
-    value = int(word[0].item())
-    if clear:
-        word.zero_()
-    return value
+    value = _lib.ctypes.c_int()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().spx_workspace_status(word, value, int(clear), _raw_stream(dev.index)),
+                   "spx_workspace_status")
+    return value.value
 
 
 def _aligned_heads(t: Tensor) -> Tensor:
@@ -427,7 +433,7 @@ def _attend(q: Tensor, k: Tensor, v: Tensor, g: Tensor, cu: Tensor | None, state
     nbytes = _lib.load().spx_linear_attention_workspace(dims)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call("spx_linear_attention", dev, dims, _heads(q), _heads(k), _heads(v), _decays(g), _ptr(cu), _ptr(state),
-          out.data_ptr(), _ptr(last), _ptr(ws), nbytes, _status_word(dev).data_ptr())
+          out.data_ptr(), _ptr(last), _ptr(ws), nbytes, _status_word(dev))
     return out, last
 
 
@@ -456,7 +462,7 @@ class _LinearAttention(torch.autograd.Function):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _call("spx_linear_attention_backward", dev, dims, _heads(q), _heads(k), _heads(v), _decays(g), _ptr(cu),
               _ptr(state), _heads(d_out), _ptr(d_last), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
-              _ptr(d_state), _ptr(ws), nbytes, _status_word(dev).data_ptr())
+              _ptr(d_state), _ptr(ws), nbytes, _status_word(dev))
         return dq, dk, dv, dg, d_state, None, None, None
 
 

@@ -3,11 +3,14 @@
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
 from spalmer_b200 import _lib, linear_attention, linear_attention_status
+from tests.conftest import ROOT
 from tests.test_gpu_linear_attention import DEV, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -156,3 +159,35 @@ def test_states_off_sixteen_bytes():
 
     for got, want in zip(call(off), call(lambda t: t)):
         assert torch.equal(got, want)
+
+
+FIRST_CALL = """
+import torch
+from spalmer_b200 import linear_attention, linear_attention_status
+
+q, k, v = (torch.randn(1, 300, 2, 64, device="cuda").to(torch.bfloat16) for _ in range(3))
+a = -torch.rand(1, 300, 2, device="cuda")
+cu = torch.tensor([0, 100, 50, 300], device="cuda", dtype=torch.int32)  # sequence 1 runs backwards
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, _ = linear_attention(q, k, v, a, cu_seqlens=cu)
+graph.replay()
+torch.cuda.synchronize()
+cu.copy_(torch.tensor([0, 100, 200, 300]))
+graph.replay()
+torch.cuda.synchronize()
+assert linear_attention_status(clear=False) != 0, "a later replay has cleared the status"
+assert linear_attention_status() != 0 and linear_attention_status() == 0
+graph.replay()
+torch.cuda.synchronize()
+assert linear_attention_status() == 0
+want, _ = linear_attention(q, k, v, a, cu_seqlens=cu)
+assert torch.equal(out, want)
+"""
+
+
+def test_first_call_inside_a_graph():
+    """The status word outlives a graph whose capture made the first call, and no replay clears it."""
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
