@@ -11,7 +11,7 @@ import torch
 
 from spalmer_b200 import _lib, linear_attention, linear_attention_status
 from tests.conftest import ROOT
-from tests.test_gpu_linear_attention import DEV, _inputs
+from tests.test_gpu_linear_attention import DEV, _check_forward, _check_gradients, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +191,40 @@ def test_first_call_inside_a_graph():
 
     done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=ROOT, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 72)])
+@pytest.mark.parametrize("at", [0, 1, 31, 40, 70, 127, 128, 250, 299])
+def test_a_nan_decay_stays_on_its_side(at, dk, dv):
+    """The decay of a token is between it and those before: they keep their outputs and d q, it and those after it
+    their d k and d v.  They are those of a token that forgets everything, whose block takes the same sums."""
+
+    q, k, v, a, _ = _inputs(2, 300, 2, 2, dk, dv)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    do = torch.randn(2, 300, 2, dv, generator=g, device=DEV).to(torch.bfloat16)
+
+    def call(a):
+        ins = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = linear_attention(*ins, a)[0]
+        return out.detach(), *torch.autograd.grad(out, ins, do)
+
+    spoilt, forgets = a.clone(), a.clone()
+    spoilt[:, at], forgets[:, at] = math.nan, -math.inf
+    for i, (got, want) in enumerate(zip(call(spoilt), call(forgets))):
+        keep = slice(None, at) if i < 2 else slice(at, None)
+        assert torch.isfinite(want.float()).all() and torch.equal(got[:, keep], want[:, keep])
+        if at:
+            assert torch.isnan(got[:, at:] if i < 2 else got[:, :at]).any()
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 72)])
+@pytest.mark.parametrize("resets", [(27,), (0, 5, 9, 30), tuple(range(26)), tuple(range(0, 32, 3))])
+@pytest.mark.parametrize("strong", [-math.inf, -150.0, -60.0])
+def test_many_strong_decays_in_a_block(strong, resets, dk, dv):
+    """Tokens that forget (nearly) everything, up to 26 of a block of 32, with mild ones after and between them."""
+
+    q, k, v, a, state = _inputs(1, 300, 2, 1, dk, dv, init=True, span=(50.0, 300.0))
+    for block in (0, 64, 160, 224, 256):
+        a[:, [block + r for r in resets]] = strong
+    _check_forward(q, k, v, a, state)
+    _check_gradients(q, k, v, a, None)  # the first state's gradient has passed all of them: below FP32's range
