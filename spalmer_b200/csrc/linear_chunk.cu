@@ -1371,7 +1371,7 @@ int launch_la_chunk(const LaArgs& a, bool precise, void* workspace, cudaStream_t
   if (lanes == 0) return SPX_OK;
   const int sms = device_sm_count();
   c.nseg = segments_for(a, lanes, sms);
-  if (lanes * c.nseg > 0x7FFFFFFF) return SPX_ERR_UNSUPPORTED;
+  if (lanes * c.nseg > 0x7FFFFFFF - sms) return SPX_ERR_UNSUPPORTED;  // a step past the last item is an int too
   c.la = a;
   int dkb = 1;
   for (int i = 0; i < a.njobs; ++i) {
