@@ -9,7 +9,7 @@ import sys
 import pytest
 import torch
 
-from spalmer_b200 import _lib, linear_attention, linear_attention_status
+from spalmer_b200 import _lib, linear_attention, linear_attention_status, linear_attention_step
 from tests.conftest import ROOT
 from tests.test_gpu_linear_attention import DEV, _check_forward, _check_gradients, _inputs
 
@@ -228,3 +228,54 @@ def test_many_strong_decays_in_a_block(strong, resets, dk, dv):
         a[:, [block + r for r in resets]] = strong
     _check_forward(q, k, v, a, state)
     _check_gradients(q, k, v, a, None)  # the first state's gradient has passed all of them: below FP32's range
+
+
+def _odd_views(q, k, v):
+    """The same values as views of one leaf: off 16 bytes, and no stride of tokens or heads a multiple of 16 bytes."""
+
+    lead, width = q.shape[:-2], max(q.shape[-1], v.shape[-1])
+    heads = q.shape[-2] + 2 * k.shape[-2]
+    wide = torch.zeros(math.prod(lead) * heads * (width + 1) + 3, device=DEV, dtype=torch.bfloat16)
+    rows = wide[3:].view(*lead, heads, width + 1)
+    at = 0
+    for t in (q, k, v):
+        rows[..., at:at + t.shape[-2], :t.shape[-1]] = t
+        at += t.shape[-2]
+    wide.requires_grad_(True)
+    rows = wide[3:].view(*lead, heads, width + 1)
+    at, views = 0, []
+    for t in (q, k, v):
+        view = rows[..., at:at + t.shape[-2], :t.shape[-1]]
+        assert torch.equal(view, t) and view.data_ptr() % 16 and view.stride(-2) % 8
+        views.append(view)
+        at += t.shape[-2]
+    return wide, views
+
+
+@pytest.mark.parametrize("B,T,H,kv,dk,dv", [(2, 300, 4, 2, 64, 64), (1, 5, 3, 3, 40, 128), (2, 150, 2, 1, 128, 72)])
+def test_misaligned_views(B, T, H, kv, dk, dv):
+    q, k, v, a, state = _inputs(B, T, H, kv, dk, dv, init=True)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    do = torch.randn(B, T, H, dv, generator=g, device=DEV).to(torch.bfloat16)
+    ins = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out, last = linear_attention(*ins, a, initial_state=state, return_state=True)
+    want = torch.autograd.grad(out, ins, do)
+    wide, views = _odd_views(q, k, v)
+    odd = torch.empty(do.numel() + 1, dtype=do.dtype, device=DEV)[1:].view(do.shape).copy_(do)
+    out2, last2 = linear_attention(*views, a, initial_state=state, return_state=True)
+    assert torch.equal(out2, out) and torch.equal(last2, last)
+    for x, y in zip(torch.autograd.grad(out2, views, odd, retain_graph=True), want):
+        assert torch.equal(x, y)
+    (whole,) = torch.autograd.grad(out2, wide, odd)
+    assert torch.equal(whole.sort().values, torch.cat([*(y.flatten() for y in want), whole.new_zeros(
+        whole.numel() - sum(y.numel() for y in want))]).sort().values)
+
+
+def test_misaligned_views_of_a_step():
+    q, k, v, a, state = _inputs(1, 5, 4, 2, 64, 72, n=5, init=True)
+    q, k, v, a = q[0], k[0], v[0], a[0]
+    _, views = _odd_views(q, k, v)
+    other = state.clone()
+    want = linear_attention_step(q, k, v, a, state)
+    assert torch.equal(linear_attention_step(*(t.detach() for t in views), a, other), want)
+    assert torch.equal(other, state)
