@@ -61,8 +61,7 @@ def _require(tensor: Tensor, name: str, dtype: torch.dtype | tuple, device: torc
 def _refuse_tangents(name: str, *tensors: Tensor | None) -> None:
     """Forward-mode derivatives are not implemented; a dual tensor does not require grad and would lose its tangent."""
 
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                              for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
@@ -146,7 +145,7 @@ def _norm_forward(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: 
         f32 = residual.dtype == _F32
         r = _rows(residual, d, 4 if f32 else 2)
         total = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    w = _dense(weight)
+    w = _dense(weight) if weight.data_ptr() % 16 or not weight.is_contiguous() else weight
     if rows:
         out = torch.empty_like(hidden, memory_format=torch.contiguous_format)
     if mxfp8:
@@ -211,7 +210,8 @@ def add_rms_norm(hidden: Tensor, residual: Tensor | None, weight: Tensor, eps: f
     """
 
     _check_norm(hidden, residual, weight, eps)
-    _refuse_tangents("add_rms_norm", hidden, residual, weight)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("add_rms_norm", hidden, residual, weight)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         normed, summed = _AddRMSNorm.apply(hidden, residual, weight, float(eps))
@@ -232,7 +232,8 @@ def add_rms_norm_mxfp8(hidden: Tensor, residual: Tensor | None, weight: Tensor, 
     d = _check_norm(hidden, residual, weight, eps)
     if d % 32:
         raise ValueError("the row length must be a multiple of the block size 32")
-    _refuse_tangents("add_rms_norm_mxfp8", hidden, residual, weight)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("add_rms_norm_mxfp8", hidden, residual, weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, residual, weight)):
         raise NotImplementedError("add_rms_norm_mxfp8 implements the forward pass only")
     normed, values, scales, summed = _norm_forward(hidden, residual, weight, float(eps), rows, True)
@@ -355,7 +356,8 @@ def rotary_embed(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Te
     tokens = math.prod(q.shape[:-2])
     if positions.numel() not in (tokens, q.shape[-3]) or (positions.numel() != tokens and positions.ndim != 1):
         raise ValueError(f"positions must hold one position per token ({tokens}, or {q.shape[-3]} shared by the batch)")
-    _refuse_tangents("rotary_embed", q, k)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("rotary_embed", q, k)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, positions, frequencies, bool(interleaved), float(factor))
     return _rotate(q, k, positions, frequencies, bool(interleaved), float(factor), False)
@@ -528,7 +530,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scal
         if tuple(initial_state.shape) != want:
             raise ValueError(f"initial_state must be {list(want)}")
         initial_state = _dense(initial_state)
-    _refuse_tangents("linear_attention", q, k, v, log_decay, initial_state)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("linear_attention", q, k, v, log_decay, initial_state)
     q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         return _LinearAttention.apply(q, k, v, log_decay, initial_state, cu_seqlens, scale, return_state)
@@ -562,7 +565,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if slots.shape != (B,):
             raise ValueError(f"slots must be [{B}]")
         slots = slots.contiguous()
-    _refuse_tangents("linear_attention_step", q, k, v, log_decay, state)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("linear_attention_step", q, k, v, log_decay, state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
         raise NotImplementedError("linear_attention_step implements the forward pass only")
