@@ -18,10 +18,12 @@
 // Operand precision.  a, b, c are exact BF16.  What is not is split into BF16
 // parts that are multiplied one after another into the same FP32 accumulator:
 //   c scaled by its decay (into the state): three parts where a caller keeps the
-//     last state (exact), else two (2^-18);
+//     last state (exact), else two (2^-18; the first state's gradient too);
 //   the decayed a . b matrix and the state (into out): one part in the forward
-//     pass, whose output is rounded to BF16 as coarsely, two in the gradients,
-//     because d decay is a long sum of q . dq - k . dk that cancels.
+//     pass, whose output is rounded to BF16 as coarsely (2.3e-3 from 64 bits, one
+//     rounding alone 1.7e-3; two parts: 158 us and not 133 for 65,536 tokens of 12
+//     heads of 64, and no room for them beside three parts of c at 128 wide), two in
+//     the gradients, because d decay is a long sum of q . dq - k . dk that cancels.
 //
 // Decay factors are exponentials of sums <= 0, never quotients, so no decay
 // overflows: inside a 32-token block the sum between two tokens, across blocks a
@@ -30,8 +32,8 @@
 // from an edge are taken directly, so that a token that forgets everything costs the
 // other blocks and the state no digits, and a NaN reaches no token on its other side.
 // Between two tokens of one block the sum is the difference of two such sums and off by
-// 2^-24 of them: factors by 3e-5 at most after one token that forgets everything, 4e-4
-// after 26 of them in a block, 6e-6 in a block that decays by less than 2^-100.
+// about 2^-24 of them: factors by 3e-5 at most in a block that decays by 2^-150 in all,
+// 4e-4 after 26 tokens that forget everything.
 //
 // How lanes meet SMs.  Too few lanes: the sequence is cut into segments; a pass
 // over b and c alone gives each segment's state from zero, a small kernel chains
@@ -42,12 +44,12 @@
 // the later steps 72).
 //
 // What bounds it: neither HBM nor the tensor cores, but instructions.  A chunk of
-// 64-wide heads takes about 3,600 cycles (gradients 4,300) in which four schedulers
-// issue 55% of the time and wait for instruction fetch in a quarter of the rest: a
-// dozen roles run at once, so that their code has to stay small, and unrolling or
-// prefetching more made every loop slower.  65,536 tokens of 12 heads of 64: forward
-// 140 us (403 MB, 2.9 TB/s), the three gradients 424 us.  8,190 tokens of 16 heads of
-// 128 over 4 shared ones: 87 and 211 us.
+// 64-wide heads takes about 6,000 cycles, in the gradients too (1.75 GHz under this
+// kernel), in which four schedulers issue 48 to 57% of the time and wait for
+// instruction fetch in a quarter of the rest: a dozen roles run at once, so that their
+// code has to stay small, and unrolling or prefetching more made every loop slower.
+// 65,536 tokens of 12 heads of 64: forward 142 us (403 MB, 2.8 TB/s), the three
+// gradients 431 us.  8,190 tokens of 16 heads of 128 over 4 shared ones: 88 and 213 us.
 //
 // Warps: 0-7 the decayed a . b matrix (TMEM -> registers -> TMEM operand), 8-15
 // scaled c, 16-19 the state, 20-27 the epilogue, 28 and 31 TMA, 29 MMA, 30

@@ -508,7 +508,15 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scal
     fixed length, say) have zero outputs and gradients.  An entry that is out of
     order makes its sequence an empty one and shows in ``linear_attention_status``.  ``initial_state`` and the returned last state
     are FP32 [B or n, heads, key_dim, value_dim].  Nothing passes from one
-    sequence to another, non-finite values included.
+    sequence to another, non-finite values included; inside one, a value that is
+    not finite may reach outputs up to 127 tokens before it.
+
+    Products are summed and states kept in FP32.  In packed rows, and batched ones of
+    more than eight tokens, the decayed ``q . k`` and the state are rounded to BF16
+    where they are multiplied into ``out`` (2.3e-3 from the exact output in the mean,
+    against 1.7e-3 of its own rounding), and into gradients with twice the digits;
+    ``out`` may differ in its last bit with ``return_state``, as a state that is
+    handed out has FP32's digits.
 
     Differentiable in q, k, v, log_decay and initial_state, through the output
     and the last state; the backward keeps nothing but the inputs.
